@@ -59,7 +59,7 @@ def _log_int(rng, lo, hi):
 
 def draw(rng):
     if rng.random() < 0.3:
-        rows, cols = _log_int(rng, 1, 8192), _log_int(rng, 1, 25088)
+        rows, cols = _log_int(rng, 1, 8192), _log_int(rng, 256, 25088)
         return {"op": "dropout", "back": rng.random() < 0.5, "dtype": rng.choice(["bf16", "fp32"]), "rows": rows, "cols": cols,
                 "pitch": cols + rng.choice([0, 0, 1, 8, 40]), "p": rng.choice([0.0, 0.1, 0.25, 0.5, 0.9])}
     grad = rng.random() < 0.6
@@ -72,7 +72,7 @@ def draw(rng):
         if n * d * v <= budget and n * v <= 8192 * 65536 and v * d <= 65536 * 4096:
             break
     return {"op": "xent", "grad": grad, "dtype": dtype, "n": n, "d": d, "v": v, "bias": rng.random() < 0.5,
-            "reduction": rng.choice(["mean", "sum", "none"]), "ignored": rng.choice([0.0, 0.0, 0.1, 0.5]),
+            "reduction": rng.choice(["mean", "sum", "none"]), "ignored": rng.choice([0.0, 0.0, 0.1, 0.5]) if n >= 64 else 0.0,
             "smoothing": rng.choice([0.0, 0.0, 0.1])}
 
 
