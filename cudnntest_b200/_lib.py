@@ -17,8 +17,10 @@ NCHW, NHWC, CHWN = 0, 1, 2
 FP32, TF32, BF16, FP32X3 = 0, 1, 2, 3
 OPERAND_AUTO, OPERAND_BF16, OPERAND_F16 = 0, 1, 2
 OUT_SAME, OUT_FP32, OUT_BF16 = 0, 1, 2
+MEAN, SUM, NONE = 0, 1, 2
 OK, E_BADARG, E_UNSUPPORTED, E_WORKSPACE, E_CUDA, E_TIMEOUT = 0, -1, -2, -3, -4, -5
 LAYOUT_CODES = {"NCHW": NCHW, "NHWC": NHWC, "CHWN": CHWN}
+REDUCTION_CODES = {"mean": MEAN, "sum": SUM, "none": NONE}
 DTYPE_CODES = {"fp32": FP32, "tf32": TF32, "bf16": BF16, "fp32x3": FP32X3}
 
 
@@ -33,6 +35,13 @@ class ConvDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in (
         "layout_in", "layout_out", "n", "c", "h", "w", "k", "pad", "dtype", "operand", "wino",
         "relu", "has_bias", "pool2x2", "slab_images", "out_dtype")]
+
+
+class XentDesc(ctypes.Structure):
+    """struct wino_xent_desc"""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "d", "v", "dtype", "has_bias", "reduction", "has_ignore")] + [
+        ("ignore_index", ctypes.c_longlong), ("label_smoothing", ctypes.c_float)] + [
+        (n, ctypes.c_longlong) for n in ("ldx", "ldw", "lddx", "lddw", "scratch_limit")]
 
 
 def declared_symbols():
@@ -88,6 +97,16 @@ def lib():
     L.wino_maxpool2x2.argtypes = [I, I, I, I, I, I, V, V, V]
     L.wino_selftest_wait_timeout.argtypes = [I, V]
     L.wino_selftest_wait_timeout.restype = I
+    LL, ULL, XP = ctypes.c_longlong, ctypes.c_ulonglong, ctypes.POINTER(XentDesc)
+    for name in ("wino_dropout_forward", "wino_dropout_backward"):
+        getattr(L, name).argtypes = [I, LL, LL, LL, LL, ctypes.c_float, ULL, ULL, V, V, V, V]
+        getattr(L, name).restype = I
+    L.wino_xent_workspace_bytes.restype = SZ
+    L.wino_xent_workspace_bytes.argtypes = [XP, I]
+    L.wino_xent_forward.argtypes = [XP, V, V, V, V, V, V, V, SZ, V]
+    L.wino_xent_forward.restype = I
+    L.wino_xent_grad.argtypes = [XP, V, V, V, V, V, V, V, V, V, V, V, SZ, V]
+    L.wino_xent_grad.restype = I
     L.wino_stage_tile_rows.restype = ctypes.c_longlong
     L.wino_stage_tile_rows.argtypes = [P, I]
     L.wino_stage_cp.argtypes = [P]

@@ -1,0 +1,72 @@
+// Shared by the linear softmax cross entropy's products (xent_gemm.cu) and its driver and row kernels (xent.cu).
+#pragma once
+
+#include "ptx.cuh"
+
+namespace wino {
+
+constexpr int XE_BM = 256, XE_BN = 256, XE_BK = 64;      // tile of a CTA pair, contraction elements per ring slot
+constexpr int XE_STATUS_TARGET = 100;                    // status word: a target outside 0 ... v-1
+
+// A BF16 operand: `planes` matrices (parts of a split float operand, or one) of `rows` x `cols`, rows `pitch` and planes
+// `plane_pitch` elements apart.  The contraction runs along the columns, or along the rows where `along_rows` is set.
+struct XeOperand {
+    const void* ptr;
+    long long rows, cols, pitch, plane_pitch;
+    int planes;
+    bool along_rows;
+};
+
+// What the epilogue does with a 256 x 256 tile of the product (m rows x n columns)
+enum XeEpilogue {
+    XE_F32 = 0,     // store floats, or add them to what is there
+    XE_BF16 = 1,    // round and store
+    XE_STATS = 2,   // per row: maximum, sum of exponentials (and of logits) of this tile's columns; the target's logit
+    XE_DZ = 3,      // g (softmax - one-hot), rounded to BF16 (or split into three BF16 planes), and its column sums
+};
+
+struct XeOutput {
+    void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16: m rows; XE_DZ: [planes][m][pitch] BF16
+    long long pitch = 0;
+    int splits = 1;                 // parts of the contraction, one buffer each (XE_F32)
+    bool add = false;               // XE_F32: add instead of store
+    // XE_STATS, XE_DZ
+    const float* bias = nullptr;    // of column 0 of this product
+    const long long* target = nullptr;
+    int col_base = 0;               // class number of column 0
+    float2* stats = nullptr;        // [column tile][m] (maximum, sum)
+    float* zsum = nullptr;          // [column tile][m] sum of logits, or NULL
+    float* zt = nullptr;            // [m] logit of the target
+    const float* lse = nullptr;     // [m]
+    const float* rowg = nullptr;    // [m] weight of a row, 0 for one that does not count
+    float smooth_t = 1.f, smooth_all = 0.f;   // 1 - s, s / v
+    float* db_part = nullptr;       // [m / 32][db_pitch] column sums of 32 rows each, or NULL
+    long long db_pitch = 0;
+};
+
+// product of a (m x k) and b (n x k)^T, contraction length k
+int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m, long long n, long long k, const XeOutput& out,
+            cudaStream_t st);
+
+__device__ __forceinline__ float xe_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float XE_LOG2E = 1.4426950408889634f;
+
+// v = p0 + p1 + p2 with BF16 parts (each remainder is rounded to nearest, so three parts hold 24 bits).  A float that
+// rounds to BF16's infinity keeps its upper half instead; infinities and NaN stay in the first part.
+__device__ __forceinline__ void xe_split3(float v, __nv_bfloat16& p0, __nv_bfloat16& p1, __nv_bfloat16& p2) {
+    p0 = __float2bfloat16_rn(v);
+    const uint32_t mag = __float_as_uint(v) & 0x7fffffffu;
+    if (mag >= 0x7f7f8000u) {
+        if (mag >= 0x7f800000u) { p1 = p2 = __float2bfloat16_rn(0.f); return; }
+        p0 = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
+    }
+    const float r1 = v - __bfloat162float(p0);
+    p1 = __float2bfloat16_rn(r1);
+    p2 = __float2bfloat16_rn(r1 - __bfloat162float(p1));
+}
+
+}  // namespace wino

@@ -1,0 +1,552 @@
+// The products of the linear softmax cross entropy (sm_100a): logits z = x W^T, dx = dz W, dW = dz^T x, one kernel with
+// the step that follows fused into its epilogue.
+//
+// CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles), for the reason given in gemm_tc_pair.cu: half of B comes from the
+// partner's shared memory, so a 64-deep slice costs 32 KB of L2 reads per SM.  Operands are BF16; what changes between the
+// three products is along which axis of the stored matrix the contraction runs:
+//   z : x and W along their columns (K-major);  dx: dz along its columns, W along its rows;  dW: dz and x along their rows.
+// An operand contracted along its rows is fetched as boxes of 64 columns x 64 rows and given to the MMA as an MN-major
+// tile (transpose bit of the instruction descriptor, 8-row groups 1 KiB apart, 64-column blocks 8 KiB apart), so nothing
+// is ever transposed in memory.
+// FP32X3: each operand is three BF16 planes; the contraction runs over six pairs of planes, the smallest products first so
+// that they add up before the accumulator is large.
+//
+// Roles as in gemm_tc_pair.cu: warp 0 TMA, warp 1 of the leader MMA, warps 2-5 epilogue with two accumulators in tensor
+// memory, so the epilogue of a tile runs under the products of the next.  Tiles are walked in bands of eight row blocks,
+// rows fastest, so that the pairs working at a time share both operands through the L2.
+// Bound: tensor pipe for wide layers; the read of W (or the write of dW) where rows are few.
+#include <mutex>
+
+#include "tcgen05.cuh"
+#include "xent.cuh"
+
+namespace wino {
+
+namespace {
+
+constexpr int XE_THREADS = 192;
+constexpr int XE_TILE_BYTES = 128 * 128;             // a CTA's share of an operand per ring slot: 128 rows x 64 BF16
+constexpr int XE_STAGE_TILE = 32 * 128;              // epilogue staging: 32 rows x 128 bytes
+constexpr int XE_EPI_WARPS = 4;
+constexpr int XE_BAND = 8;
+
+enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
+
+struct XeParams {
+    long long m, n;
+    int mpairs, nblocks, splits, kchunks, pairs;
+    unsigned char pa[6], pb[6];       // planes of a and b, one entry per partial product
+    uint32_t idesc;
+    int* status;
+    int add;
+    const float* bias;
+    const long long* target;
+    int col_base;
+    float2* stats;
+    float* zsum;
+    float* zt;
+    const float* lse;
+    const float* rowg;
+    float smooth_t, smooth_all;
+    float* db_part;
+    long long db_pitch;
+};
+
+template <int EPI, int PLANES>
+struct XeSmem {
+    static constexpr int STORE_TILES = EPI == XE_STATS ? 0 : EPI == XE_DZ ? PLANES : 1;      // per staging buffer
+    static constexpr int STAGES = EPI == XE_DZ && PLANES == 3 ? 4 : 6;
+    static constexpr int A_OFF = 0;
+    static constexpr int B_OFF = STAGES * XE_TILE_BYTES;
+    static constexpr int STORE_OFF = B_OFF + STAGES * XE_TILE_BYTES;
+    static constexpr int BUF = STORE_TILES * XE_STAGE_TILE;
+    static constexpr int NBUF = 2;
+    static constexpr int BAR_OFF = STORE_OFF + NBUF * XE_EPI_WARPS * BUF;
+    static constexpr int SLOT_OFF = BAR_OFF + 8 * (2 * STAGES + 4);
+    static constexpr int TOTAL = SLOT_OFF + 16 + 1024;
+};
+
+// MN-major tile with 128-byte swizzle: rows of 64 elements (128 bytes) along M or N, one row per contraction element,
+// groups of 8 contraction elements 1 KiB apart, blocks of 64 M / N elements 8 KiB apart
+__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(8192 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
+                 "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+
+// v[i] of lane l -> lane i holds the sum over lanes of v[i] (halving exchange, 31 shuffles)
+__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) {
+        const bool up = lane & w;
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+            const float send = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, w);
+        }
+    }
+    return v[0];
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 o = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&o);
+}
+
+template <int EPI, int PLANES, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1)
+xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+               const __grid_constant__ CUtensorMap tm_out, const XeParams p) {
+    using L = XeSmem<EPI, PLANES>;
+    constexpr int STAGES = L::STAGES;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;       // same offset in both CTAs of the pair
+    uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t a_ring = base + L::A_OFF, b_ring = base + L::B_OFF;
+    const uint32_t bar_full = base + L::BAR_OFF, bar_empty = bar_full + 8 * STAGES;
+    const uint32_t bar_tfull = bar_empty + 8 * STAGES, bar_tempty = bar_tfull + 16;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen_base + L::SLOT_OFF);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + L::SLOT_OFF + 4);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_ctarank();          // 0 = leader (issues the MMAs, owns the "full" and "tempty" barriers)
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full + 8 * s, 1);
+            mbar_init(bar_empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar_tfull + 8 * a, 1);
+            mbar_init(bar_tempty + 8 * a, 2 * XE_EPI_WARPS);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32((const void*)tmem_slot), 512);
+    tc_fence_before();
+    cluster_sync_all();            // barriers of both CTAs initialised before any remote arrive or TMA completion
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const long long tiles = (long long)p.mpairs * p.nblocks, total = tiles * p.splits;
+    const long long pair = blockIdx.x / 2, npairs = gridDim.x / 2;
+
+    auto decode = [&](long long u, int& sp, int& mp, int& nb) {
+        sp = (int)(u / tiles);
+        const long long t = u % tiles, band = (long long)XE_BAND * p.nblocks;
+        const int first = (int)(t / band) * XE_BAND;
+        const int height = p.mpairs - first < XE_BAND ? p.mpairs - first : XE_BAND;
+        mp = first + (int)((t % band) % height);
+        nb = (int)((t % band) / height);
+    };
+    auto chunk_range = [&](int sp, int& c0, int& c1) {
+        c0 = (int)((long long)sp * p.kchunks / p.splits);
+        c1 = (int)((long long)(sp + 1) * p.kchunks / p.splits);
+    };
+
+    if (warp == 0) {
+        const bool issuer = elect_one();
+        const uint32_t full_leader = mapa_shared(bar_full, 0);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (long long u = pair; ok && u < total; u += npairs) {
+            int sp, mp, nb, c0, c1;
+            decode(u, sp, mp, nb);
+            chunk_range(sp, c0, c1);
+            const int arow = (mp * 2 + (int)rank) * 128;               // this CTA's 128 rows of a
+            const int brow = nb * XE_BN + (int)rank * 128;             // this CTA's half of the rows of b
+            for (int q = 0; ok && q < p.pairs; ++q) {
+                const int pa = p.pa[q], pb = p.pb[q];
+                for (int kc = c0; kc < c1; ++kc) {
+                    if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XE_WAIT_EMPTY)) { ok = false; break; }
+                    if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 4 * XE_TILE_BYTES);
+                    if (issuer) {
+                        const uint32_t bar = full_leader + 8 * stage, as = a_ring + stage * XE_TILE_BYTES, bs = b_ring + stage * XE_TILE_BYTES;
+                        if (A_MN) {
+                            tma_load_3d_pair(as, &tm_a, bar, arow, kc * XE_BK, pa);
+                            tma_load_3d_pair(as + 8192, &tm_a, bar, arow + 64, kc * XE_BK, pa);
+                        } else {
+                            tma_load_3d_pair(as, &tm_a, bar, kc * XE_BK, arow, pa);
+                        }
+                        if (B_MN) {
+                            tma_load_3d_pair(bs, &tm_b, bar, brow, kc * XE_BK, pb);
+                            tma_load_3d_pair(bs + 8192, &tm_b, bar, brow + 64, kc * XE_BK, pb);
+                        } else {
+                            tma_load_3d_pair(bs, &tm_b, bar, kc * XE_BK, brow, pb);
+                        }
+                    }
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+            }
+        }
+        if (!ok && issuer) drain_after_abort();
+    } else if (warp == 1) {
+        if (rank == 0) {   // warp-uniform loop, one elected lane issues the tcgen05 instructions
+            const bool issuer = elect_one();
+            int stage = 0, as = 0;
+            uint32_t phase = 0, aphase = 0;
+            bool ok = true;
+            for (long long u = pair; ok && u < total; u += npairs) {
+                int sp, mp, nb, c0, c1;
+                decode(u, sp, mp, nb);
+                chunk_range(sp, c0, c1);
+                if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (uint32_t)(as * XE_BN);
+                const int steps = (c1 - c0) * p.pairs;
+                for (int kc = 0; kc < steps; ++kc) {
+                    if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XE_WAIT_FULL)) { ok = false; break; }
+                    tc_fence_after();
+                    // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
+                    const uint32_t at = a_ring + stage * XE_TILE_BYTES, bt = b_ring + stage * XE_TILE_BYTES;
+                    const uint64_t a_desc = A_MN ? smem_desc_mn128(at) : smem_desc_k128(at);
+                    const uint64_t b_desc = B_MN ? smem_desc_mn128(bt) : smem_desc_k128(bt);
+                    constexpr uint64_t a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
+#pragma unroll
+                    for (int ks = 0; ks < XE_BK / 16; ++ks)
+                        if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, p.idesc, (kc | ks) ? 1u : 0u);
+                    if (issuer) tc_commit_pair(bar_empty + 8 * stage, 3);       // frees the slot in both CTAs
+                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                }
+                if (ok && issuer) tc_commit_pair(bar_tfull + 8 * as, 3);        // accumulator ready in both CTAs
+                as ^= 1;
+                if (as == 0) aphase ^= 1;
+            }
+        }
+    } else {
+        const int quarter = warp % 4;                 // tensor-memory lanes [32*quarter, 32*quarter + 32)
+        uint8_t* stage_gen = gen_base + L::STORE_OFF + quarter * L::NBUF * L::BUF;
+        const uint32_t stage_s = base + L::STORE_OFF + quarter * L::NBUF * L::BUF;
+        const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
+        int as = 0;
+        uint32_t aphase = 0, issued = 0;
+        bool ok = true;
+        // the staging buffer that is free next (its earlier store has been read out of shared memory)
+        auto next_buffer = [&]() -> uint32_t {
+            const uint32_t buf = issued & 1;
+            if (issued >= 2) {
+                if (lane == 0) tma_store_wait_read<1>();
+                __syncwarp();
+            }
+            ++issued;
+            return buf;
+        };
+        for (long long u = pair; ok && u < total; u += npairs) {
+            int sp, mp, nb;
+            decode(u, sp, mp, nb);
+            if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
+            tc_fence_after();
+            const long long row0 = (long long)(mp * 2 + (int)rank) * 128 + quarter * 32;
+            const long long row = row0 + lane;
+            const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * XE_BN);
+            auto release = [&]() {                    // this warp's share of the accumulator is in registers
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * as);
+            };
+            if constexpr (EPI == XE_F32) {
+#pragma unroll 1
+                for (int chunk = 0; chunk < XE_BN / 32; ++chunk) {
+                    uint32_t r[32];
+                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 32), r);
+                    tmem_ld_wait();
+                    if (chunk == XE_BN / 32 - 1) release();
+                    const long long col0 = (long long)nb * XE_BN + chunk * 32;
+                    if (row0 < p.m && col0 < p.n) {
+                        const uint32_t buf = next_buffer();
+                        float4* dst = reinterpret_cast<float4*>(stage_gen + buf * L::BUF + lane * 128);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            dst[j ^ (lane & 7)] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                                                              __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (p.add) tma_reduce_add_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, sp);
+                            else tma_store_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, sp);
+                            tma_store_commit();
+                        }
+                    }
+                }
+            } else if constexpr (EPI == XE_BF16) {
+#pragma unroll 1
+                for (int chunk = 0; chunk < XE_BN / 64; ++chunk) {
+                    uint32_t r[64];
+                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 64), *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 64 + 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+                    tmem_ld_wait();
+                    if (chunk == XE_BN / 64 - 1) release();
+                    const long long col0 = (long long)nb * XE_BN + chunk * 64;
+                    if (row0 < p.m && col0 < p.n) {
+                        const uint32_t buf = next_buffer();
+                        uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + lane * 128);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(r[8 * j + 2 * e]), __uint_as_float(r[8 * j + 2 * e + 1]));
+                            dst[j ^ (lane & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, 0);
+                            tma_store_commit();
+                        }
+                    }
+                }
+            } else {
+                const bool live = row < p.m;
+                // column of the target within this tile (any value outside 0 ... 255 when it lies elsewhere)
+                long long tcol = -1;
+                if (live) tcol = p.target[row] - p.col_base - (long long)nb * XE_BN;
+                if (tcol < 0 || tcol >= XE_BN) tcol = -1;
+                const int tloc = (int)tcol;
+                float lse = 0.f, g = 0.f;
+                if constexpr (EPI == XE_DZ) {
+                    if (live) { lse = p.lse[row]; g = p.rowg[row]; }
+                }
+                float mx = -INFINITY, s = 0.f, zs = 0.f;
+                constexpr int GROUP = EPI == XE_DZ ? 2 : 1;       // 32-column chunks per staging tile
+#pragma unroll 1
+                for (int chunk = 0; chunk < XE_BN / 32; chunk += GROUP) {
+                    uint32_t buf = 0;
+                    const long long gcol0 = (long long)nb * XE_BN + chunk * 32;
+                    const bool gwork = row0 < p.m && gcol0 < p.n;
+                    if constexpr (EPI == XE_DZ) {
+                        if (gwork) buf = next_buffer();
+                    }
+#pragma unroll
+                    for (int h = 0; h < GROUP; ++h) {
+                        uint32_t r[32];
+                        tmem_ld_32x32(tsrc + (uint32_t)((chunk + h) * 32), r);
+                        tmem_ld_wait();
+                        if (chunk + h == XE_BN / 32 - 1) release();
+                        const long long col0 = gcol0 + h * 32;
+                        if (!gwork) continue;
+                        float z[32];
+                        const bool whole = col0 + 32 <= p.n;
+                        if (p.bias && whole) {
+                            const float4* b4 = reinterpret_cast<const float4*>(p.bias + col0);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const float4 b = __ldg(b4 + j);
+                                z[4 * j] = __uint_as_float(r[4 * j]) + b.x;
+                                z[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + b.y;
+                                z[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z;
+                                z[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
+                            if (p.bias) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i)
+                                    if (col0 + i < p.n) z[i] += __ldg(p.bias + col0 + i);
+                            }
+                        }
+                        const int tc = tloc - (chunk + h) * 32;
+                        const bool here = __any_sync(0xffffffffu, tc >= 0 && tc < 32);
+                        if constexpr (EPI == XE_STATS) {
+                            if (here) {
+                                float t = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) t = i == tc ? z[i] : t;
+                                if (tc >= 0 && tc < 32) p.zt[row] = t;
+                            }
+                            if (p.zsum) {
+                                float t = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) t += whole || col0 + i < p.n ? z[i] : 0.f;
+                                zs += t;
+                            }
+                            if (!whole) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) z[i] = col0 + i < p.n ? z[i] : -INFINITY;
+                            }
+                            float cm[4] = {z[0], z[1], z[2], z[3]};
+#pragma unroll
+                            for (int i = 4; i < 32; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
+                            const float m2 = fmaxf(fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])), mx);
+                            const float ref = m2 == -INFINITY ? 0.f : m2;      // nothing but -inf so far: every term is 0
+                            s *= xe_ex2((mx - ref) * XE_LOG2E);
+                            mx = m2;
+                            float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) t[i & 3] += xe_ex2((z[i] - ref) * XE_LOG2E);
+                            s += (t[0] + t[1]) + (t[2] + t[3]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) z[i] = g * (xe_ex2((z[i] - lse) * XE_LOG2E) - p.smooth_all);
+                            if (here) {
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) z[i] = i == tc ? z[i] - g * p.smooth_t : z[i];
+                            }
+                            if (g == 0.f) {                       // a row that does not count: exactly 0, whatever its logits
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) z[i] = 0.f;
+                            }
+                            uint8_t* tile = stage_gen + buf * L::BUF + lane * 128;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t w[PLANES][4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float v0 = z[8 * j + 2 * e], v1 = z[8 * j + 2 * e + 1];
+                                    if constexpr (PLANES == 1) {
+                                        w[0][e] = pack_bf16(v0, v1);
+                                    } else {
+                                        float r0 = v0, r1 = v1;
+#pragma unroll
+                                        for (int q = 0; q < PLANES; ++q) {
+                                            w[q][e] = pack_bf16(r0, r1);
+                                            r0 -= __uint_as_float(w[q][e] << 16);
+                                            r1 -= __uint_as_float(w[q][e] & 0xffff0000u);
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int q = 0; q < PLANES; ++q)
+                                    reinterpret_cast<uint4*>(tile + q * XE_STAGE_TILE)[(4 * h + j) ^ (lane & 7)] =
+                                        make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+                            }
+                            if (p.db_part) {
+                                const float cs = column_sums(z, lane);
+                                if (col0 + lane < p.n) p.db_part[(row0 / 32) * p.db_pitch + col0 + lane] = cs;
+                            }
+                        }
+                    }
+                    if constexpr (EPI == XE_DZ) {
+                        if (gwork) {
+                            fence_async_shared();
+                            __syncwarp();
+                            if (lane == 0) {
+#pragma unroll
+                                for (int q = 0; q < PLANES; ++q)
+                                    tma_store_3d(&tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)gcol0, (int)row0, q);
+                                tma_store_commit();
+                            }
+                        }
+                    }
+                }
+                if constexpr (EPI == XE_STATS) {
+                    if (live) {
+                        p.stats[(long long)nb * p.m + row] = make_float2(mx, s);
+                        if (p.zsum) p.zsum[(long long)nb * p.m + row] = zs;
+                    }
+                }
+            }
+            as ^= 1;
+            if (as == 0) aphase ^= 1;
+        }
+        if (lane == 0) tma_store_wait_all();
+    }
+
+    // neither CTA may leave (or give back tensor memory) while its partner can still read its shared memory,
+    // signal its barriers or run an MMA over both tensor memories
+    tc_fence_before();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+template <int EPI, int PLANES, bool A_MN, bool B_MN>
+int run(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap& tm_out, const XeParams& p, cudaStream_t st) {
+    using L = XeSmem<EPI, PLANES>;
+    static_assert(L::TOTAL <= 232448, "shared memory budget of one CTA exceeded");
+    static std::once_flag once[64];
+    int dev = 0;
+    WINO_CUDA_CHECK(cudaGetDevice(&dev));
+    cudaError_t attr_err = cudaSuccess;
+    std::call_once(once[dev & 63], [&] {
+        attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+    });
+    WINO_CUDA_CHECK(attr_err);
+    const long long total = (long long)p.mpairs * p.nblocks * p.splits;
+    long long pairs = sm_count() / 2;
+    if (total < pairs) pairs = total;
+    count_launch();
+    xe_gemm_kernel<EPI, PLANES, A_MN, B_MN><<<(unsigned)(2 * pairs), XE_THREADS, L::TOTAL, st>>>(tm_a, tm_b, tm_out, p);
+    WINO_CUDA_CHECK(cudaGetLastError());
+    return WINO_OK;
+}
+
+// boxes of 64 columns (128 bytes, 128-byte swizzle): 128 rows for a K-major share, 64 rows (one contraction element each)
+// for an MN-major one
+int operand_map(CUtensorMap* map, const XeOperand& o) {
+    const unsigned long long dims[3] = {(unsigned long long)o.cols, (unsigned long long)o.rows, (unsigned long long)o.planes};
+    const unsigned long long strides[2] = {(unsigned long long)o.pitch * 2, (unsigned long long)o.plane_pitch * 2};
+    const unsigned box[3] = {64u, o.along_rows ? 64u : 128u, 1u};
+    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1);
+}
+
+}  // namespace
+
+int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m, long long n, long long k, const XeOutput& out,
+            cudaStream_t st) {
+    CUtensorMap tm_a, tm_b, tm_out;
+    int rc;
+    if ((rc = operand_map(&tm_a, a)) || (rc = operand_map(&tm_b, b))) return rc;
+    const bool f32 = epi == XE_F32;
+    if (epi == XE_STATS) {
+        tm_out = tm_a;
+    } else {
+        const int es = f32 ? 4 : 2;
+        const int planes = f32 ? out.splits : epi == XE_DZ ? a.planes : 1;
+        const unsigned long long dims[3] = {(unsigned long long)n, (unsigned long long)m, (unsigned long long)planes};
+        const unsigned long long strides[2] = {(unsigned long long)out.pitch * es, (unsigned long long)(out.pitch * m) * es};
+        const unsigned box[3] = {(unsigned)(128 / es), 32u, 1u};
+        if ((rc = encode_tensor_map(&tm_out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, out.ptr, dims,
+                                    strides, box, 1)))
+            return rc;
+    }
+    XeParams p = {};
+    p.m = m; p.n = n;
+    p.mpairs = (int)((m + XE_BM - 1) / XE_BM);
+    p.nblocks = (int)((n + XE_BN - 1) / XE_BN);
+    p.kchunks = (int)((k + XE_BK - 1) / XE_BK);
+    p.splits = out.splits;
+    if (a.planes == 3) {
+        static const unsigned char pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
+        p.pairs = 6;
+        for (int i = 0; i < 6; ++i) { p.pa[i] = pa[i]; p.pb[i] = pb[i]; }
+    } else {
+        p.pairs = 1;
+    }
+    p.idesc = make_idesc(OP_BF16, XE_BN, XE_BM) | (a.along_rows ? 1u << 15 : 0u) | (b.along_rows ? 1u << 16 : 0u);
+    if ((rc = status_word(&p.status))) return rc;
+    p.add = out.add;
+    p.bias = out.bias; p.target = out.target; p.col_base = out.col_base;
+    p.stats = out.stats; p.zsum = out.zsum; p.zt = out.zt;
+    p.lse = out.lse; p.rowg = out.rowg; p.smooth_t = out.smooth_t; p.smooth_all = out.smooth_all;
+    p.db_part = out.db_part; p.db_pitch = out.db_pitch;
+    if (!a.along_rows && !b.along_rows) {
+        if (epi == XE_F32) return run<XE_F32, 1, false, false>(tm_a, tm_b, tm_out, p, st);
+        if (epi == XE_STATS) return run<XE_STATS, 1, false, false>(tm_a, tm_b, tm_out, p, st);
+        if (epi == XE_DZ) return a.planes == 3 ? run<XE_DZ, 3, false, false>(tm_a, tm_b, tm_out, p, st) : run<XE_DZ, 1, false, false>(tm_a, tm_b, tm_out, p, st);
+    } else if (!a.along_rows) {
+        if (epi == XE_F32) return run<XE_F32, 1, false, true>(tm_a, tm_b, tm_out, p, st);
+        if (epi == XE_BF16) return run<XE_BF16, 1, false, true>(tm_a, tm_b, tm_out, p, st);
+    } else if (b.along_rows) {
+        if (epi == XE_F32) return run<XE_F32, 1, true, true>(tm_a, tm_b, tm_out, p, st);
+        if (epi == XE_BF16) return run<XE_BF16, 1, true, true>(tm_a, tm_b, tm_out, p, st);
+    }
+    return fail(WINO_E_BADARG, "xent: no kernel for this product");
+}
+
+}  // namespace wino

@@ -147,6 +147,61 @@ int wino_layout_convert(int layout_src, int layout_dst, int n, int c, int h, int
 int wino_maxpool2x2(int layout, int n, int c, int h, int w, int dtype, const void* in, void* out,
                     wino_stream_t stream);
 
+/* ---- classifier head: dropout, linear softmax cross entropy -------------------------------------------
+ * What a program needs to fit or evaluate a classifier on the convolution stack's features.  The reference only
+ * infers (fc14 / fc15 / fc16 + softmax, netTest/cudnn_test_0124/VGG_Batched/Network.h:668-704) and has no counterpart. */
+
+/* Dropout of a (rows, cols) matrix whose rows start ldx / ldy elements apart; dtype WINO_FP32 (4-byte) or WINO_BF16.
+ *   y = x * 65536 / (65536 - T) where kept, +0 where dropped (whatever x holds there, NaN included), T = round(65536 p)
+ * The mask is never stored: element e = r * cols + c is kept when the 16-bit lane e mod 8 (low halves first) of
+ * Philox4x32-10 (Salmon et al., 2011) with key = seed and counter = (e div 8, offset) is at least T.  It depends on seed,
+ * offset and e alone, not on type, pitches or launch, so the backward pass draws it again: dx = the same map of dy.
+ * offset_dev (may be NULL) points to a device word that is added to `offset` when the kernel runs, so that a captured
+ * graph can draw a fresh mask on every replay.  p in [0, 1]; p = 1 gives zeros.  y may be x itself (same pitch). */
+int wino_dropout_forward(int dtype, long long rows, long long cols, long long ldx, long long ldy, float p,
+                         unsigned long long seed, unsigned long long offset, const unsigned long long* offset_dev,
+                         const void* x, void* y, wino_stream_t stream);
+int wino_dropout_backward(int dtype, long long rows, long long cols, long long lddy, long long lddx, float p,
+                          unsigned long long seed, unsigned long long offset, const unsigned long long* offset_dev,
+                          const void* dy, void* dx, wino_stream_t stream);
+
+/* Softmax cross entropy of a linear layer, z = x W^T + bias, without an (n, v) tensor of logits in the caller's memory:
+ *   lse_i = log sum_j exp z_ij,   loss_i = lse_i - (1 - s) z_i,t(i) - s/v sum_j z_ij        (s = label_smoothing)
+ *   dz_ij = g_i (exp(z_ij - lse_i) - (1 - s) [j = t(i)] - s/v),  dx = dz W,  dW = dz^T x,  dbias = sum_i dz_i
+ * x (n, d), W (v, d), dx, dW: row-major with pitches ldx, ldw, lddx, lddw; bias, dbias: v floats; target: n 64-bit
+ * integers.  WINO_MEAN divides by the number of rows that count (0 rows: loss and gradients are 0). */
+enum { WINO_MEAN = 0, WINO_SUM = 1, WINO_NONE = 2 };
+typedef struct wino_xent_desc {
+    int n, d, v;               /* rows (0 allowed), features, classes                                               */
+    int dtype;                 /* WINO_BF16: bfloat16 x, W, dx, dW; products exact, sums in FP32, dz rounded to bfloat16
+                                  for the two gradient products.  WINO_FP32X3: float tensors, every operand split into
+                                  three bfloat16 parts, six partial products: FP32-level accuracy on tensor cores
+                                  (values below 2^-110 lose the parts that BF16 cannot hold, under 2^-133)             */
+    int has_bias;
+    int reduction;             /* WINO_MEAN, WINO_SUM: one float of loss; WINO_NONE: n floats                       */
+    int has_ignore;            /* rows with target == ignore_index leave no trace: loss_i = lse_i = 0, dx_i = 0, and
+                                  x_i may hold anything, NaN included                                               */
+    long long ignore_index;    /* any value; may also be a class                                                    */
+    float label_smoothing;     /* 0 ... 1                                                                           */
+    long long ldx, ldw, lddx, lddw;   /* pitches in elements, 0 = d.  Base addresses: 16-byte aligned               */
+    long long scratch_limit;   /* bytes of scratch that may grow with n * v; 0 = 1 GiB.  Beyond it the gradient is
+                                  computed in pieces of the vocabulary (at least 256 classes each) whose logits are
+                                  computed again                                                                    */
+} wino_xent_desc;
+
+/* Scratch of wino_xent_forward (grad = 0) or wino_xent_grad (grad = 1); 0 for a bad descriptor. */
+size_t wino_xent_workspace_bytes(const wino_xent_desc* d, int grad);
+/* loss (and lse, n floats, unless NULL). */
+int wino_xent_forward(const wino_xent_desc* d, const void* x, const void* w, const float* bias, const long long* target,
+                      float* loss, float* lse, void* workspace, size_t workspace_bytes, wino_stream_t stream);
+/* loss (and lse unless NULL) and the gradients in one call.  dloss: upstream gradient, one float (WINO_MEAN, WINO_SUM) or
+ * n floats (WINO_NONE) on the device, NULL = 1.  dx, dw, dbias: NULL where not wanted.  A target outside 0 ... v-1 that is
+ * not ignored makes its row's loss NaN, keeps the row out of the gradients, and the next wino_device_status() returns
+ * WINO_E_BADARG (wino_xent_forward likewise).  Results are deterministic (no atomics on results). */
+int wino_xent_grad(const wino_xent_desc* d, const void* x, const void* w, const float* bias, const long long* target,
+                   const float* dloss, float* loss, float* lse, void* dx, void* dw, float* dbias, void* workspace,
+                   size_t workspace_bytes, wino_stream_t stream);
+
 /* TEST-ONLY: launches one small CTA in which a bounded device-side wait runs out after `limit_ms` (1 ... 1000)
  * milliseconds, because nothing ever arrives on its mbarrier.  The CTA records the give-up, lets its other warps leave
  * through the abort flag, frees its tensor memory and returns by itself; the next wino_device_status() returns
