@@ -1,11 +1,15 @@
 // Linear softmax cross entropy with its gradient: driver and row kernels (the products are in xent_gemm.cu).
 //
 // The logits z = x W^T exist one tile at a time.  Two ways, by size:
-//   * kept (few rows or classes): the logits product is split along the features until the GPU is full, the parts are
-//     floats in the scratch, and row kernels make lse, loss and dz of them: three products (2 n v d flops each) in all;
-//   * recomputed: the logits product leaves only a maximum and a sum per row and 256 classes; the gradient then walks the
-//     vocabulary in pieces, computes a piece's logits again, turns them into dz in the epilogue, and multiplies dz into
-//     dx and dW before the next piece: four products, scratch bounded by desc.scratch_limit.
+//   * kept: where rows or classes are few the logits product is split along the features until the GPU is full; its
+//     float parts in the scratch become lse, loss and dz in row kernels.  Unsplit, floats are kept as well where that is
+//     cheaper than a fourth product (below);
+//   * as exponentials: BF16 without a bias whose dz fits the scratch.  The logits product leaves a maximum and a sum per
+//     row and 128 classes and exp(z - maximum) as BF16 in the place of dz; one pass over it makes dz.  Three products
+//     (2 n v d flops each) either way;
+//   * recomputed: the logits product leaves only the statistics; the gradient then walks the vocabulary in pieces, computes
+//     a piece's logits again, turns them into dz in the epilogue, and multiplies dz into dx and dW before the next piece:
+//     four products, scratch bounded by desc.scratch_limit.
 // dz is held as BF16 (one part; the rounding is that of every BF16 operand, and halves what the two gradient products
 // read) or as three BF16 parts (FP32X3).  dbias sums the unrounded dz.  Statistics, lse and losses are FP32, the sum over
 // rows FP64.
@@ -167,12 +171,12 @@ __global__ void __launch_bounds__(128) xe_rows_from_logits_kernel(float* __restr
     }
 }
 
-// one block: loss over the rows, and every row's weight in the gradient
-__global__ void __launch_bounds__(1024) xe_loss_kernel(const RowArgs a, int reduction, const float* __restrict__ dloss, float* __restrict__ loss,
-                                                       float* __restrict__ rowg) {
+// one block: loss over the rows; every row's own weight in the gradient (rowg) and the factor they share (scale), to which
+// dz_factor (XeDzRule's f) belongs
+__global__ void __launch_bounds__(1024) xe_loss_kernel(const RowArgs a, int reduction, const float* __restrict__ dloss, float dz_factor,
+                                                       float* __restrict__ loss, float* __restrict__ rowg, float* __restrict__ scale) {
     __shared__ double rs[32];
     __shared__ long long rc[32];
-    __shared__ float inv_s;
     double sum = 0;
     long long count = 0;
     for (long long i = threadIdx.x; i < a.n; i += 1024) {
@@ -191,23 +195,21 @@ __global__ void __launch_bounds__(1024) xe_loss_kernel(const RowArgs a, int redu
     if (threadIdx.x == 0) {
         for (int i = 1; i < 32; ++i) { sum += rs[i]; count += rc[i]; }
         const double inv = reduction == WINO_MEAN ? 1.0 / (double)(count > 0 ? count : 1) : 1.0;
-        inv_s = (float)inv;
         if (reduction != WINO_NONE) loss[0] = (float)(sum * inv);
+        if (rowg) scale[0] = (float)(inv * dz_factor * (dloss && reduction != WINO_NONE ? (double)dloss[0] : 1.0));
     }
-    __syncthreads();
     if (!rowg) return;
-    const float inv = inv_s;
     for (long long i = threadIdx.x; i < a.n; i += 1024) {
-        const float up = dloss ? dloss[reduction == WINO_NONE ? i : 0] : 1.f;
-        rowg[i] = row_counts(a.rule, a.target[i]) ? up * inv : 0.f;
+        const float own = dloss && reduction == WINO_NONE ? dloss[i] : 1.f;
+        rowg[i] = row_counts(a.rule, a.target[i]) ? own : 0.f;
     }
 }
 
 // dz of kept logits: two classes per thread, 32 rows per block, and the block's column sums
 template <int PLANES>
 __global__ void __launch_bounds__(128) xe_dz_from_logits_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ lse,
-                                                                const float* __restrict__ rowg, const long long* __restrict__ target, float smooth_t,
-                                                                float smooth_all, __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
+                                                                const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
+                                                                __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
     const unsigned cblocks = (unsigned)(v + 255) / 256, part = blockIdx.x / cblocks;
     const int c = (int)((blockIdx.x % cblocks) * 128 + threadIdx.x) * 2;
     if (c >= v) return;
@@ -219,9 +221,9 @@ __global__ void __launch_bounds__(128) xe_dz_from_logits_kernel(const float* __r
         const float2 q = *reinterpret_cast<const float2*>(z + r * zpitch + c);
         const float l = lse[r], g = rowg[r];
         const long long t = target[r];
-        float a = xe_ex2((q.x - l) * XE_LOG2E) - smooth_all, b = xe_ex2((q.y - l) * XE_LOG2E) - smooth_all;
-        if (t == c) a -= smooth_t;
-        if (t == c + 1) b -= smooth_t;
+        float a = xe_ex2((q.x - l) * XE_LOG2E) * rule.pf - rule.smooth_all, b = xe_ex2((q.y - l) * XE_LOG2E) * rule.pf - rule.smooth_all;
+        if (t == c) a -= rule.smooth_t;
+        if (t == c + 1) b -= rule.smooth_t;
         a = g == 0.f ? 0.f : a * g;                       // a row that does not count: exactly 0, whatever its logits
         b = g == 0.f || c + 1 >= v ? 0.f : b * g;
         s0 += a;
@@ -237,7 +239,42 @@ __global__ void __launch_bounds__(128) xe_dz_from_logits_kernel(const float* __r
     if (db_part) *reinterpret_cast<float2*>(db_part + (long long)part * dpitch + c) = make_float2(s0, s1);
 }
 
-__global__ void __launch_bounds__(256) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, float* __restrict__ db) {
+// exponentials (kept in the place of dz) -> dz, eight classes per thread.  The target's probability comes from its logit in
+// FP32, the others' from the rounded exponential: off by one more BF16 rounding.
+__global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __restrict__ dz, int pitch, long long n, const float2* __restrict__ stats,
+                                                             const float* __restrict__ zt, const float* __restrict__ lse, const float* __restrict__ rowg,
+                                                             const long long* __restrict__ target, const XeDzRule rule) {
+    const int octs = pitch / 8;
+    const long long total = n * octs;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / octs;
+        const int c = (int)(i - r * octs) * 8;
+        uint4* at = reinterpret_cast<uint4*>(dz + r * pitch + c);
+        const float g = rowg[r];
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (g != 0.f) {
+            q = *at;
+            const float l = lse[r], f = xe_ex2((stats[c / XE_STAT_COLS * n + r].x - l) * XE_LOG2E) * rule.pf;
+            const long long t = target[r] - c;
+            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float a = __uint_as_float(w[e] << 16) * f - rule.smooth_all, b = __uint_as_float(w[e] & 0xffff0000u) * f - rule.smooth_all;
+                if (t >> 1 == e) {
+                    const float pt = xe_ex2((zt[r] - l) * XE_LOG2E) * rule.pf - rule.smooth_all - rule.smooth_t;
+                    if (t & 1) b = pt; else a = pt;
+                }
+                const __nv_bfloat162 o = __floats2bfloat162_rn(a * g, b * g);
+                w[e] = *reinterpret_cast<const uint32_t*>(&o);
+            }
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *at = q;
+    }
+}
+
+__global__ void __launch_bounds__(256) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, const float* __restrict__ scale,
+                                                    float* __restrict__ db) {
     __shared__ float red[8][32];
     const int l = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + l;
     float s = 0.f;
@@ -247,7 +284,7 @@ __global__ void __launch_bounds__(256) xe_db_kernel(const float* __restrict__ pa
     __syncthreads();
     if (g == 0 && c < cols) {
         for (int i = 1; i < 8; ++i) s += red[i][l];
-        db[c] = s;
+        db[c] = s * *scale;
     }
 }
 
@@ -281,12 +318,13 @@ unsigned loop_blocks(long long items) {
 struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
-    bool pack_x, pack_w, kept;
+    bool pack_x, pack_w;
+    bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw;
     int zpitch, piece, pieces, dzpitch;
     bool dx_direct, dw_direct;           // the product's epilogue stores the caller's matrix
     int dpitch;                          // of float dx / dw buffers in the scratch
-    size_t off_x, off_w, off_z, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_dz, off_db, off_dx, off_dw, total;
+    size_t off_x, off_w, off_z, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_scale, off_dz, off_db, off_dx, off_dw, total;
 };
 
 // parts of the contraction so that tiles * parts fills the CTA pairs, each with at least four ring slots of work
@@ -330,15 +368,16 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const long long kd = (d->d + XE_BK - 1) / XE_BK;
     p.splits_z = split_count(tiles_of(n, v), kd, products);
     p.zpitch = round_up(d->v, 4);
-    const long long kept_bytes = n * (p.zpitch * 4ll * p.splits_z + (grad ? round_up(d->v, 8) * 2ll * p.planes : 0));
-    // Logits are kept where the product is split anyway; where it is not, storing and reading them (14 bytes each) has to
-    // cost less than computing them twice (2 d flops each), and to fit.
+    const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll * p.splits_z;
+    // Kept floats cost 14 bytes a logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured
+    // 6.5 TB/s and 1.4 PFLOP/s the product is the dearer one from d = 1000 (200) on.
     if (p.splits_z > 1) p.kept = true;
-    else p.kept = grad && kept_bytes <= limit && d->d >= 1024;
+    else if (grad && bf16 && !d->has_bias && dz_bytes <= limit) p.exps = true;
+    else p.kept = grad && z_bytes + dz_bytes <= limit && d->d >= (bf16 ? 1024 : 256);
     if (!p.kept) p.splits_z = 1;
     p.piece = d->v;
     p.pieces = 1;
-    if (grad && !p.kept) {
+    if (grad && !p.kept && !p.exps) {
         long long most = limit / (n > 0 ? n * 2 * p.planes : 1) / XE_BN * XE_BN;
         if (most < XE_BN) most = XE_BN;
         if (most < v) {
@@ -364,7 +403,8 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.off_rowloss = take(un * 4);
     p.off_rowg = take(un * 4);
     p.off_zt = take(un * 4);
-    const size_t vtiles = (size_t)((v + XE_BN - 1) / XE_BN);
+    p.off_scale = take(4);
+    const size_t vtiles = (size_t)((v + XE_STAT_COLS - 1) / XE_STAT_COLS);
     p.off_zsum = take(p.kept || d->label_smoothing <= 0.f ? 0 : vtiles * un * 4);
     p.off_z = take(p.kept ? un * p.zpitch * 4 * p.splits_z : vtiles * un * 8);
     p.off_x = take(p.pack_x ? un * p.dp * 2 * p.planes : 0);
@@ -394,10 +434,11 @@ int pack(const wino_xent_desc& d, const Plan& p, const void* src, long long ld, 
 
 // one gradient product: into the caller's matrix where its epilogue can store it, else through float buffers
 int grad_product(const Plan& p, const wino_xent_desc& d, const XeOperand& a, const XeOperand& b, long long rows, long long k, bool direct, int splits,
-                 bool first, bool last, void* out, long long ld, float* buf, cudaStream_t st) {
+                 bool first, bool last, void* out, long long ld, float* buf, const float* scale, cudaStream_t st) {
     XeOutput o;
     int rc;
     o.add = !first;
+    o.scale = scale;
     if (direct) {
         o.ptr = out;
         o.pitch = ld;
@@ -473,17 +514,25 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         oz.stats = reinterpret_cast<float2*>(ws + p.off_z);
         oz.zsum = d.label_smoothing > 0.f ? f(p.off_zsum) : nullptr;
         oz.zt = f(p.off_zt);
-        if ((rc = xe_gemm(XE_STATS, ox, ow, n, v, d.d, oz, st))) return rc;
+        if (p.exps) {
+            oz.ptr = ws + p.off_dz;
+            oz.pitch = p.dzpitch;
+        }
+        if ((rc = xe_gemm(p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, oz, st))) return rc;
         count_launch();
-        xe_rows_from_stats_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(oz.stats, oz.zsum, oz.zt, (int)((v + XE_BN - 1) / XE_BN), ra);
+        xe_rows_from_stats_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(oz.stats, oz.zsum, oz.zt, (int)((v + XE_STAT_COLS - 1) / XE_STAT_COLS), ra);
     }
     WINO_CUDA_CHECK(cudaGetLastError());
+    XeDzRule dzr;
+    const float s = d.label_smoothing, dz_factor = s <= 0.5f ? 1.f - s : 1.f;
+    dzr.pf = 1.f / dz_factor;
+    dzr.smooth_t = s <= 0.5f ? 1.f : 1.f - s;
+    dzr.smooth_all = (float)((double)s / (double)v / (double)dz_factor);
     count_launch();
-    xe_loss_kernel<<<1, 1024, 0, st>>>(ra, d.reduction, dloss, loss, grad ? f(p.off_rowg) : nullptr);
+    xe_loss_kernel<<<1, 1024, 0, st>>>(ra, d.reduction, dloss, dz_factor, loss, grad ? f(p.off_rowg) : nullptr, f(p.off_scale));
     WINO_CUDA_CHECK(cudaGetLastError());
     if (!grad || (!dx && !dw && !db)) return WINO_OK;
 
-    const float smooth_t = 1.f - d.label_smoothing, smooth_all = (float)((double)d.label_smoothing / (double)v);
     const int parts = (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
     __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + p.off_dz);
     float* db_part = db ? f(p.off_db) : nullptr;
@@ -496,35 +545,39 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             const unsigned grid = (unsigned)((vc + 255) / 256) * (unsigned)parts;
             count_launch();
             if (p.planes == 1)
-                xe_dz_from_logits_kernel<1><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, smooth_t, smooth_all, dz, p.dzpitch, db_part);
+                xe_dz_from_logits_kernel<1><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, dzr, dz, p.dzpitch, db_part);
             else
-                xe_dz_from_logits_kernel<3><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, smooth_t, smooth_all, dz, p.dzpitch, db_part);
+                xe_dz_from_logits_kernel<3><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, dzr, dz, p.dzpitch, db_part);
+            WINO_CUDA_CHECK(cudaGetLastError());
+        } else if (p.exps) {
+            count_launch();
+            xe_dz_from_exp_kernel<<<loop_blocks(n * (p.dzpitch / 8)), 256, 0, st>>>(dz, p.dzpitch, n, oz.stats, oz.zt, ra.lse, f(p.off_rowg), target, dzr);
             WINO_CUDA_CHECK(cudaGetLastError());
         } else {
             XeOutput o;
             o.ptr = dz; o.pitch = p.dzpitch;
             o.bias = b ? b + v0 : nullptr;
             o.target = target; o.col_base = v0;
-            o.lse = ra.lse; o.rowg = f(p.off_rowg); o.smooth_t = smooth_t; o.smooth_all = smooth_all;
+            o.lse = ra.lse; o.rowg = f(p.off_rowg); o.rule = dzr;
             o.db_part = db_part; o.db_pitch = p.dzpitch;
             if ((rc = xe_gemm(XE_DZ, ox, wp, n, vc, d.d, o, st))) return rc;
         }
         if (db) {
             count_launch();
-            xe_db_kernel<<<(unsigned)((vc + 31) / 32), 256, 0, st>>>(db_part, parts, p.dzpitch, vc, db + v0);
+            xe_db_kernel<<<(unsigned)((vc + 31) / 32), 256, 0, st>>>(db_part, parts, p.dzpitch, vc, f(p.off_scale), db + v0);
             WINO_CUDA_CHECK(cudaGetLastError());
         }
         XeOperand odz = {dz, n, vc, p.dzpitch, n * p.dzpitch, p.planes, false};
         if (dx) {
             XeOperand wr = wp;
             wr.along_rows = true;
-            if ((rc = grad_product(p, d, odz, wr, n, vc, p.dx_direct, p.splits_dx, i == 0, i == p.pieces - 1, dx, p.lddx, f(p.off_dx), st))) return rc;
+            if ((rc = grad_product(p, d, odz, wr, n, vc, p.dx_direct, p.splits_dx, i == 0, i == p.pieces - 1, dx, p.lddx, f(p.off_dx), f(p.off_scale), st))) return rc;
         }
         if (dw) {
             XeOperand zr = odz, xr = ox;
             zr.along_rows = xr.along_rows = true;
             if ((rc = grad_product(p, d, zr, xr, vc, n, p.dw_direct, p.splits_dw, true, true, static_cast<char*>(dw) + (size_t)v0 * p.lddw * p.es, p.lddw,
-                                   f(p.off_dw), st)))
+                                   f(p.off_dw), f(p.off_scale), st)))
                 return rc;
         }
     }

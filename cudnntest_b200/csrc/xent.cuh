@@ -19,27 +19,40 @@ struct XeOperand {
 
 // What the epilogue does with a 256 x 256 tile of the product (m rows x n columns)
 enum XeEpilogue {
-    XE_F32 = 0,     // store floats, or add them to what is there
-    XE_BF16 = 1,    // round and store
-    XE_STATS = 2,   // per row: maximum, sum of exponentials (and of logits) of this tile's columns; the target's logit
-    XE_DZ = 3,      // g (softmax - one-hot), rounded to BF16 (or split into three BF16 planes), and its column sums
+    XE_F32 = 0,       // scale, store floats or add them to what is there
+    XE_BF16 = 1,      // scale, round and store
+    XE_STATS = 2,     // per row and 128 columns: maximum, sum of exponentials (and of logits); the target's logit
+    XE_STATS_E = 3,   // the same, and the exponentials exp(z - maximum) themselves, rounded to BF16
+    XE_DZ = 4,        // the gradient of the logits, rounded to BF16 (or split into three BF16 planes), and its column sums
+};
+constexpr int XE_STAT_COLS = 128;
+
+// The gradient of a logit as it is stored: g ((p - s/v) / f - [target] (1 - s) / f), where f = 1 - s (1 if s > 1/2) and g is
+// the row's weight without what all rows share.  The rest, f times the common factor, is applied to the finished products:
+// a row's target has the value -1 + small, which BF16 holds well, where -(1 - s) / rows, alike in all rows, would be off by
+// the same rounding in every one of them (measured: relative error of dx 3.7e-3 against 2.0e-3).
+struct XeDzRule {
+    float pf = 1.f;           // 1 / f
+    float smooth_t = 1.f;     // (1 - s) / f
+    float smooth_all = 0.f;   // s / v / f
 };
 
 struct XeOutput {
-    void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16: m rows; XE_DZ: [planes][m][pitch] BF16
+    void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16, XE_STATS_E: m rows; XE_DZ: [planes][m][pitch] BF16
     long long pitch = 0;
     int splits = 1;                 // parts of the contraction, one buffer each (XE_F32)
     bool add = false;               // XE_F32: add instead of store
-    // XE_STATS, XE_DZ
+    const float* scale = nullptr;   // XE_F32, XE_BF16: device scalar the product is multiplied by, or NULL
+    // XE_STATS, XE_STATS_E, XE_DZ
     const float* bias = nullptr;    // of column 0 of this product
     const long long* target = nullptr;
     int col_base = 0;               // class number of column 0
-    float2* stats = nullptr;        // [column tile][m] (maximum, sum)
-    float* zsum = nullptr;          // [column tile][m] sum of logits, or NULL
+    float2* stats = nullptr;        // [n / 128][m] (maximum, sum)
+    float* zsum = nullptr;          // [n / 128][m] sum of logits, or NULL
     float* zt = nullptr;            // [m] logit of the target
     const float* lse = nullptr;     // [m]
     const float* rowg = nullptr;    // [m] weight of a row, 0 for one that does not count
-    float smooth_t = 1.f, smooth_all = 0.f;   // 1 - s, s / v
+    XeDzRule rule;
     float* db_part = nullptr;       // [m / 32][db_pitch] column sums of 32 rows each, or NULL
     long long db_pitch = 0;
 };

@@ -8,12 +8,17 @@
 // An operand contracted along its rows is fetched as boxes of 64 columns x 64 rows and given to the MMA as an MN-major
 // tile (transpose bit of the instruction descriptor, 8-row groups 1 KiB apart, 64-column blocks 8 KiB apart), so nothing
 // is ever transposed in memory.
-// FP32X3: each operand is three BF16 planes; the contraction runs over six pairs of planes, the smallest products first so
-// that they add up before the accumulator is large.
+// FP32X3: each operand is three BF16 planes; a block of the contraction runs over six pairs of planes, the smallest
+// products first so that they add up before the accumulator is large.
 //
-// Roles as in gemm_tc_pair.cu: warp 0 TMA, warp 1 of the leader MMA, warps 2-5 epilogue with two accumulators in tensor
-// memory, so the epilogue of a tile runs under the products of the next.  Tiles are walked in bands of eight row blocks,
-// rows fastest, so that the pairs working at a time share both operands through the L2.
+// The tensor cores truncate when they add to an accumulator, which over a contraction of 1000 elements biases a sum by
+// some 10^-6 of itself.  So the contraction is cut into blocks (256 elements for FP32X3, 1024 for BF16); each block's sum is
+// fetched from tensor memory and added to the tile's sums in registers, rounded to nearest, while the next block runs in
+// the other accumulator.
+//
+// Roles as in gemm_tc_pair.cu: warp 0 TMA, warp 1 of the leader MMA, warps 2-9 epilogue: a warp holds 32 rows x 128 columns
+// of the tile in 128 registers a thread and gives the accumulator back before it works on them.  Tiles are walked in bands
+// of eight row blocks, rows fastest, so that the pairs working at a time share both operands through the L2.
 // Bound: tensor pipe for wide layers; the read of W (or the write of dW) where rows are few.
 #include <mutex>
 
@@ -24,10 +29,11 @@ namespace wino {
 
 namespace {
 
-constexpr int XE_THREADS = 192;
+constexpr int XE_THREADS = 320;
 constexpr int XE_TILE_BYTES = 128 * 128;             // a CTA's share of an operand per ring slot: 128 rows x 64 BF16
 constexpr int XE_STAGE_TILE = 32 * 128;              // epilogue staging: 32 rows x 128 bytes
-constexpr int XE_EPI_WARPS = 4;
+constexpr int XE_EPI_WARPS = 8;
+constexpr int XE_WCOLS = 128;                        // columns of an epilogue warp
 constexpr int XE_BAND = 8;
 
 enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
@@ -35,10 +41,12 @@ enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53
 struct XeParams {
     long long m, n;
     int mpairs, nblocks, splits, kchunks, pairs;
+    int block;                        // ring slots per block of the contraction (and plane pair)
     unsigned char pa[6], pb[6];       // planes of a and b, one entry per partial product
     uint32_t idesc;
     int* status;
     int add;
+    const float* scale;
     const float* bias;
     const long long* target;
     int col_base;
@@ -47,20 +55,20 @@ struct XeParams {
     float* zt;
     const float* lse;
     const float* rowg;
-    float smooth_t, smooth_all;
+    XeDzRule rule;
     float* db_part;
     long long db_pitch;
 };
 
 template <int EPI, int PLANES>
 struct XeSmem {
-    static constexpr int STORE_TILES = EPI == XE_STATS ? 0 : EPI == XE_DZ ? PLANES : 1;      // per staging buffer
-    static constexpr int STAGES = EPI == XE_DZ && PLANES == 3 ? 4 : 6;
+    static constexpr int STORE_TILES = EPI == XE_STATS ? 0 : PLANES;      // per staging buffer
+    static constexpr int STAGES = PLANES == 3 ? 4 : EPI == XE_STATS ? 6 : 5;
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = STAGES * XE_TILE_BYTES;
     static constexpr int STORE_OFF = B_OFF + STAGES * XE_TILE_BYTES;
     static constexpr int BUF = STORE_TILES * XE_STAGE_TILE;
-    static constexpr int NBUF = 2;
+    static constexpr int NBUF = PLANES == 3 ? 1 : 2;
     static constexpr int BAR_OFF = STORE_OFF + NBUF * XE_EPI_WARPS * BUF;
     static constexpr int SLOT_OFF = BAR_OFF + 8 * (2 * STAGES + 4);
     static constexpr int TOTAL = SLOT_OFF + 16 + 1024;
@@ -84,8 +92,8 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32
                  : "memory");
 }
 
-// v[i] of lane l -> lane i holds the sum over lanes of v[i] (halving exchange, 31 shuffles)
-__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+// v[i] of lane l -> lane i returns the sum over lanes of v[i] (halving exchange, 31 shuffles); v is used up
+__device__ __forceinline__ float column_sums(float* v, int lane) {
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) {
         const bool up = lane & w;
@@ -168,9 +176,10 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             chunk_range(sp, c0, c1);
             const int arow = (mp * 2 + (int)rank) * 128;               // this CTA's 128 rows of a
             const int brow = nb * XE_BN + (int)rank * 128;             // this CTA's half of the rows of b
+            for (int cb = c0; ok && cb < c1; cb += p.block)
             for (int q = 0; ok && q < p.pairs; ++q) {
-                const int pa = p.pa[q], pb = p.pb[q];
-                for (int kc = c0; kc < c1; ++kc) {
+                const int pa = p.pa[q], pb = p.pb[q], ce = cb + p.block < c1 ? cb + p.block : c1;
+                for (int kc = cb; kc < ce; ++kc) {
                     if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XE_WAIT_EMPTY)) { ok = false; break; }
                     if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 4 * XE_TILE_BYTES);
                     if (issuer) {
@@ -203,75 +212,117 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 int sp, mp, nb, c0, c1;
                 decode(u, sp, mp, nb);
                 chunk_range(sp, c0, c1);
-                if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + (uint32_t)(as * XE_BN);
-                const int steps = (c1 - c0) * p.pairs;
-                for (int kc = 0; kc < steps; ++kc) {
-                    if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XE_WAIT_FULL)) { ok = false; break; }
+                for (int cb = c0; ok && cb < c1; cb += p.block) {
+                    const int steps = (cb + p.block < c1 ? p.block : c1 - cb) * p.pairs;
+                    if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
                     tc_fence_after();
-                    // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
-                    const uint32_t at = a_ring + stage * XE_TILE_BYTES, bt = b_ring + stage * XE_TILE_BYTES;
-                    const uint64_t a_desc = A_MN ? smem_desc_mn128(at) : smem_desc_k128(at);
-                    const uint64_t b_desc = B_MN ? smem_desc_mn128(bt) : smem_desc_k128(bt);
-                    constexpr uint64_t a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
+                    const uint32_t d_tmem = tmem_base + (uint32_t)(as * XE_BN);
+                    for (int kc = 0; kc < steps; ++kc) {
+                        if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XE_WAIT_FULL)) { ok = false; break; }
+                        tc_fence_after();
+                        // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
+                        const uint32_t at = a_ring + stage * XE_TILE_BYTES, bt = b_ring + stage * XE_TILE_BYTES;
+                        const uint64_t a_desc = A_MN ? smem_desc_mn128(at) : smem_desc_k128(at);
+                        const uint64_t b_desc = B_MN ? smem_desc_mn128(bt) : smem_desc_k128(bt);
+                        constexpr uint64_t a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
 #pragma unroll
-                    for (int ks = 0; ks < XE_BK / 16; ++ks)
-                        if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, p.idesc, (kc | ks) ? 1u : 0u);
-                    if (issuer) tc_commit_pair(bar_empty + 8 * stage, 3);       // frees the slot in both CTAs
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                        for (int ks = 0; ks < XE_BK / 16; ++ks)
+                            if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, p.idesc, (kc | ks) ? 1u : 0u);
+                        if (issuer) tc_commit_pair(bar_empty + 8 * stage, 3);       // frees the slot in both CTAs
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+                    }
+                    if (ok && issuer) tc_commit_pair(bar_tfull + 8 * as, 3);        // this block's sums are ready in both CTAs
+                    as ^= 1;
+                    if (as == 0) aphase ^= 1;
                 }
-                if (ok && issuer) tc_commit_pair(bar_tfull + 8 * as, 3);        // accumulator ready in both CTAs
-                as ^= 1;
-                if (as == 0) aphase ^= 1;
             }
         }
     } else {
         const int quarter = warp % 4;                 // tensor-memory lanes [32*quarter, 32*quarter + 32)
-        uint8_t* stage_gen = gen_base + L::STORE_OFF + quarter * L::NBUF * L::BUF;
-        const uint32_t stage_s = base + L::STORE_OFF + quarter * L::NBUF * L::BUF;
+        const int half = (warp - 2) / 4;              // columns [128*half, 128*half + 128)
+        uint8_t* stage_gen = gen_base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
+        const uint32_t stage_s = base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
         const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
         int as = 0;
         uint32_t aphase = 0, issued = 0;
         bool ok = true;
+        const float scale = (EPI == XE_F32 || EPI == XE_BF16) && p.scale ? *p.scale : 1.f;
         // the staging buffer that is free next (its earlier store has been read out of shared memory)
         auto next_buffer = [&]() -> uint32_t {
-            const uint32_t buf = issued & 1;
-            if (issued >= 2) {
-                if (lane == 0) tma_store_wait_read<1>();
+            const uint32_t buf = L::NBUF == 1 ? 0 : issued & 1;
+            if (issued >= (uint32_t)L::NBUF) {
+                if (lane == 0) tma_store_wait_read<L::NBUF - 1>();
                 __syncwarp();
             }
             ++issued;
             return buf;
         };
         for (long long u = pair; ok && u < total; u += npairs) {
-            int sp, mp, nb;
+            int sp, mp, nb, c0, c1;
             decode(u, sp, mp, nb);
-            if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
-            tc_fence_after();
+            chunk_range(sp, c0, c1);
             const long long row0 = (long long)(mp * 2 + (int)rank) * 128 + quarter * 32;
-            const long long row = row0 + lane;
-            const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * XE_BN);
-            auto release = [&]() {                    // this warp's share of the accumulator is in registers
+            const long long row = row0 + lane, wcol = (long long)nb * XE_BN + half * XE_WCOLS;
+
+            float z[XE_WCOLS];                        // this thread's row of the tile
+            for (int cb = c0; cb < c1; cb += p.block) {
+                if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * XE_BN + half * XE_WCOLS);
+                if (cb == c0) {
+#pragma unroll
+                    for (int j = 0; j < XE_WCOLS / 32; ++j) tmem_ld_32x32(tsrc + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * j]));
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < XE_WCOLS / 16; ++j) {
+                        uint32_t r[16];
+                        tmem_ld_32x16(tsrc + j * 16, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[16 * j + i] += __uint_as_float(r[i]);
+                    }
+                }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * as);
+                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * as);       // this warp's share of the accumulator is in registers
+                as ^= 1;
+                if (as == 0) aphase ^= 1;
+            }
+            if (!ok) break;
+            if (row0 >= p.m || wcol >= p.n) continue;
+
+            // 64 columns of values, packed as BF16 pairs, to plane `plane` of the output
+            auto stage64 = [&](const uint32_t (&w)[32], uint32_t buf, int plane) {
+                uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + plane * XE_STAGE_TILE + lane * 128);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dst[j ^ (lane & 7)] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
             };
+            auto store64 = [&](uint32_t buf, long long col0, int planes) {
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    for (int q = 0; q < planes; ++q)
+                        tma_store_3d(&tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)col0, (int)row0, q);
+                    tma_store_commit();
+                }
+            };
+
+            if constexpr (EPI == XE_F32 || EPI == XE_BF16) {
+#pragma unroll
+                for (int i = 0; i < XE_WCOLS; ++i) z[i] *= scale;
+            }
             if constexpr (EPI == XE_F32) {
-#pragma unroll 1
-                for (int chunk = 0; chunk < XE_BN / 32; ++chunk) {
-                    uint32_t r[32];
-                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 32), r);
-                    tmem_ld_wait();
-                    if (chunk == XE_BN / 32 - 1) release();
-                    const long long col0 = (long long)nb * XE_BN + chunk * 32;
-                    if (row0 < p.m && col0 < p.n) {
+#pragma unroll
+                for (int chunk = 0; chunk < XE_WCOLS / 32; ++chunk) {
+                    const long long col0 = wcol + chunk * 32;
+                    if (col0 < p.n) {
                         const uint32_t buf = next_buffer();
                         float4* dst = reinterpret_cast<float4*>(stage_gen + buf * L::BUF + lane * 128);
+                        const float* v = &z[chunk * 32];
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
-                            dst[j ^ (lane & 7)] = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                                              __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+                            dst[j ^ (lane & 7)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                         fence_async_shared();
                         __syncwarp();
                         if (lane == 0) {
@@ -282,175 +333,143 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     }
                 }
             } else if constexpr (EPI == XE_BF16) {
-#pragma unroll 1
-                for (int chunk = 0; chunk < XE_BN / 64; ++chunk) {
-                    uint32_t r[64];
-                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 64), *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-                    tmem_ld_32x32(tsrc + (uint32_t)(chunk * 64 + 32), *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-                    tmem_ld_wait();
-                    if (chunk == XE_BN / 64 - 1) release();
-                    const long long col0 = (long long)nb * XE_BN + chunk * 64;
-                    if (row0 < p.m && col0 < p.n) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (wcol + h * 64 < p.n) {
                         const uint32_t buf = next_buffer();
-                        uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + lane * 128);
+                        uint32_t w[32];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(r[8 * j + 2 * e]), __uint_as_float(r[8 * j + 2 * e + 1]));
-                            dst[j ^ (lane & 7)] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, 0);
-                            tma_store_commit();
-                        }
+                        for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                        stage64(w, buf, 0);
+                        store64(buf, wcol + h * 64, 1);
                     }
                 }
             } else {
-                const bool live = row < p.m;
-                // column of the target within this tile (any value outside 0 ... 255 when it lies elsewhere)
-                long long tcol = -1;
-                if (live) tcol = p.target[row] - p.col_base - (long long)nb * XE_BN;
-                if (tcol < 0 || tcol >= XE_BN) tcol = -1;
-                const int tloc = (int)tcol;
-                float lse = 0.f, g = 0.f;
-                if constexpr (EPI == XE_DZ) {
-                    if (live) { lse = p.lse[row]; g = p.rowg[row]; }
-                }
-                float mx = -INFINITY, s = 0.f, zs = 0.f;
-                constexpr int GROUP = EPI == XE_DZ ? 2 : 1;       // 32-column chunks per staging tile
-#pragma unroll 1
-                for (int chunk = 0; chunk < XE_BN / 32; chunk += GROUP) {
-                    uint32_t buf = 0;
-                    const long long gcol0 = (long long)nb * XE_BN + chunk * 32;
-                    const bool gwork = row0 < p.m && gcol0 < p.n;
-                    if constexpr (EPI == XE_DZ) {
-                        if (gwork) buf = next_buffer();
+                const bool live = row < p.m, whole = wcol + XE_WCOLS <= p.n;
+                if (p.bias) {
+                    if (whole) {
+                        const float4* b4 = reinterpret_cast<const float4*>(p.bias + wcol);
+#pragma unroll
+                        for (int j = 0; j < XE_WCOLS / 4; ++j) {
+                            const float4 b = __ldg(b4 + j);
+                            z[4 * j] += b.x;
+                            z[4 * j + 1] += b.y;
+                            z[4 * j + 2] += b.z;
+                            z[4 * j + 3] += b.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < XE_WCOLS; ++i)
+                            if (wcol + i < p.n) z[i] += __ldg(p.bias + wcol + i);
                     }
+                }
+                // column of the target among this warp's, -1 when it lies elsewhere
+                int tc = -1;
+                if (live) {
+                    const long long t = p.target[row] - p.col_base - wcol;
+                    if (t >= 0 && t < XE_WCOLS) tc = (int)t;
+                }
+                const bool here = __any_sync(0xffffffffu, tc >= 0);
+                if constexpr (EPI == XE_STATS || EPI == XE_STATS_E) {
+                    if (here) {
+                        float t = 0.f;
 #pragma unroll
-                    for (int h = 0; h < GROUP; ++h) {
-                        uint32_t r[32];
-                        tmem_ld_32x32(tsrc + (uint32_t)((chunk + h) * 32), r);
-                        tmem_ld_wait();
-                        if (chunk + h == XE_BN / 32 - 1) release();
-                        const long long col0 = gcol0 + h * 32;
-                        if (!gwork) continue;
-                        float z[32];
-                        const bool whole = col0 + 32 <= p.n;
-                        if (p.bias && whole) {
-                            const float4* b4 = reinterpret_cast<const float4*>(p.bias + col0);
+                        for (int i = 0; i < XE_WCOLS; ++i) t = i == tc ? z[i] : t;
+                        if (tc >= 0) p.zt[row] = t;
+                    }
+                    if (p.zsum) {
+                        float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float4 b = __ldg(b4 + j);
-                                z[4 * j] = __uint_as_float(r[4 * j]) + b.x;
-                                z[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + b.y;
-                                z[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + b.z;
-                                z[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + b.w;
-                            }
-                        } else {
+                        for (int i = 0; i < XE_WCOLS; ++i) t[i & 3] += whole || wcol + i < p.n ? z[i] : 0.f;
+                        if (live) p.zsum[wcol / XE_STAT_COLS * p.m + row] = (t[0] + t[1]) + (t[2] + t[3]);
+                    }
+                    if (!whole) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(r[i]);
-                            if (p.bias) {
+                        for (int i = 0; i < XE_WCOLS; ++i) z[i] = wcol + i < p.n ? z[i] : -INFINITY;
+                    }
+                    float cm[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    if (col0 + i < p.n) z[i] += __ldg(p.bias + col0 + i);
+                    for (int i = 4; i < XE_WCOLS; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
+                    const float mx = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3]));
+                    const float ref = mx == -INFINITY ? 0.f : mx;      // nothing but -inf: every term is 0
+                    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < XE_WCOLS; ++i) {
+                        z[i] = xe_ex2((z[i] - ref) * XE_LOG2E);
+                        t[i & 3] += z[i];
+                    }
+                    if (live) p.stats[wcol / XE_STAT_COLS * p.m + row] = make_float2(mx, (t[0] + t[1]) + (t[2] + t[3]));
+                    if constexpr (EPI == XE_STATS_E) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (wcol + h * 64 < p.n) {
+                                const uint32_t buf = next_buffer();
+                                uint32_t w[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                stage64(w, buf, 0);
+                                store64(buf, wcol + h * 64, 1);
                             }
                         }
-                        const int tc = tloc - (chunk + h) * 32;
-                        const bool here = __any_sync(0xffffffffu, tc >= 0 && tc < 32);
-                        if constexpr (EPI == XE_STATS) {
-                            if (here) {
-                                float t = 0.f;
+                    }
+                } else {
+                    float lse = 0.f, g = 0.f;
+                    if (live) { lse = p.lse[row]; g = p.rowg[row]; }
+                    const float gp = g * p.rule.pf, ga = g * p.rule.smooth_all;
+                    // a row that does not count: exactly 0, whatever its logits
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) t = i == tc ? z[i] : t;
-                                if (tc >= 0 && tc < 32) p.zt[row] = t;
-                            }
-                            if (p.zsum) {
-                                float t = 0.f;
+                    for (int i = 0; i < XE_WCOLS; ++i) z[i] = g == 0.f ? 0.f : gp * xe_ex2((z[i] - lse) * XE_LOG2E) - ga;
+                    if (here) {
+                        const float gt = g * p.rule.smooth_t;
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) t += whole || col0 + i < p.n ? z[i] : 0.f;
-                                zs += t;
-                            }
-                            if (!whole) {
+                        for (int i = 0; i < XE_WCOLS; ++i) z[i] = i == tc ? z[i] - gt : z[i];
+                    }
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) z[i] = col0 + i < p.n ? z[i] : -INFINITY;
-                            }
-                            float cm[4] = {z[0], z[1], z[2], z[3]};
+                    for (int h = 0; h < 2; ++h) {
+                        if (wcol + h * 64 < p.n) {
+                            const uint32_t buf = next_buffer();
+                            uint32_t w[32];
+                            if constexpr (PLANES == 1) {
 #pragma unroll
-                            for (int i = 4; i < 32; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
-                            const float m2 = fmaxf(fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])), mx);
-                            const float ref = m2 == -INFINITY ? 0.f : m2;      // nothing but -inf so far: every term is 0
-                            s *= xe_ex2((mx - ref) * XE_LOG2E);
-                            mx = m2;
-                            float t[4] = {0.f, 0.f, 0.f, 0.f};
+                                for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                stage64(w, buf, 0);
+                                store64(buf, wcol + h * 64, 1);
+                                if (p.db_part) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) t[i & 3] += xe_ex2((z[i] - ref) * XE_LOG2E);
-                            s += (t[0] + t[1]) + (t[2] + t[3]);
-                        } else {
+                                    for (int k = 0; k < 2; ++k) {
+                                        const long long col = wcol + h * 64 + k * 32 + lane;
+                                        const float cs = column_sums(&z[64 * h + 32 * k], lane);
+                                        if (col < p.n) p.db_part[(row0 / 32) * p.db_pitch + col] = cs;
+                                    }
+                                }
+                            } else {
+                                if (p.db_part) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) z[i] = g * (xe_ex2((z[i] - lse) * XE_LOG2E) - p.smooth_all);
-                            if (here) {
+                                    for (int k = 0; k < 2; ++k) {
+                                        float c[32];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) z[i] = i == tc ? z[i] - g * p.smooth_t : z[i];
-                            }
-                            if (g == 0.f) {                       // a row that does not count: exactly 0, whatever its logits
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) z[i] = 0.f;
-                            }
-                            uint8_t* tile = stage_gen + buf * L::BUF + lane * 128;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t w[PLANES][4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const float v0 = z[8 * j + 2 * e], v1 = z[8 * j + 2 * e + 1];
-                                    if constexpr (PLANES == 1) {
-                                        w[0][e] = pack_bf16(v0, v1);
-                                    } else {
-                                        float r0 = v0, r1 = v1;
-#pragma unroll
-                                        for (int q = 0; q < PLANES; ++q) {
-                                            w[q][e] = pack_bf16(r0, r1);
-                                            r0 -= __uint_as_float(w[q][e] << 16);
-                                            r1 -= __uint_as_float(w[q][e] & 0xffff0000u);
-                                        }
+                                        for (int i = 0; i < 32; ++i) c[i] = z[64 * h + 32 * k + i];
+                                        const long long col = wcol + h * 64 + k * 32 + lane;
+                                        const float cs = column_sums(c, lane);
+                                        if (col < p.n) p.db_part[(row0 / 32) * p.db_pitch + col] = cs;
                                     }
                                 }
 #pragma unroll
-                                for (int q = 0; q < PLANES; ++q)
-                                    reinterpret_cast<uint4*>(tile + q * XE_STAGE_TILE)[(4 * h + j) ^ (lane & 7)] =
-                                        make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
-                            }
-                            if (p.db_part) {
-                                const float cs = column_sums(z, lane);
-                                if (col0 + lane < p.n) p.db_part[(row0 / 32) * p.db_pitch + col0 + lane] = cs;
-                            }
-                        }
-                    }
-                    if constexpr (EPI == XE_DZ) {
-                        if (gwork) {
-                            fence_async_shared();
-                            __syncwarp();
-                            if (lane == 0) {
+                                for (int q = 0; q < PLANES; ++q) {        // round, keep the remainder for the next plane
 #pragma unroll
-                                for (int q = 0; q < PLANES; ++q)
-                                    tma_store_3d(&tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)gcol0, (int)row0, q);
-                                tma_store_commit();
+                                    for (int i = 0; i < 32; ++i) {
+                                        w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                        z[64 * h + 2 * i] -= __uint_as_float(w[i] << 16);
+                                        z[64 * h + 2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+                                    }
+                                    stage64(w, buf, q);
+                                }
+                                store64(buf, wcol + h * 64, PLANES);
                             }
                         }
-                    }
-                }
-                if constexpr (EPI == XE_STATS) {
-                    if (live) {
-                        p.stats[(long long)nb * p.m + row] = make_float2(mx, s);
-                        if (p.zsum) p.zsum[(long long)nb * p.m + row] = zs;
                     }
                 }
             }
-            as ^= 1;
-            if (as == 0) aphase ^= 1;
         }
         if (lane == 0) tma_store_wait_all();
     }
@@ -521,6 +540,7 @@ int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m,
     p.nblocks = (int)((n + XE_BN - 1) / XE_BN);
     p.kchunks = (int)((k + XE_BK - 1) / XE_BK);
     p.splits = out.splits;
+    p.block = a.planes == 3 ? 4 : 16;
     if (a.planes == 3) {
         static const unsigned char pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
         p.pairs = 6;
@@ -531,13 +551,15 @@ int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m,
     p.idesc = make_idesc(OP_BF16, XE_BN, XE_BM) | (a.along_rows ? 1u << 15 : 0u) | (b.along_rows ? 1u << 16 : 0u);
     if ((rc = status_word(&p.status))) return rc;
     p.add = out.add;
+    p.scale = out.scale;
     p.bias = out.bias; p.target = out.target; p.col_base = out.col_base;
     p.stats = out.stats; p.zsum = out.zsum; p.zt = out.zt;
-    p.lse = out.lse; p.rowg = out.rowg; p.smooth_t = out.smooth_t; p.smooth_all = out.smooth_all;
+    p.lse = out.lse; p.rowg = out.rowg; p.rule = out.rule;
     p.db_part = out.db_part; p.db_pitch = out.db_pitch;
     if (!a.along_rows && !b.along_rows) {
         if (epi == XE_F32) return run<XE_F32, 1, false, false>(tm_a, tm_b, tm_out, p, st);
         if (epi == XE_STATS) return run<XE_STATS, 1, false, false>(tm_a, tm_b, tm_out, p, st);
+        if (epi == XE_STATS_E) return run<XE_STATS_E, 1, false, false>(tm_a, tm_b, tm_out, p, st);
         if (epi == XE_DZ) return a.planes == 3 ? run<XE_DZ, 3, false, false>(tm_a, tm_b, tm_out, p, st) : run<XE_DZ, 1, false, false>(tm_a, tm_b, tm_out, p, st);
     } else if (!a.along_rows) {
         if (epi == XE_F32) return run<XE_F32, 1, false, true>(tm_a, tm_b, tm_out, p, st);

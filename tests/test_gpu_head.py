@@ -85,6 +85,9 @@ class Case:
         e32[~counts] = 0
         # an exponential below 2^-126 is flushed to 0, and so may be a part of a split value: at most 4 * 2^-126 in dz
         # before the row's weight (logits thousands apart make such values, and x of thousands carries them into dW)
+        # Without a bias BF16 may hold the exponentials before dz is made of them: one more rounding of p.
+        if self.dtype == "bf16" and self.bd is None:
+            e32 = e32 + np.abs(g)[:, None] * BF * 1.01 * p * counts[:, None]
         edz = e32 + store * (np.abs(ref["dz"]) + e32) + (np.abs(g) * counts)[:, None] * 2.0 ** -124
         adz = np.abs(ref["dz"]) + edz
         out = BF if self.dtype == "bf16" else F32
@@ -116,7 +119,12 @@ CASES = [
     (300, 201, 1100, "fp32", dict(ldx=204, ldw=201)),
     (2305, 40, 2100, "bf16", {}),                                 # statistics in the epilogue, logits recomputed
     (2305, 40, 2100, "fp32", {}),
-    (2304, 1024, 2050, "bf16", dict(bias=False)),                 # logits kept, contraction not split
+    (2304, 1024, 2050, "bf16", {}),                               # logits kept as floats, contraction not split
+    (2304, 300, 2050, "fp32", {}),
+    (2304, 1024, 2050, "bf16", dict(bias=False)),                 # logits kept as exponentials
+    (2500, 24, 2303, "bf16", dict(bias=False)),
+    (300, 2200, 700, "bf16", dict(bias=False)),                   # blocks of the contraction: 1024 + 1024 + 152
+    (2100, 700, 2400, "fp32", {}),                                # 256 + 256 + 188, logits recomputed below
     (4000, 64, 5, "bf16", {}),                                    # long contraction of dW over rows, few classes
     (5, 48, 20000, "fp32", {}),                                   # long contraction of dx over classes, few rows
 ]

@@ -94,7 +94,7 @@ def test_xent_scratch_is_bounded():
     L = cb.lib()
     s = _desc(n=4096, d=512, v=65536, scratch_limit=64 << 20)
     small = L.wino_xent_workspace_bytes(ctypes.byref(s), 1)
-    stats = 65536 // 256 * 4096 * 8
+    stats = 65536 // 128 * 4096 * 8
     assert small <= (64 << 20) + stats + 5 * 4096 * 4 + 74 * 256 * 256 * 4 + (1 << 16)
     s.scratch_limit = 0
     assert L.wino_xent_workspace_bytes(ctypes.byref(s), 1) > small
