@@ -14,6 +14,7 @@
 // read) or as three BF16 parts (FP32X3).  dbias sums the unrounded dz.  Statistics, lse and losses are FP32, the sum over
 // rows FP64.
 #include <cmath>
+#include <cstring>
 
 #include "xent.cuh"
 
@@ -32,26 +33,43 @@ __host__ __device__ inline bool row_ignored(const RowRule& r, long long t) { ret
 __host__ __device__ inline bool row_counts(const RowRule& r, long long t) { return !row_ignored(r, t) && t >= 0 && t < r.v; }
 
 // ---- operand packing ---------------------------------------------------------------------------------------
-// src (rows x cols, pitch ld) -> PLANES x rows x pitch BF16; rows that do not count become zero where target is given
+struct PackJob {
+    const void* src;
+    long long ld, rows;
+    __nv_bfloat16* dst;
+    const long long* target;            // rows that do not count become zero where target is given
+};
+// src (rows x cols, pitch ld) -> PLANES x rows x pitch BF16, four columns per thread, for up to two matrices
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) xe_pack_kernel(const T* __restrict__ src, long long ld, __nv_bfloat16* __restrict__ dst, long long rows,
-                                                      int cols, int pitch, const long long* __restrict__ target, const RowRule rule) {
-    const int quads = pitch / 4;
-    const long long total = rows * quads;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / quads;
+__global__ void __launch_bounds__(256) xe_pack_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const unsigned quads = (unsigned)pitch / 4;
+    const long long items0 = j0.rows * quads, total = items0 + j1.rows * quads;
+    for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < total; k += (long long)gridDim.x * 256) {
+        const bool second = k >= items0;
+        const PackJob& j = second ? j1 : j0;
+        const long long i = second ? k - items0 : k;
+        const long long r = i < (1ll << 32) ? (long long)((unsigned)i / quads) : i / quads;
         const int c = (int)(i - r * quads) * 4;
-        const bool live = !target || row_counts(rule, target[r]);
+        const bool live = !j.target || row_counts(rule, j.target[r]);
+        const T* src = static_cast<const T*>(j.src) + r * j.ld + c;
+        T v[4];
+        if (live && sizeof(T) == 4 && c + 4 <= cols && ((uintptr_t)src & 15) == 0) {
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = live && c + e < cols ? src[e] : from_float<T>(0.f);
+        }
         __nv_bfloat16 part[PLANES][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const T v = live && c + e < cols ? src[r * ld + c + e] : from_float<T>(0.f);
-            if constexpr (PLANES == 3) xe_split3(to_float<T>(v), part[0][e], part[1][e], part[2][e]);
-            else part[0][e] = __float2bfloat16_rn(to_float<T>(v));
+            if constexpr (PLANES == 3) xe_split3(to_float<T>(v[e]), part[0][e], part[1][e], part[2][e]);
+            else part[0][e] = __float2bfloat16_rn(to_float<T>(v[e]));
         }
 #pragma unroll
         for (int q = 0; q < PLANES; ++q)
-            *reinterpret_cast<uint2*>(dst + (q * rows + r) * pitch + c) = *reinterpret_cast<const uint2*>(part[q]);
+            *reinterpret_cast<uint2*>(j.dst + (q * j.rows + r) * pitch + c) = *reinterpret_cast<const uint2*>(part[q]);
     }
 }
 
@@ -60,18 +78,23 @@ struct RowArgs {
     RowRule rule;
     long long n;
     const long long* target;
+    const float* dloss;         // n upstream gradients (WINO_NONE), or NULL
     float smooth;               // s
     float inv_v;                // 1 / v
     float* lse;                 // scratch
     float* lse_out;             // caller's, or NULL
-    float* rowloss;
+    float* rowloss;             // scratch, or the caller's (WINO_NONE)
+    float* rowg;                // a row's own weight in the gradient; 0: does not count
+    float* loss;                // mean or sum, written by the block that finishes last; NULL: left to the rows
+    int mean;
+    int* count;                 // [0] rows that count, [1] blocks that are done (both set to 0 by the kernel before)
     int* status;
 };
 
-__device__ __forceinline__ void finish_row(const RowArgs& a, long long row, float m, float s, float zsum, float zt) {
+// one thread per row: loss, lse, weight.  Returns whether the row counts.
+__device__ __forceinline__ bool finish_row(const RowArgs& a, long long row, float lse, float zsum, float zt) {
     const long long t = a.target[row];
     const bool counts = row_counts(a.rule, t);
-    const float lse = m + logf(s);
     float loss = (1.f - a.smooth) * (lse - zt);
     if (a.smooth > 0.f) loss += a.smooth * (lse - zsum * a.inv_v);
     if (!counts) {
@@ -80,7 +103,35 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, long long row, floa
     }
     a.lse[row] = lse;
     a.rowloss[row] = loss;
+    a.rowg[row] = counts ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
     if (a.lse_out) a.lse_out[row] = counts ? lse : 0.f;
+    return counts;
+}
+
+// The block that finishes last sums the rows' losses (in the same order whichever block that is).  All threads call it.
+template <int THREADS>
+__device__ __forceinline__ void finish_loss(const RowArgs& a) {
+    if (!a.loss) return;
+    __shared__ int last;
+    __shared__ double rs[THREADS / 32];
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.count + 1, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double sum = 0;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < a.n; i += THREADS) sum += __ldcg(a.rowloss + i);
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if (threadIdx.x % 32 == 0) rs[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < THREADS / 32; ++i) sum += rs[i];
+        const int count = __ldcg(a.count);
+        *a.loss = (float)(a.mean ? sum / (count > 0 ? count : 1) : sum);
+    }
 }
 
 // joins (maximum, sum) pairs
@@ -90,64 +141,255 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = mm;
 }
 
-// 32 rows x 8 threads per row over the column tiles' statistics
+// 32 rows x 8 threads per row over the column tiles' statistics, eight tiles in flight per thread
 __global__ void __launch_bounds__(256) xe_rows_from_stats_kernel(const float2* __restrict__ stats, const float* __restrict__ zsum,
                                                                  const float* __restrict__ zt, int tiles, const RowArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
     __shared__ float2 red[8][32];
     __shared__ float redz[8][32];
     const int l = threadIdx.x % 32, g = threadIdx.x / 32;
     const long long row = (long long)blockIdx.x * 32 + l;
     float m = -INFINITY, s = 0.f, z = 0.f;
     if (row < a.n) {
-        for (int i = g; i < tiles; i += 8) {
-            const float2 v = stats[(long long)i * a.n + row];
-            join(m, s, v.x, v.y);
-            if (zsum) z += zsum[(long long)i * a.n + row];
+        for (int i = g; i < tiles; i += 64) {
+            float2 v[8];
+            float mm = m;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = i + 8 * e < tiles ? stats[(long long)(i + 8 * e) * a.n + row] : make_float2(-INFINITY, 0.f);
+                mm = fmaxf(mm, v[e].x);
+            }
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            s *= xe_ex2((m - ref) * XE_LOG2E);
+            m = mm;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[e].y * xe_ex2((v[e].x - ref) * XE_LOG2E);
+            if (zsum) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (i + 8 * e < tiles) z += zsum[(long long)(i + 8 * e) * a.n + row];
+            }
         }
     }
     red[g][l] = make_float2(m, s);
     redz[g][l] = z;
     __syncthreads();
-    if (g == 0 && row < a.n) {
-        for (int i = 1; i < 8; ++i) {
-            join(m, s, red[i][l].x, red[i][l].y);
-            z += redz[i][l];
+    if (g == 0) {
+        bool counts = false;
+        if (row < a.n) {
+            for (int i = 1; i < 8; ++i) {
+                join(m, s, red[i][l].x, red[i][l].y);
+                z += redz[i][l];
+            }
+            counts = finish_row(a, row, m + logf(s), z, row_counts(a.rule, a.target[row]) ? zt[row] : 0.f);
         }
-        finish_row(a, row, m, s, z, row_counts(a.rule, a.target[row]) ? zt[row] : 0.f);
+        const unsigned live = __ballot_sync(0xffffffffu, counts);
+        if (l == 0) atomicAdd(a.count, __popc(live));
+    }
+    finish_loss<256>(a);
+}
+
+// bias of columns c ... c + 3 (c a multiple of 4, the base 16-byte aligned); columns past v become -inf
+__device__ __forceinline__ void add_bias(float (&e)[4], int c, int v, const float* __restrict__ bias) {
+    if (c + 4 <= v) {
+        if (bias) {
+            const float4 b = __ldg(reinterpret_cast<const float4*>(bias + c));
+            e[0] += b.x; e[1] += b.y; e[2] += b.z; e[3] += b.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (c + k >= v) e[k] = -INFINITY;
+            else if (bias) e[k] += bias[c + k];
+        }
     }
 }
 
-// one block per row over `splits` partial logits: their sum (with the bias) replaces the first part
-__global__ void __launch_bounds__(128) xe_rows_from_logits_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias,
-                                                                  const RowArgs a) {
-    __shared__ float red[3][4];
+// sum of the parts of four logits and the bias
+__device__ __forceinline__ void gather_logits(float (&e)[4], const float* zr, long long plane, int splits, int c, int v,
+                                              const float* __restrict__ bias) {
+    float4 q = *reinterpret_cast<const float4*>(zr + c);
+    for (int i = 1; i + 8 <= splits; i += 8) {
+        float4 o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = *reinterpret_cast<const float4*>(zr + (i + k) * plane + c);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { q.x += o[k].x; q.y += o[k].y; q.z += o[k].z; q.w += o[k].w; }
+    }
+    {
+        const int i0 = 1 + (splits - 1) / 8 * 8;
+        float4 o[7];                                     // the rest, in flight together
+#pragma unroll
+        for (int k = 0; k < 7; ++k)
+            if (i0 + k < splits) o[k] = *reinterpret_cast<const float4*>(zr + (i0 + k) * plane + c);
+#pragma unroll
+        for (int k = 0; k < 7; ++k)
+            if (i0 + k < splits) { q.x += o[k].x; q.y += o[k].y; q.z += o[k].z; q.w += o[k].w; }
+    }
+    e[0] = q.x; e[1] = q.y; e[2] = q.z; e[3] = q.w;
+    add_bias(e, c, v, bias);
+}
+
+// logits of `count` groups of four columns, `step` columns apart; all loads of an unsplit product in flight together
+template <bool SPLIT, int COUNT>
+__device__ __forceinline__ void gather_groups(float (&e)[COUNT][4], const float* zr, long long plane, int splits, int c0, int step, int v,
+                                              const float* __restrict__ bias) {
+    if constexpr (!SPLIT) {
+        float4 q[COUNT];
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i)
+            if (c0 + i * step < v) q[i] = *reinterpret_cast<const float4*>(zr + c0 + i * step);
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            e[i][0] = q[i].x; e[i][1] = q[i].y; e[i][2] = q[i].z; e[i][3] = q[i].w;
+            add_bias(e[i], c0 + i * step, v, bias);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const int c = c0 + i * step;
+            if (c < v) gather_logits(e[i], zr, plane, splits, c, v, bias);
+            else e[i][0] = e[i][1] = e[i][2] = e[i][3] = -INFINITY;
+        }
+    }
+}
+
+// Kept logits -> lse, loss and dz (PLANES BF16 planes; 0: floats, which may replace the first part of the logits) in one go.  A block takes a run of rows; a thread holds the same 4 * QUADS columns of each
+// in registers, from the sum of the parts to dz, and their column sums over the run.  v <= 4 * THREADS * QUADS.
+// 1024 threads an SM (64 registers), half of that where the parts of several groups of columns are in flight.
+template <int THREADS, int QUADS, int PLANES, bool GRAD, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, (SPLIT && QUADS > 1 ? 512 : 1024) / THREADS) xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
+                                                          const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int WARPS = THREADS / 32;
+    __shared__ float red[2][3][WARPS];          // two sets, used by turns: a row's second barrier frees the other set
+    __shared__ float zt_s;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const long long r0 = blockIdx.x * a.n / gridDim.x, r1 = (blockIdx.x + 1) * a.n / gridDim.x, plane = a.n * zpitch;
+    float sums[GRAD ? QUADS : 1][4];
+#pragma unroll
+    for (int q = 0; q < (GRAD ? QUADS : 1); ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[q][k] = 0.f;
+    int live = 0;
+    for (long long row = r0; row < r1; ++row) {
+        const bool counts = row_counts(a.rule, a.target[row]);
+        const int t = counts ? (int)a.target[row] : -1;
+        float e[QUADS][4], m = -INFINITY, zsum = 0.f;
+        gather_groups<SPLIT>(e, z + row * zpitch, plane, splits, threadIdx.x * 4, THREADS * 4, v, bias);
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) {
+            const int c = (q * THREADS + threadIdx.x) * 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                m = fmaxf(m, e[q][k]);
+                if (c + k < v) zsum += e[q][k];
+                if (c + k == t) zt_s = e[q][k];
+            }
+        }
+#pragma unroll
+        for (int w = 16; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        if (lane == 0) red[row & 1][0][warp] = m;
+        __syncthreads();
+        m = red[row & 1][0][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) m = fmaxf(m, red[row & 1][0][w]);
+        const float ref = m == -INFINITY ? 0.f : m, zt = zt_s;
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += xe_ex2((e[q][k] - ref) * XE_LOG2E);
+#pragma unroll
+        for (int w = 16; w >= 1; w >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, w);
+            zsum += __shfl_xor_sync(0xffffffffu, zsum, w);
+        }
+        if (lane == 0) { red[row & 1][1][warp] = s; red[row & 1][2][warp] = zsum; }
+        __syncthreads();
+        s = red[row & 1][1][0];
+        zsum = red[row & 1][2][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) { s += red[row & 1][1][w]; zsum += red[row & 1][2][w]; }
+        const float lse = m + logf(s);
+        if (threadIdx.x == 0) live += finish_row(a, row, lse, zsum, counts ? zt : 0.f);
+        if constexpr (GRAD) {
+            const float g = counts ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
+#pragma unroll
+            for (int q = 0; q < QUADS; ++q) {
+                const int c = (q * THREADS + threadIdx.x) * 4;
+                if (c < v) {
+                    float d[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        d[k] = xe_ex2((e[q][k] - lse) * XE_LOG2E) * rule.pf - rule.smooth_all;
+                        if (c + k == t) d[k] -= rule.smooth_t;
+                        d[k] = g == 0.f || c + k >= v ? 0.f : d[k] * g;      // a row that does not count: exactly 0, whatever its logits
+                        sums[q][k] += d[k];
+                    }
+                    if constexpr (PLANES == 0) *reinterpret_cast<float4*>(static_cast<float*>(dz) + row * dpitch + c) = make_float4(d[0], d[1], d[2], d[3]);
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(d[0], d[1]), hi = __floats2bfloat162_rn(d[2], d[3]);
+                        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(dz) + (p * a.n + row) * dpitch + c) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                        d[0] -= __low2float(lo); d[1] -= __high2float(lo);
+                        d[2] -= __low2float(hi); d[3] -= __high2float(hi);
+                    }
+                }
+            }
+        }
+    }
+    if (threadIdx.x == 0 && live) atomicAdd(a.count, live);
+    if constexpr (GRAD && PLANES > 0) {
+        if (db_part) {
+#pragma unroll
+            for (int q = 0; q < QUADS; ++q) {
+                const int c = (q * THREADS + threadIdx.x) * 4;
+                if (c < v) *reinterpret_cast<float4*>(db_part + (long long)blockIdx.x * dpitch + c) = make_float4(sums[q][0], sums[q][1], sums[q][2], sums[q][3]);
+            }
+        }
+    }
+    finish_loss<THREADS>(a);
+}
+
+// The same for any v, in two kernels: one block per row for the statistics (the sum of several parts replaces the first), ...
+template <bool SPLIT>
+__global__ void __launch_bounds__(256, SPLIT ? 1 : 4) xe_wide_rows_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, const RowArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float red[3][8];
     __shared__ float zt_s;
     const long long row = blockIdx.x;
-    const long long t = a.target[row];
+    const bool counts = row_counts(a.rule, a.target[row]);
+    const int t = counts ? (int)a.target[row] : -1;
     float* zr = z + row * pitch;
-    const long long plane = a.n * pitch;
     float m = -INFINITY, s = 0.f, zsum = 0.f;
     if (threadIdx.x == 0) zt_s = 0.f;
     __syncthreads();
-    for (int c = threadIdx.x * 4; c < v; c += 512) {
-        float4 q = *reinterpret_cast<const float4*>(zr + c);
-        for (int i = 1; i < splits; ++i) {
-            const float4 o = *reinterpret_cast<const float4*>(zr + i * plane + c);
-            q.x += o.x; q.y += o.y; q.z += o.z; q.w += o.w;
-        }
-        float e[4] = {q.x, q.y, q.z, q.w};
+    // four groups of four columns at a time, so that their loads overlap and the running maximum moves once
+    for (int c0 = threadIdx.x * 4; c0 < v; c0 += 4096) {
+        float e[4][4], m2 = m;
+        gather_groups<SPLIT>(e, zr, a.n * pitch, splits, c0, 1024, v, bias);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = c + i < v;
-            if (bias && in) e[i] += bias[c + i];
-            if (in) zsum += e[i];
-            if (c + i == t) zt_s = e[i];
-            if (!in) e[i] = -INFINITY;
+        for (int q = 0; q < 4; ++q) {
+            const int c = c0 + q * 1024;
+            if (SPLIT && c < v) *reinterpret_cast<float4*>(zr + c) = make_float4(e[q][0], e[q][1], e[q][2], e[q][3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (c + i < v) zsum += e[q][i];
+                if (c + i == t) zt_s = e[q][i];
+                m2 = fmaxf(m2, e[q][i]);
+            }
         }
-        *reinterpret_cast<float4*>(zr + c) = make_float4(e[0], e[1], e[2], e[3]);
-        const float cm = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), m2 = fmaxf(m, cm), ref = m2 == -INFINITY ? 0.f : m2;
-        s = s * xe_ex2((m - ref) * XE_LOG2E) + ((xe_ex2((e[0] - ref) * XE_LOG2E) + xe_ex2((e[1] - ref) * XE_LOG2E)) +
-                                                (xe_ex2((e[2] - ref) * XE_LOG2E) + xe_ex2((e[3] - ref) * XE_LOG2E)));
+        const float ref = m2 == -INFINITY ? 0.f : m2;
+        s *= xe_ex2((m - ref) * XE_LOG2E);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += xe_ex2((e[q][i] - ref) * XE_LOG2E);
         m = m2;
     }
 #pragma unroll
@@ -163,68 +405,38 @@ __global__ void __launch_bounds__(128) xe_rows_from_logits_kernel(float* __restr
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 4; ++i) {
+        for (int i = 1; i < 8; ++i) {
             join(m, s, red[0][i], red[1][i]);
             zsum += red[2][i];
         }
-        finish_row(a, row, m, s, zsum, zt_s);
+        if (finish_row(a, row, m + logf(s), zsum, zt_s)) atomicAdd(a.count, 1);
     }
+    finish_loss<256>(a);
 }
 
-// one block: loss over the rows; every row's own weight in the gradient (rowg) and the factor they share (scale), to which
-// dz_factor (XeDzRule's f) belongs
-__global__ void __launch_bounds__(1024) xe_loss_kernel(const RowArgs a, int reduction, const float* __restrict__ dloss, float dz_factor,
-                                                       float* __restrict__ loss, float* __restrict__ rowg, float* __restrict__ scale) {
-    __shared__ double rs[32];
-    __shared__ long long rc[32];
-    double sum = 0;
-    long long count = 0;
-    for (long long i = threadIdx.x; i < a.n; i += 1024) {
-        const float l = a.rowloss[i];
-        sum += l;
-        count += row_counts(a.rule, a.target[i]);
-        if (reduction == WINO_NONE) loss[i] = l;
-    }
-#pragma unroll
-    for (int w = 16; w >= 1; w >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        count += __shfl_xor_sync(0xffffffffu, count, w);
-    }
-    if (threadIdx.x % 32 == 0) { rs[threadIdx.x / 32] = sum; rc[threadIdx.x / 32] = count; }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 32; ++i) { sum += rs[i]; count += rc[i]; }
-        const double inv = reduction == WINO_MEAN ? 1.0 / (double)(count > 0 ? count : 1) : 1.0;
-        if (reduction != WINO_NONE) loss[0] = (float)(sum * inv);
-        if (rowg) scale[0] = (float)(inv * dz_factor * (dloss && reduction != WINO_NONE ? (double)dloss[0] : 1.0));
-    }
-    if (!rowg) return;
-    for (long long i = threadIdx.x; i < a.n; i += 1024) {
-        const float own = dloss && reduction == WINO_NONE ? dloss[i] : 1.f;
-        rowg[i] = row_counts(a.rule, a.target[i]) ? own : 0.f;
-    }
-}
-
-// dz of kept logits: two classes per thread, 32 rows per block, and the block's column sums
+// ... and dz, two classes per thread, 32 rows per block, with the block's column sums.  bias: NULL where z has it already
 template <int PLANES>
-__global__ void __launch_bounds__(128) xe_dz_from_logits_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ lse,
-                                                                const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
-                                                                __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
+__global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ bias, const float* __restrict__ lse,
+                                                         const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
+                                                         __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
+    pdl_launch_dependents();
+    pdl_wait();
     const unsigned cblocks = (unsigned)(v + 255) / 256, part = blockIdx.x / cblocks;
     const int c = (int)((blockIdx.x % cblocks) * 128 + threadIdx.x) * 2;
     if (c >= v) return;
     const long long r0 = (long long)part * XE_ROWS_PER_PART;
     const long long r1 = r0 + XE_ROWS_PER_PART < n ? r0 + XE_ROWS_PER_PART : n;
     float s0 = 0.f, s1 = 0.f;
-#pragma unroll 4
+    const float b0 = bias ? bias[c] : 0.f, b1 = bias && c + 1 < v ? bias[c + 1] : 0.f;
+#pragma unroll 8
     for (long long r = r0; r < r1; ++r) {
         const float2 q = *reinterpret_cast<const float2*>(z + r * zpitch + c);
         const float l = lse[r], g = rowg[r];
         const long long t = target[r];
-        float a = xe_ex2((q.x - l) * XE_LOG2E) * rule.pf - rule.smooth_all, b = xe_ex2((q.y - l) * XE_LOG2E) * rule.pf - rule.smooth_all;
+        float a = xe_ex2((q.x + b0 - l) * XE_LOG2E) * rule.pf - rule.smooth_all, b = xe_ex2((q.y + b1 - l) * XE_LOG2E) * rule.pf - rule.smooth_all;
         if (t == c) a -= rule.smooth_t;
         if (t == c + 1) b -= rule.smooth_t;
-        a = g == 0.f ? 0.f : a * g;                       // a row that does not count: exactly 0, whatever its logits
+        a = g == 0.f ? 0.f : a * g;
         b = g == 0.f || c + 1 >= v ? 0.f : b * g;
         s0 += a;
         s1 += b;
@@ -244,47 +456,68 @@ __global__ void __launch_bounds__(128) xe_dz_from_logits_kernel(const float* __r
 __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __restrict__ dz, int pitch, long long n, const float2* __restrict__ stats,
                                                              const float* __restrict__ zt, const float* __restrict__ lse, const float* __restrict__ rowg,
                                                              const long long* __restrict__ target, const XeDzRule rule) {
-    const int octs = pitch / 8;
-    const long long total = n * octs;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / octs;
-        const int c = (int)(i - r * octs) * 8;
-        uint4* at = reinterpret_cast<uint4*>(dz + r * pitch + c);
-        const float g = rowg[r];
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (g != 0.f) {
-            q = *at;
-            const float l = lse[r], f = xe_ex2((stats[c / XE_STAT_COLS * n + r].x - l) * XE_LOG2E) * rule.pf;
-            const long long t = target[r] - c;
-            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    pdl_launch_dependents();
+    pdl_wait();
+    // a block takes 256 x 4 groups of a row at a time: one division per block, four loads in flight per thread
+    const int octs = pitch / 8, spans = (octs + 1023) / 1024;
+    for (long long b = blockIdx.x; b < n * spans; b += gridDim.x) {
+        const long long r = b / spans;
+        const int o0 = (int)(b - r * spans) * 1024 + threadIdx.x;
+        uint4* at = reinterpret_cast<uint4*>(dz + r * pitch);
+        const float g = rowg[r], l = lse[r];
+        const long long t = target[r];
+        uint4 q[4];
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int o = o0 + i * 256;
+            if (o < octs && g != 0.f) {
+                q[i] = at[o];
+                f[i] = stats[(long long)(o / (XE_STAT_COLS / 8)) * n + r].x;
+            }
+        }
+        const float pt = g != 0.f ? g * (xe_ex2((zt[r] - l) * XE_LOG2E) * rule.pf - rule.smooth_all - rule.smooth_t) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int o = o0 + i * 256;
+            if (o >= octs) continue;
+            if (g == 0.f) { at[o] = make_uint4(0, 0, 0, 0); continue; }
+            const float h = xe_ex2((f[i] - l) * XE_LOG2E) * rule.pf;
+            uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float a = __uint_as_float(w[e] << 16) * f - rule.smooth_all, b = __uint_as_float(w[e] & 0xffff0000u) * f - rule.smooth_all;
-                if (t >> 1 == e) {
-                    const float pt = xe_ex2((zt[r] - l) * XE_LOG2E) * rule.pf - rule.smooth_all - rule.smooth_t;
-                    if (t & 1) b = pt; else a = pt;
-                }
-                const __nv_bfloat162 o = __floats2bfloat162_rn(a * g, b * g);
-                w[e] = *reinterpret_cast<const uint32_t*>(&o);
+                const __nv_bfloat162 v = __floats2bfloat162_rn((__uint_as_float(w[e] << 16) * h - rule.smooth_all) * g,
+                                                               (__uint_as_float(w[e] & 0xffff0000u) * h - rule.smooth_all) * g);
+                w[e] = *reinterpret_cast<const uint32_t*>(&v);
             }
-            q = make_uint4(w[0], w[1], w[2], w[3]);
+            if (t >> 3 == o) {                            // the target's own value
+                const uint32_t b16 = __bfloat16_as_ushort(__float2bfloat16_rn(pt));
+                const int e = (int)(t & 7);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (e >> 1 == k) w[k] = e & 1 ? (w[k] & 0xffffu) | b16 << 16 : (w[k] & 0xffff0000u) | b16;
+            }
+            at[o] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        *at = q;
     }
 }
 
-__global__ void __launch_bounds__(256) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, const float* __restrict__ scale,
-                                                    float* __restrict__ db) {
-    __shared__ float red[8][32];
+// dbias from the column sums of runs of rows, 32 columns per block
+__global__ void __launch_bounds__(512) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, const XeScale scale, float* __restrict__ db) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float red[16][32];
     const int l = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + l;
     float s = 0.f;
-    if (c < cols)
-        for (int i = g; i < parts; i += 8) s += part[(long long)i * pitch + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = g; i < parts; i += 16) s += part[(long long)i * pitch + c];
+    }
     red[g][l] = s;
     __syncthreads();
     if (g == 0 && c < cols) {
-        for (int i = 1; i < 8; ++i) s += red[i][l];
-        db[c] = s * *scale;
+        for (int i = 1; i < 16; ++i) s += red[i][l];
+        db[c] = s * xe_scale(scale);
     }
 }
 
@@ -292,6 +525,8 @@ __global__ void __launch_bounds__(256) xe_db_kernel(const float* __restrict__ pa
 template <typename T>
 __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict__ part, int splits, long long rows, int cols, int pitch, T* __restrict__ out,
                                                         long long ld) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int quads = (cols + 3) / 4;
     const long long total = rows * quads, plane = rows * pitch;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
@@ -309,37 +544,197 @@ __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict_
     }
 }
 
+// ---- few products: FP32 arithmetic on the caller's matrices --------------------------------------------------
+// Below some millions of products a tensor-core launch is mostly set-up (8 us each with one tile), and the operands fit
+// the L2 many times over: three plain kernels take 2 to 4 us each.
+template <typename T>
+__device__ __forceinline__ void load4(float (&v)[4], const T* p, int left, bool aligned) {
+    if (aligned && left >= 4) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p);
+            v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xffff0000u);
+            v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? to_float<T>(p[e]) : 0.f;
+    }
+}
+
+// logits: a warp multiplies one class with eight rows, lanes along the features; blockIdx.z: part of the features
+constexpr int XE_SMALL_ROWS = 8, XE_SMALL_SLICE = 2048;
+template <typename T>
+__global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int n, int d, int v,
+                                                              int zpitch, float* __restrict__ z, int* zero) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x % 32, j = blockIdx.x * 8 + threadIdx.x / 32, r0 = blockIdx.y * XE_SMALL_ROWS;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
+    if (j >= v) return;
+    const int k0 = blockIdx.z * XE_SMALL_SLICE, k1 = k0 + XE_SMALL_SLICE < d ? k0 + XE_SMALL_SLICE : d;
+    const bool aligned = ldx % 4 == 0 && ldw % 4 == 0;         // the bases are
+    const T* row[XE_SMALL_ROWS];                               // rows past the last read it again
+#pragma unroll
+    for (int r = 0; r < XE_SMALL_ROWS; ++r) row[r] = x + (long long)(r0 + r < n ? r0 + r : n - 1) * ldx;
+    float acc[XE_SMALL_ROWS];
+#pragma unroll
+    for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] = 0.f;
+    if (aligned && (k1 - k0) % 4 == 0) {
+        // whole vectors: nine loads in flight per step, two steps
+#pragma unroll 2
+        for (int k = k0 + lane * 4; k < k1; k += 128) {
+            float a[4], b[XE_SMALL_ROWS][4];
+            load4(a, w + j * ldw + k, 4, true);
+#pragma unroll
+            for (int r = 0; r < XE_SMALL_ROWS; ++r) load4(b[r], row[r] + k, 4, true);
+#pragma unroll
+            for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] += (a[0] * b[r][0] + a[1] * b[r][1]) + (a[2] * b[r][2] + a[3] * b[r][3]);
+        }
+    } else {
+#pragma unroll 4
+        for (int k = k0 + lane; k < k1; k += 32) {
+            const float a = to_float<T>(w[j * ldw + k]);
+#pragma unroll
+            for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] += a * to_float<T>(row[r][k]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < XE_SMALL_ROWS; ++r) {
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], s);
+        if (lane == r && r0 + r < n) z[((long long)blockIdx.z * n + r0 + r) * zpitch + j] = acc[r];
+    }
+}
+
+// out[o][k] = scale sum_c coef(o, c) M[c][k]: dx (o rows, c classes, M = W) and dW (o classes, c rows, M = x; and dbias),
+// from dz in floats.  A block makes eight o by 128 k; its eight warps share the sum over c, whose coefficients sit in
+// shared memory.  A row that does not count has nothing but zeros there and is not read.
+constexpr int XE_SMALL_MAX = 1024;                 // most rows, most classes
+constexpr int XE_SMALL_GRAD_SMEM = XE_SMALL_MAX * 8 * 4;
+template <typename T>
+struct SmallGrad {
+    const T* x; const T* w;
+    T* dx; T* dw;
+    float* db;
+    long long ldx, ldw, lddx, lddw;
+    const float* dz;
+    int n, d, v, dzpitch, kblocks, dx_blocks;
+    XeScale scale;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    extern __shared__ __align__(16) float coef[];            // [c][8], then [warp][8][128] sums
+    const bool is_dw = (int)blockIdx.x >= a.dx_blocks;
+    const int b = is_dw ? blockIdx.x - a.dx_blocks : blockIdx.x;
+    const int o0 = b / a.kblocks * 8, k = (b % a.kblocks) * 128 + (threadIdx.x % 32) * 4, warp = threadIdx.x / 32;
+    const int outs = is_dw ? a.v : a.n, len = is_dw ? a.n : a.v;
+    for (int i = threadIdx.x; i < len * 8; i += 256) {
+        const int c = is_dw ? i / 8 : i % len, o = is_dw ? i % 8 : i / len;
+        const bool in = o0 + o < outs;
+        coef[c * 8 + o] = in ? a.dz[(long long)(is_dw ? c : o0 + o) * a.dzpitch + (is_dw ? o0 + o : c)] : 0.f;
+    }
+    __syncthreads();
+    const float scale = xe_scale(a.scale);
+    if (is_dw && a.db && k < 128 && threadIdx.x < 8 && o0 + threadIdx.x < outs) {
+        float s = 0.f;
+        for (int c = 0; c < len; ++c) s += coef[c * 8 + threadIdx.x];
+        a.db[o0 + threadIdx.x] = s * scale;
+    }
+    T* out = is_dw ? a.dw : a.dx;
+    if (!out) return;
+    const T* m = is_dw ? a.x : a.w;
+    const long long ldm = is_dw ? a.ldx : a.ldw, ldo = is_dw ? a.lddw : a.lddx;
+    const bool aligned = ldm % 4 == 0;
+    float acc[8][4];
+#pragma unroll
+    for (int o = 0; o < 8; ++o)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[o][e] = 0.f;
+    if (k < a.d) {
+#pragma unroll 4
+        for (int c = warp; c < len; c += 8) {
+            const float4 p = *reinterpret_cast<const float4*>(coef + c * 8), q = *reinterpret_cast<const float4*>(coef + c * 8 + 4);
+            const float f[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+            if (p.x == 0.f && p.y == 0.f && p.z == 0.f && p.w == 0.f && q.x == 0.f && q.y == 0.f && q.z == 0.f && q.w == 0.f) continue;
+            float v[4];
+            load4(v, m + c * ldm + k, a.d - k, aligned);
+#pragma unroll
+            for (int o = 0; o < 8; ++o)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[o][e] += f[o] * v[e];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < 8; ++o) *reinterpret_cast<float4*>(coef + (warp * 8 + o) * 128 + (threadIdx.x % 32) * 4) = make_float4(acc[o][0], acc[o][1], acc[o][2], acc[o][3]);
+    __syncthreads();
+    // warp -> output row, lane -> columns
+    if (o0 + warp < outs) {
+        const int kb = (b % a.kblocks) * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int kk = i * 32 + threadIdx.x % 32;
+            float s = 0.f;
+#pragma unroll
+            for (int g = 0; g < 8; ++g) s += coef[(g * 8 + warp) * 128 + kk];
+            if (kb + kk < a.d) out[(long long)(o0 + warp) * ldo + kb + kk] = from_float<T>(s * scale);
+        }
+    }
+}
+
 unsigned loop_blocks(long long items) {
     const long long b = (items + 255) / 256, most = 16ll * sm_count();
     return (unsigned)(b < 1 ? 1 : b < most ? b : most);
 }
 
 // ---- plan ----------------------------------------------------------------------------------------------------
+constexpr long long XE_SMALL_PRODUCTS = 4ll << 20;   // n v d up to which xe_small_* run
+
 struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
+    bool small;                          // FP32 arithmetic instead of tensor cores
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw;
-    int zpitch, piece, pieces, dzpitch;
+    int zpitch, piece, pieces, dzpitch, parts;
     bool dx_direct, dw_direct;           // the product's epilogue stores the caller's matrix
     int dpitch;                          // of float dx / dw buffers in the scratch
-    size_t off_x, off_w, off_z, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_scale, off_dz, off_db, off_dx, off_dw, total;
+    size_t off_x, off_w, off_z, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_count, off_dz, off_db, off_dx, off_dw, total;
 };
 
-// parts of the contraction so that tiles * parts fills the CTA pairs, each with at least four ring slots of work
-int split_count(long long tiles, long long chunks, int partial_products) {
-    const long long pairs = sm_count() / 2;
-    if (tiles >= pairs || tiles == 0) return 1;
-    long long s = pairs / tiles;
-    if (s > chunks * partial_products / 4) s = chunks * partial_products / 4;
-    if (s > chunks) s = chunks;
-    return (int)(s < 1 ? 1 : s);
+// Parts of a contraction of `chunks` ring slots (times `products` plane pairs), so that tiles * parts fills the CTA pairs in
+// as few whole turns as possible.  Estimated time: turns of the slots (0.28 us each on a pair) and of the epilogue (1.5 us),
+// and, for more than one part, writing and reading the floats of every part (5 TB/s) and, where `join` is set, a launch.
+int split_count(long long rows, long long cols, long long chunks, int products, bool join) {
+    const long long pairs = sm_count() / 2, tiles = ((rows + XE_BM - 1) / XE_BM) * ((cols + XE_BN - 1) / XE_BN);
+    if (tiles >= 4 * pairs || tiles == 0 || chunks == 1) return 1;
+    const double part_us = (double)rows * (double)cols * 8.0 / 5e6;
+    int best = 1;
+    double best_us = 1e30;
+    for (long long s = 1; s <= chunks && s <= 64 && (s == 1 || tiles * s <= 4 * pairs); ++s) {
+        const double us = (double)((tiles * s + pairs - 1) / pairs) * ((double)((chunks + s - 1) / s) * products * 0.28 + 1.5) +
+                          (s > 1 || !join ? part_us * (double)s : 0.0) + (s > 1 && join ? 3.0 : 0.0);
+        if (us < best_us) { best_us = us; best = (int)s; }
+    }
+    return best;
 }
 
-long long tiles_of(long long rows, long long cols) { return ((rows + XE_BM - 1) / XE_BM) * ((cols + XE_BN - 1) / XE_BN); }
+// rows of dz a block of xe_rows_kernel sums up: as many blocks as fit the GPU twice at 1024 threads an SM
+int row_blocks(long long n, int threads) {
+    const long long most = 2048ll / threads * sm_count();
+    return (int)(n < most ? n : most);
+}
+constexpr int XE_ROWS_MAX_V = 512 * 4 * 4;          // widest row of xe_rows_kernel: wider ones spill, and one block an SM is
+                                                    // slower than two kernels (1024 x 21841: 130 us against 92)
+int row_threads(int v) { return v <= 512 ? 128 : v <= 4096 ? 256 : 512; }
 
-int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
+int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     if (!d) return fail(WINO_E_BADARG, "xent: NULL descriptor");
     if (d->n < 0 || d->d <= 0 || d->v <= 0) return fail(WINO_E_BADARG, "xent: n must be at least 0, d and v positive");
     if (d->d > (1 << 30) || d->v > (1 << 30) || d->n > (1 << 30)) return fail(WINO_E_UNSUPPORTED, "xent: extents above 2^30");
@@ -366,14 +761,22 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.pack_x = !bf16 || p.ldx % 8 != 0 || (grad && d->has_ignore);
     p.pack_w = !bf16 || p.ldw % 8 != 0;
     const long long kd = (d->d + XE_BK - 1) / XE_BK;
-    p.splits_z = split_count(tiles_of(n, v), kd, products);
+    p.splits_z = split_count(n, v, kd, products, false);
     p.zpitch = round_up(d->v, 4);
-    const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll * p.splits_z;
-    // Kept floats cost 14 bytes a logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured
-    // 6.5 TB/s and 1.4 PFLOP/s the product is the dearer one from d = 1000 (200) on.
-    if (p.splits_z > 1) p.kept = true;
+    const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll;
+    const bool fits = z_bytes * p.splits_z + (grad ? dz_bytes : 0) <= limit;
+    // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
+    // logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured 6.5 TB/s and 1.4 PFLOP/s the
+    // product is the dearer one from d = 1000 (200) on.
+    const bool few = n * v <= 64ll * XE_BM * XE_BN;
+    p.small = n > 0 && d->v <= XE_SMALL_MAX && (!grad || n <= XE_SMALL_MAX) && n * v <= XE_SMALL_PRODUCTS / d->d;
+    if (p.small) {
+        p.kept = true;
+        p.pack_x = p.pack_w = false;
+        p.splits_z = (d->d + XE_SMALL_SLICE - 1) / XE_SMALL_SLICE;
+    } else if (few && fits) p.kept = true;
     else if (grad && bf16 && !d->has_bias && dz_bytes <= limit) p.exps = true;
-    else p.kept = grad && z_bytes + dz_bytes <= limit && d->d >= (bf16 ? 1024 : 256);
+    else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
     if (!p.kept) p.splits_z = 1;
     p.piece = d->v;
     p.pieces = 1;
@@ -388,10 +791,12 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     }
     p.dzpitch = round_up(p.piece, 8);
     p.dpitch = round_up(d->d, 4);
-    p.splits_dx = split_count(tiles_of(n, d->d), (p.piece + XE_BK - 1) / XE_BK, products);
-    p.splits_dw = split_count(tiles_of(p.piece, d->d), (n + XE_BK - 1) / XE_BK, products);
-    p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16) && (p.lddx * p.es) % 16 == 0;
-    p.dw_direct = p.splits_dw == 1 && (p.lddw * p.es) % 16 == 0;
+    p.splits_dx = split_count(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true);
+    p.splits_dw = split_count(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
+    // more than one piece adds up in floats: in dx itself, or in the scratch
+    p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
+    p.dw_direct = p.splits_dw == 1;
+    p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, row_threads(d->v)) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;
@@ -403,7 +808,7 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.off_rowloss = take(un * 4);
     p.off_rowg = take(un * 4);
     p.off_zt = take(un * 4);
-    p.off_scale = take(4);
+    p.off_count = take(8);               // rows that count, blocks that are done
     const size_t vtiles = (size_t)((v + XE_STAT_COLS - 1) / XE_STAT_COLS);
     p.off_zsum = take(p.kept || d->label_smoothing <= 0.f ? 0 : vtiles * un * 4);
     p.off_z = take(p.kept ? un * p.zpitch * 4 * p.splits_z : vtiles * un * 8);
@@ -411,7 +816,7 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.off_w = take(p.pack_w ? (size_t)v * p.dp * 2 * p.planes : 0);
     if (grad) {
         p.off_dz = take(un * p.dzpitch * 2 * p.planes);
-        p.off_db = take(d->has_bias ? (size_t)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART) * p.dzpitch * 4 : 0);
+        p.off_db = take(d->has_bias ? (size_t)p.parts * p.dzpitch * 4 : 0);
         p.off_dx = take(p.dx_direct ? 0 : un * p.dpitch * 4 * p.splits_dx);
         p.off_dw = take(p.dw_direct ? 0 : (size_t)p.piece * p.dpitch * 4 * p.splits_dw);
     }
@@ -420,42 +825,65 @@ int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     return WINO_OK;
 }
 
-int pack(const wino_xent_desc& d, const Plan& p, const void* src, long long ld, long long rows, void* dst, const long long* target, const RowRule& rule,
-         cudaStream_t st) {
-    const unsigned blocks = loop_blocks(rows * (p.dp / 4));
+// Every kernel of a call is launched with programmatic serialisation and waits for its predecessor itself: its blocks are
+// set up while that one ends (five launches of the 256 x 25088 x 1000 gradient: PDL_MEASURE).
+template <typename... KArgs, typename... Args>
+int xe_launch(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, cudaStream_t st, Args... args) {
     count_launch();
-    if (d.dtype == WINO_BF16)
-        xe_pack_kernel<__nv_bfloat16, 1><<<blocks, 256, 0, st>>>((const __nv_bfloat16*)src, ld, (__nv_bfloat16*)dst, rows, d.d, p.dp, target, rule);
-    else
-        xe_pack_kernel<float, 3><<<blocks, 256, 0, st>>>((const float*)src, ld, (__nv_bfloat16*)dst, rows, d.d, p.dp, target, rule);
-    WINO_CUDA_CHECK(cudaGetLastError());
+    WINO_CUDA_CHECK(launch_kernel(kernel, grid, dim3((unsigned)block), smem, st, true, args...));
     return WINO_OK;
 }
 
-// one gradient product: into the caller's matrix where its epilogue can store it, else through float buffers
-int grad_product(const Plan& p, const wino_xent_desc& d, const XeOperand& a, const XeOperand& b, long long rows, long long k, bool direct, int splits,
-                 bool first, bool last, void* out, long long ld, float* buf, const float* scale, cudaStream_t st) {
-    XeOutput o;
-    int rc;
-    o.add = !first;
-    o.scale = scale;
-    if (direct) {
-        o.ptr = out;
-        o.pitch = ld;
-        return xe_gemm(d.dtype == WINO_BF16 ? XE_BF16 : XE_F32, a, b, rows, d.d, k, o, st);
-    }
-    o.ptr = buf;
-    o.pitch = p.dpitch;
-    const long long chunks = (k + XE_BK - 1) / XE_BK;          // a short last piece adds to fewer of the parts
-    o.splits = chunks < splits ? (int)chunks : splits;
-    if ((rc = xe_gemm(XE_F32, a, b, rows, d.d, k, o, st))) return rc;
-    if (!last) return WINO_OK;
+// A plan follows from the descriptor and the number of SMs alone; the last one of a thread is kept, since programs come
+// back with the same descriptor step after step.
+int make_plan(const wino_xent_desc* d, bool grad, Plan* out) {
+    struct Last { wino_xent_desc d; bool grad; int sms; Plan plan; };
+    static thread_local Last last = {};
+    const int sms = sm_count();
+    if (d && last.sms == sms && last.grad == grad && memcmp(&last.d, d, sizeof(*d)) == 0) { *out = last.plan; return WINO_OK; }
+    const int rc = build_plan(d, grad, out);
+    if (rc == WINO_OK) { memcpy(&last.d, d, sizeof(*d)); last.grad = grad; last.sms = sms; last.plan = *out; }
+    return rc;
+}
+
+// planes: 0, 1, 3 as in xe_rows_kernel, -1 for statistics and loss alone
+template <int THREADS, int QUADS>
+int launch_rows(int planes, unsigned blocks, cudaStream_t st, const float* z, int splits, int v, int zpitch, const float* bias, const RowArgs& ra,
+                 const XeDzRule& rule, void* dz, int dpitch, float* db_part) {
+    auto go = [&](auto kernel) { return xe_launch(kernel, blocks, THREADS, 0, st, z, splits, v, zpitch, bias, ra, rule, dz, dpitch, db_part); };
+    const bool split = splits > 1;
+    if (planes < 0) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, false, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, false, false>);
+    if (planes == 1) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, true, false>);
+    if (planes == 3) return split ? go(xe_rows_kernel<THREADS, QUADS, 3, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 3, true, false>);
+    if constexpr (THREADS * QUADS * 4 <= XE_SMALL_MAX)
+        return split ? go(xe_rows_kernel<THREADS, QUADS, 0, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 0, true, false>);
+    return fail(WINO_E_BADARG, "xent: no row kernel");
+}
+
+template <typename T>
+int launch_small_logits(const void* x, long long ldx, const void* w, long long ldw, const wino_xent_desc& d, const Plan& p, float* z, int* zero, cudaStream_t st) {
+    const dim3 grid((unsigned)(d.v + 7) / 8, (unsigned)(d.n + XE_SMALL_ROWS - 1) / XE_SMALL_ROWS, (unsigned)p.splits_z);
+    return xe_launch(xe_small_logits_kernel<T>, grid, 256, 0, st, (const T*)x, ldx, (const T*)w, ldw, d.n, d.d, d.v, p.zpitch, z, zero);
+}
+
+template <typename T>
+int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* db, const wino_xent_desc& d, const Plan& p, const float* dz, const XeScale& scale,
+                      cudaStream_t st) {
+    SmallGrad<T> a;
+    a.x = (const T*)x; a.w = (const T*)w; a.dx = (T*)dx; a.dw = (T*)dw; a.db = db;
+    a.ldx = p.ldx; a.ldw = p.ldw; a.lddx = p.lddx; a.lddw = p.lddw;
+    a.dz = dz; a.n = d.n; a.d = d.d; a.v = d.v; a.dzpitch = p.zpitch;
+    a.kblocks = (d.d + 127) / 128;
+    a.dx_blocks = dx ? (d.n + 7) / 8 * a.kblocks : 0;
+    a.scale = scale;
+    const int dw_blocks = dw || db ? (d.v + 7) / 8 * a.kblocks : 0;
+    return xe_launch(xe_small_grad_kernel<T>, (unsigned)(a.dx_blocks + dw_blocks), 256, XE_SMALL_GRAD_SMEM, st, a);
+}
+
+int finish(const wino_xent_desc& d, const Plan& p, const float* buf, int splits, long long rows, void* out, long long ld, cudaStream_t st) {
     const unsigned blocks = loop_blocks(rows * ((d.d + 3) / 4));
-    count_launch();
-    if (d.dtype == WINO_BF16) xe_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(buf, splits, rows, d.d, p.dpitch, (__nv_bfloat16*)out, ld);
-    else xe_finish_kernel<float><<<blocks, 256, 0, st>>>(buf, splits, rows, d.d, p.dpitch, (float*)out, ld);
-    WINO_CUDA_CHECK(cudaGetLastError());
-    return WINO_OK;
+    if (d.dtype == WINO_BF16) return xe_launch(xe_finish_kernel<__nv_bfloat16>, blocks, 256, 0, st, buf, splits, rows, d.d, p.dpitch, (__nv_bfloat16*)out, ld);
+    return xe_launch(xe_finish_kernel<float>, blocks, 256, 0, st, buf, splits, rows, d.d, p.dpitch, (float*)out, ld);
 }
 
 int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, const float* bias, const long long* target, const float* dloss, float* loss,
@@ -484,102 +912,153 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     auto f = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
 
     const RowRule rule = {d.v, d.has_ignore, d.ignore_index};
-    XeOperand ox = {x, n, d.d, p.ldx, n * p.ldx, 1, false}, ow = {w, v, d.d, p.ldw, v * p.ldw, 1, false};
-    if (p.pack_x) {
-        if ((rc = pack(d, p, x, p.ldx, n, ws + p.off_x, grad && d.has_ignore ? target : nullptr, rule, st))) return rc;
-        ox = {ws + p.off_x, n, d.d, p.dp, n * p.dp, p.planes, false};
-    }
-    if (p.pack_w) {
-        if ((rc = pack(d, p, w, p.ldw, v, ws + p.off_w, nullptr, rule, st))) return rc;
-        ow = {ws + p.off_w, v, d.d, p.dp, v * p.dp, p.planes, false};
+    XeOperand ox = {x, n, d.d, p.ldx, n * p.ldx, p.planes, false}, ow = {w, v, d.d, p.ldw, v * p.ldw, p.planes, false};
+    if (p.pack_x || p.pack_w) {
+        PackJob jobs[2] = {};
+        int k = 0;
+        if (p.pack_x) {
+            jobs[k++] = {x, p.ldx, n, reinterpret_cast<__nv_bfloat16*>(ws + p.off_x), grad && d.has_ignore ? target : nullptr};
+            ox = {ws + p.off_x, n, d.d, p.dp, n * p.dp, p.planes, false};
+        }
+        if (p.pack_w) {
+            jobs[k++] = {w, p.ldw, v, reinterpret_cast<__nv_bfloat16*>(ws + p.off_w), nullptr};
+            ow = {ws + p.off_w, v, d.d, p.dp, v * p.dp, p.planes, false};
+        }
+        const unsigned blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * (p.dp / 4));
+        if (d.dtype == WINO_BF16) rc = xe_launch(xe_pack_kernel<__nv_bfloat16, 1>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
+        else rc = xe_launch(xe_pack_kernel<float, 3>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
+        if (rc) return rc;
     }
 
-    RowArgs ra;
-    ra.rule = rule; ra.n = n; ra.target = target;
-    ra.smooth = d.label_smoothing; ra.inv_v = (float)(1.0 / (double)v);
-    ra.lse = f(p.off_lse); ra.lse_out = lse; ra.rowloss = f(p.off_rowloss);
-    if ((rc = status_word(&ra.status))) return rc;
-    const float* b = d.has_bias ? bias : nullptr;
-    XeOutput oz;
-    if (p.kept) {
-        oz.ptr = ws + p.off_z;
-        oz.pitch = p.zpitch;
-        oz.splits = p.splits_z;
-        if ((rc = xe_gemm(XE_F32, ox, ow, n, v, d.d, oz, st))) return rc;
-        count_launch();
-        xe_rows_from_logits_kernel<<<(unsigned)n, 128, 0, st>>>(f(p.off_z), p.splits_z, d.v, p.zpitch, b, ra);
-    } else {
-        oz.bias = b;
-        oz.target = target;
-        oz.stats = reinterpret_cast<float2*>(ws + p.off_z);
-        oz.zsum = d.label_smoothing > 0.f ? f(p.off_zsum) : nullptr;
-        oz.zt = f(p.off_zt);
-        if (p.exps) {
-            oz.ptr = ws + p.off_dz;
-            oz.pitch = p.dzpitch;
-        }
-        if ((rc = xe_gemm(p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, oz, st))) return rc;
-        count_launch();
-        xe_rows_from_stats_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(oz.stats, oz.zsum, oz.zt, (int)((v + XE_STAT_COLS - 1) / XE_STAT_COLS), ra);
-    }
-    WINO_CUDA_CHECK(cudaGetLastError());
-    XeDzRule dzr;
     const float s = d.label_smoothing, dz_factor = s <= 0.5f ? 1.f - s : 1.f;
+    XeDzRule dzr;
     dzr.pf = 1.f / dz_factor;
     dzr.smooth_t = s <= 0.5f ? 1.f : 1.f - s;
     dzr.smooth_all = (float)((double)s / (double)v / (double)dz_factor);
-    count_launch();
-    xe_loss_kernel<<<1, 1024, 0, st>>>(ra, d.reduction, dloss, dz_factor, loss, grad ? f(p.off_rowg) : nullptr, f(p.off_scale));
-    WINO_CUDA_CHECK(cudaGetLastError());
-    if (!grad || (!dx && !dw && !db)) return WINO_OK;
-
-    const int parts = (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
+    RowArgs ra;
+    ra.rule = rule; ra.n = n; ra.target = target;
+    ra.dloss = d.reduction == WINO_NONE ? dloss : nullptr;
+    ra.smooth = s; ra.inv_v = (float)(1.0 / (double)v);
+    ra.lse = f(p.off_lse); ra.lse_out = lse; ra.rowg = f(p.off_rowg);
+    ra.rowloss = d.reduction == WINO_NONE ? loss : f(p.off_rowloss);
+    ra.loss = d.reduction == WINO_NONE ? nullptr : loss;
+    ra.mean = d.reduction == WINO_MEAN;
+    ra.count = reinterpret_cast<int*>(ws + p.off_count);
+    if ((rc = status_word(&ra.status))) return rc;
+    const float* b = d.has_bias ? bias : nullptr;
+    const bool wide = d.v > XE_ROWS_MAX_V;
     __nv_bfloat16* dz = reinterpret_cast<__nv_bfloat16*>(ws + p.off_dz);
     float* db_part = db ? f(p.off_db) : nullptr;
+    XeScale scale;
+    scale.count = ra.count;
+    scale.dloss = d.reduction == WINO_NONE ? nullptr : dloss;
+    scale.factor = dz_factor;
+    scale.mean = ra.mean;
+
+    const bool products = grad && (dx || dw || db);
+    XeProduct pz = {p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
+    pz.out.zero = ra.count;
+    if (p.kept) {
+        float* z = f(p.off_z);
+        pz.out.ptr = z;
+        pz.out.pitch = p.zpitch;
+        pz.out.splits = p.splits_z;
+        if (!p.small) rc = xe_gemm(&pz, 1, st);
+        else if (p.es == 2) rc = launch_small_logits<__nv_bfloat16>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
+        else rc = launch_small_logits<float>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
+        if (rc) return rc;
+        if (wide) {
+            rc = xe_launch(p.splits_z > 1 ? xe_wide_rows_kernel<true> : xe_wide_rows_kernel<false>, (unsigned)n, 256, 0, st, z, p.splits_z, d.v, p.zpitch, b, ra);
+        } else {
+            const unsigned blocks = (unsigned)row_blocks(n, row_threads(d.v));
+            auto rows_fn = d.v <= 512 ? launch_rows<128, 1> : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
+                         : d.v <= 4096 ? launch_rows<256, 4> : launch_rows<512, 4>;
+            if (p.small && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, nullptr);
+            else rc = rows_fn(products ? p.planes : -1, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, dz, p.dzpitch, db_part);
+        }
+    } else {
+        pz.out.bias = b;
+        pz.out.target = target;
+        pz.out.stats = reinterpret_cast<float2*>(ws + p.off_z);
+        pz.out.zsum = d.label_smoothing > 0.f ? f(p.off_zsum) : nullptr;
+        pz.out.zt = f(p.off_zt);
+        if (p.exps) {
+            pz.out.ptr = dz;
+            pz.out.pitch = p.dzpitch;
+        }
+        if ((rc = xe_gemm(&pz, 1, st))) return rc;
+        rc = xe_launch(xe_rows_from_stats_kernel, (unsigned)((n + 31) / 32), 256, 0, st, pz.out.stats, pz.out.zsum, pz.out.zt, (int)((v + XE_STAT_COLS - 1) / XE_STAT_COLS), ra);
+    }
+    if (rc) return rc;
+
+    if (!products) return WINO_OK;
+    if (p.small)
+        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, st)
+                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, st);
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, vc = d.v - v0 < p.piece ? d.v - v0 : p.piece;
         XeOperand wp = ow;                 // the piece's rows of W
         wp.ptr = static_cast<const char*>(ow.ptr) + (size_t)v0 * ow.pitch * 2;
         wp.rows = vc;
-        if (p.kept) {
-            const unsigned grid = (unsigned)((vc + 255) / 256) * (unsigned)parts;
-            count_launch();
-            if (p.planes == 1)
-                xe_dz_from_logits_kernel<1><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, dzr, dz, p.dzpitch, db_part);
-            else
-                xe_dz_from_logits_kernel<3><<<grid, 128, 0, st>>>(f(p.off_z), vc, p.zpitch, n, ra.lse, f(p.off_rowg), target, dzr, dz, p.dzpitch, db_part);
-            WINO_CUDA_CHECK(cudaGetLastError());
+        if (p.kept && wide) {
+            const unsigned grid = (unsigned)((vc + 255) / 256) * (unsigned)p.parts;
+            if (p.planes == 1) rc = xe_launch(xe_wide_dz_kernel<1>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, p.splits_z > 1 ? nullptr : b, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
+            else rc = xe_launch(xe_wide_dz_kernel<3>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, p.splits_z > 1 ? nullptr : b, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
         } else if (p.exps) {
-            count_launch();
-            xe_dz_from_exp_kernel<<<loop_blocks(n * (p.dzpitch / 8)), 256, 0, st>>>(dz, p.dzpitch, n, oz.stats, oz.zt, ra.lse, f(p.off_rowg), target, dzr);
-            WINO_CUDA_CHECK(cudaGetLastError());
-        } else {
-            XeOutput o;
-            o.ptr = dz; o.pitch = p.dzpitch;
-            o.bias = b ? b + v0 : nullptr;
-            o.target = target; o.col_base = v0;
-            o.lse = ra.lse; o.rowg = f(p.off_rowg); o.rule = dzr;
-            o.db_part = db_part; o.db_pitch = p.dzpitch;
-            if ((rc = xe_gemm(XE_DZ, ox, wp, n, vc, d.d, o, st))) return rc;
+            rc = xe_launch(xe_dz_from_exp_kernel, loop_blocks(n * ((p.dzpitch / 8 + 1023) / 1024) * 256), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt, ra.lse, ra.rowg, target, dzr);
+        } else if (!p.kept) {
+            XeProduct pd = {XE_DZ, ox, wp, n, vc, d.d, XeOutput()};
+            pd.out.ptr = dz; pd.out.pitch = p.dzpitch;
+            pd.out.bias = b ? b + v0 : nullptr;
+            pd.out.target = target; pd.out.col_base = v0;
+            pd.out.lse = ra.lse; pd.out.rowg = ra.rowg; pd.out.rule = dzr;
+            pd.out.db_part = db_part; pd.out.db_pitch = p.dzpitch;
+            if ((rc = xe_gemm(&pd, 1, st))) return rc;
         }
+        if (rc) return rc;
         if (db) {
-            count_launch();
-            xe_db_kernel<<<(unsigned)((vc + 31) / 32), 256, 0, st>>>(db_part, parts, p.dzpitch, vc, f(p.off_scale), db + v0);
-            WINO_CUDA_CHECK(cudaGetLastError());
+            rc = xe_launch(xe_db_kernel, (unsigned)(vc + 31) / 32, 512, 0, st, db_part, p.parts, p.dzpitch, vc, scale, db + v0);
+            if (rc) return rc;
         }
-        XeOperand odz = {dz, n, vc, p.dzpitch, n * p.dzpitch, p.planes, false};
+
+        const XeOperand odz = {dz, n, vc, p.dzpitch, n * p.dzpitch, p.planes, false};
+        const bool bf16 = p.planes == 1, first = i == 0, last = i == p.pieces - 1;
+        XeProduct prod[2];
+        int count = 0;
+        auto product = [&](const XeOperand& a, const XeOperand& b, long long rows, long long k, bool direct, int splits, bool add, void* out, long long ld, float* buf) {
+            XeProduct& q = prod[count++];
+            q = {direct && bf16 ? XE_BF16 : XE_F32, a, b, rows, d.d, k, XeOutput()};
+            q.out.scale = scale;
+            q.out.add = add;
+            q.out.ptr = direct ? out : buf;
+            q.out.pitch = direct ? ld : p.dpitch;
+            const long long chunks = (k + XE_BK - 1) / XE_BK;          // a short last piece adds to fewer of the parts
+            q.out.splits = direct ? 1 : chunks < splits ? (int)chunks : splits;
+        };
+        void* dw_at = static_cast<char*>(dw) + (size_t)v0 * p.lddw * p.es;
         if (dx) {
             XeOperand wr = wp;
             wr.along_rows = true;
-            if ((rc = grad_product(p, d, odz, wr, n, vc, p.dx_direct, p.splits_dx, i == 0, i == p.pieces - 1, dx, p.lddx, f(p.off_dx), f(p.off_scale), st))) return rc;
+            product(odz, wr, n, vc, p.dx_direct, p.splits_dx, !first, dx, p.lddx, f(p.off_dx));
         }
         if (dw) {
             XeOperand zr = odz, xr = ox;
             zr.along_rows = xr.along_rows = true;
-            if ((rc = grad_product(p, d, zr, xr, vc, n, p.dw_direct, p.splits_dw, true, true, static_cast<char*>(dw) + (size_t)v0 * p.lddw * p.es, p.lddw,
-                                   f(p.off_dw), f(p.off_scale), st)))
-                return rc;
+            product(zr, xr, vc, n, p.dw_direct, p.splits_dw, false, dw_at, p.lddw, f(p.off_dw));
         }
+        // Both in one launch where their epilogues agree and one of them has few tiles: the other fills the SMs that it
+        // leaves idle (256 x 25088 x 1000: 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU
+        // runs at its power limit either way (8192 x 4096 x 50021: 8.2 ms apart, 8.4 ms together).
+        const long long cols = (d.d + XE_BN - 1) / XE_BN;
+        const long long tiles_x = (n + XE_BM - 1) / XE_BM * cols * p.splits_dx, tiles_w = ((long long)vc + XE_BM - 1) / XE_BM * cols * p.splits_dw;
+        if (count == 2 && prod[0].epi == prod[1].epi && (tiles_x < tiles_w ? tiles_x : tiles_w) < sm_count()) {
+            if ((rc = xe_gemm(prod, 2, st))) return rc;
+        } else {
+            for (int k = 0; k < count; ++k)
+                if ((rc = xe_gemm(&prod[k], 1, st))) return rc;
+        }
+        if (dx && last && !p.dx_direct && (rc = finish(d, p, f(p.off_dx), p.splits_dx, n, dx, p.lddx, st))) return rc;
+        if (dw && !p.dw_direct && (rc = finish(d, p, f(p.off_dw), p.splits_dw, vc, dw_at, p.lddw, st))) return rc;
     }
     return WINO_OK;
 }

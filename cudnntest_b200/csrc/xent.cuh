@@ -37,12 +37,25 @@ struct XeDzRule {
     float smooth_all = 0.f;   // s / v / f
 };
 
+// the factor all rows share: f of XeDzRule, the upstream gradient, 1 / (rows that count)
+struct XeScale {
+    const int* count = nullptr;       // NULL: 1
+    const float* dloss = nullptr;     // NULL: 1
+    float factor = 1.f;
+    int mean = 0;
+};
+__device__ __forceinline__ float xe_scale(const XeScale& s) {
+    if (!s.count) return 1.f;
+    const int n = *s.count;
+    return s.factor * (s.dloss ? *s.dloss : 1.f) * (s.mean ? 1.f / (float)(n > 0 ? n : 1) : 1.f);
+}
+
 struct XeOutput {
     void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16, XE_STATS_E: m rows; XE_DZ: [planes][m][pitch] BF16
     long long pitch = 0;
     int splits = 1;                 // parts of the contraction, one buffer each (XE_F32)
     bool add = false;               // XE_F32: add instead of store
-    const float* scale = nullptr;   // XE_F32, XE_BF16: device scalar the product is multiplied by, or NULL
+    XeScale scale;                  // XE_F32, XE_BF16: what the product is multiplied by
     // XE_STATS, XE_STATS_E, XE_DZ
     const float* bias = nullptr;    // of column 0 of this product
     const long long* target = nullptr;
@@ -55,11 +68,18 @@ struct XeOutput {
     XeDzRule rule;
     float* db_part = nullptr;       // [m / 32][db_pitch] column sums of 32 rows each, or NULL
     long long db_pitch = 0;
+    int* zero = nullptr;            // two device words set to 0, or NULL
 };
 
-// product of a (m x k) and b (n x k)^T, contraction length k
-int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m, long long n, long long k, const XeOutput& out,
-            cudaStream_t st);
+// one product of a (m x k) and b (n x k)^T, contraction length k
+struct XeProduct {
+    XeEpilogue epi;
+    XeOperand a, b;
+    long long m, n, k;
+    XeOutput out;
+};
+// one or two products in one launch; two must have the same epilogue, XE_F32 or XE_BF16
+int xe_gemm(const XeProduct* prod, int count, cudaStream_t st);
 
 __device__ __forceinline__ float xe_ex2(float x) {
     float y;

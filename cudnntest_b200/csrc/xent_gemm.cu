@@ -38,15 +38,19 @@ constexpr int XE_BAND = 8;
 
 enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
 
-struct XeParams {
-    long long m, n;
+struct alignas(64) XeProblem {
+    CUtensorMap tm_a, tm_b, tm_out;
+    long long m, n, tiles, units;     // units: tiles * splits
     int mpairs, nblocks, splits, kchunks, pairs;
     int block;                        // ring slots per block of the contraction (and plane pair)
     unsigned char pa[6], pb[6];       // planes of a and b, one entry per partial product
+    int a_mn, b_mn;                   // contracted along the rows of the stored matrix
     uint32_t idesc;
-    int* status;
     int add;
-    const float* scale;
+    int plain;                        // rows that TMA cannot store: out_ptr, out_pitch
+    void* out_ptr;
+    long long out_pitch;
+    XeScale scale;
     const float* bias;
     const long long* target;
     int col_base;
@@ -58,6 +62,12 @@ struct XeParams {
     XeDzRule rule;
     float* db_part;
     long long db_pitch;
+};
+struct XeParams {
+    XeProblem prob[2];
+    int lead;                         // units of the second product that a pair without a last unit of the first takes ahead
+    int* zero;
+    int* status;
 };
 
 template <int EPI, int PLANES>
@@ -111,10 +121,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&o);
 }
 
-template <int EPI, int PLANES, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1)
-xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-               const __grid_constant__ CUtensorMap tm_out, const XeParams p) {
+template <int EPI, int PLANES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_gemm_kernel(const __grid_constant__ XeParams pp) {
     using L = XeSmem<EPI, PLANES>;
     constexpr int STAGES = L::STAGES;
 
@@ -127,6 +135,7 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gen_base + L::SLOT_OFF);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_base + L::SLOT_OFF + 4);
 
+    pdl_launch_dependents();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_ctarank();          // 0 = leader (issues the MMAs, owns the "full" and "tempty" barriers)
 
@@ -147,21 +156,38 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     cluster_sync_all();            // barriers of both CTAs initialised before any remote arrive or TMA completion
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    pdl_wait();                    // everything before this ran under the predecessor
 
-    const long long tiles = (long long)p.mpairs * p.nblocks, total = tiles * p.splits;
     const long long pair = blockIdx.x / 2, npairs = gridDim.x / 2;
+    if (pp.zero && blockIdx.x == 0 && threadIdx.x < 2) pp.zero[threadIdx.x] = 0;
 
-    auto decode = [&](long long u, int& sp, int& mp, int& nb) {
-        sp = (int)(u / tiles);
-        const long long t = u % tiles, band = (long long)XE_BAND * p.nblocks;
+    // The i-th unit of this pair, -1 after the last.  Units of the first product go round the pairs; the pairs that its last
+    // turn leaves out take `lead` units of the second product each in that time, the rest of which goes round all pairs.
+    const long long units0 = pp.prob[0].units, units1 = pp.prob[1].units, over = units0 % npairs;
+    const long long mine0 = units0 / npairs + (pair < over ? 1 : 0), ahead = over && pair >= over ? pp.lead : 0;
+    const long long base1 = over ? (npairs - over) * pp.lead : 0;
+    auto unit_at = [&](long long i) -> long long {
+        if (i < mine0) return pair + i * npairs;
+        i -= mine0;
+        const long long u = i < ahead ? pair - over + i * (npairs - over) : base1 + pair + (i - ahead) * npairs;
+        return u < units1 ? units0 + u : -1;
+    };
+
+    // work unit -> problem, part of the contraction (ring slots c0 ... c1), tile
+    struct Unit { int sp, mp, nb, c0, c1; };
+    auto decode = [&](long long u, Unit& w) -> const XeProblem& {
+        const bool second = u >= pp.prob[0].units;
+        const XeProblem& p = pp.prob[second];
+        if (second) u -= pp.prob[0].units;
+        w.sp = (int)(u / p.tiles);
+        const long long t = u % p.tiles, band = (long long)XE_BAND * p.nblocks;
         const int first = (int)(t / band) * XE_BAND;
         const int height = p.mpairs - first < XE_BAND ? p.mpairs - first : XE_BAND;
-        mp = first + (int)((t % band) % height);
-        nb = (int)((t % band) / height);
-    };
-    auto chunk_range = [&](int sp, int& c0, int& c1) {
-        c0 = (int)((long long)sp * p.kchunks / p.splits);
-        c1 = (int)((long long)(sp + 1) * p.kchunks / p.splits);
+        w.mp = first + (int)((t % band) % height);
+        w.nb = (int)((t % band) / height);
+        w.c0 = (int)((long long)w.sp * p.kchunks / p.splits);
+        w.c1 = (int)((long long)(w.sp + 1) * p.kchunks / p.splits);
+        return p;
     };
 
     if (warp == 0) {
@@ -170,34 +196,37 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (long long u = pair; ok && u < total; u += npairs) {
-            int sp, mp, nb, c0, c1;
-            decode(u, sp, mp, nb);
-            chunk_range(sp, c0, c1);
-            const int arow = (mp * 2 + (int)rank) * 128;               // this CTA's 128 rows of a
-            const int brow = nb * XE_BN + (int)rank * 128;             // this CTA's half of the rows of b
-            for (int cb = c0; ok && cb < c1; cb += p.block)
-            for (int q = 0; ok && q < p.pairs; ++q) {
-                const int pa = p.pa[q], pb = p.pb[q], ce = cb + p.block < c1 ? cb + p.block : c1;
-                for (int kc = cb; kc < ce; ++kc) {
-                    if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XE_WAIT_EMPTY)) { ok = false; break; }
-                    if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 4 * XE_TILE_BYTES);
-                    if (issuer) {
-                        const uint32_t bar = full_leader + 8 * stage, as = a_ring + stage * XE_TILE_BYTES, bs = b_ring + stage * XE_TILE_BYTES;
-                        if (A_MN) {
-                            tma_load_3d_pair(as, &tm_a, bar, arow, kc * XE_BK, pa);
-                            tma_load_3d_pair(as + 8192, &tm_a, bar, arow + 64, kc * XE_BK, pa);
-                        } else {
-                            tma_load_3d_pair(as, &tm_a, bar, kc * XE_BK, arow, pa);
+        for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+            Unit w;
+            const XeProblem& p = decode(u, w);
+            const bool a_mn = p.a_mn, b_mn = p.b_mn;
+            const int arow = (w.mp * 2 + (int)rank) * 128;             // this CTA's 128 rows of a
+            const int brow = w.nb * XE_BN + (int)rank * 128;           // this CTA's half of the rows of b
+            for (int cb = w.c0; ok && cb < w.c1; cb += p.block) {
+                const int ce = cb + p.block < w.c1 ? cb + p.block : w.c1;
+                for (int q = 0; ok && q < p.pairs; ++q) {
+                    const int pa = p.pa[q], pb = p.pb[q];
+                    for (int kc = cb; kc < ce; ++kc) {
+                        if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, pp.status, XE_WAIT_EMPTY)) { ok = false; break; }
+                        if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 4 * XE_TILE_BYTES);
+                        if (issuer) {
+                            const uint32_t bar = full_leader + 8 * stage, as = a_ring + stage * XE_TILE_BYTES, bs = b_ring + stage * XE_TILE_BYTES;
+                            const int k0 = kc * XE_BK;
+                            if (a_mn) {
+                                tma_load_3d_pair(as, &p.tm_a, bar, arow, k0, pa);
+                                tma_load_3d_pair(as + 8192, &p.tm_a, bar, arow + 64, k0, pa);
+                            } else {
+                                tma_load_3d_pair(as, &p.tm_a, bar, k0, arow, pa);
+                            }
+                            if (b_mn) {
+                                tma_load_3d_pair(bs, &p.tm_b, bar, brow, k0, pb);
+                                tma_load_3d_pair(bs + 8192, &p.tm_b, bar, brow + 64, k0, pb);
+                            } else {
+                                tma_load_3d_pair(bs, &p.tm_b, bar, k0, brow, pb);
+                            }
                         }
-                        if (B_MN) {
-                            tma_load_3d_pair(bs, &tm_b, bar, brow, kc * XE_BK, pb);
-                            tma_load_3d_pair(bs + 8192, &tm_b, bar, brow + 64, kc * XE_BK, pb);
-                        } else {
-                            tma_load_3d_pair(bs, &tm_b, bar, kc * XE_BK, brow, pb);
-                        }
+                        if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     }
-                    if (++stage == STAGES) { stage = 0; phase ^= 1; }
                 }
             }
         }
@@ -208,26 +237,26 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
             int stage = 0, as = 0;
             uint32_t phase = 0, aphase = 0;
             bool ok = true;
-            for (long long u = pair; ok && u < total; u += npairs) {
-                int sp, mp, nb, c0, c1;
-                decode(u, sp, mp, nb);
-                chunk_range(sp, c0, c1);
-                for (int cb = c0; ok && cb < c1; cb += p.block) {
-                    const int steps = (cb + p.block < c1 ? p.block : c1 - cb) * p.pairs;
-                    if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
+            for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+                Unit w;
+                const XeProblem& p = decode(u, w);
+                // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
+                const bool a_mn = p.a_mn, b_mn = p.b_mn;
+                const uint64_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+                const uint64_t a0 = a_mn ? smem_desc_mn128(a_ring) : smem_desc_k128(a_ring), b0 = b_mn ? smem_desc_mn128(b_ring) : smem_desc_k128(b_ring);
+                const uint32_t idesc = p.idesc;
+                for (int cb = w.c0; ok && cb < w.c1; cb += p.block) {
+                    const int steps = (cb + p.block < w.c1 ? p.block : w.c1 - cb) * p.pairs;
+                    if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, pp.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + (uint32_t)(as * XE_BN);
                     for (int kc = 0; kc < steps; ++kc) {
-                        if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XE_WAIT_FULL)) { ok = false; break; }
+                        if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, pp.status, XE_WAIT_FULL)) { ok = false; break; }
                         tc_fence_after();
-                        // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
-                        const uint32_t at = a_ring + stage * XE_TILE_BYTES, bt = b_ring + stage * XE_TILE_BYTES;
-                        const uint64_t a_desc = A_MN ? smem_desc_mn128(at) : smem_desc_k128(at);
-                        const uint64_t b_desc = B_MN ? smem_desc_mn128(bt) : smem_desc_k128(bt);
-                        constexpr uint64_t a_step = A_MN ? 128 : 2, b_step = B_MN ? 128 : 2;
+                        const uint64_t a_desc = a0 + (uint64_t)(stage * (XE_TILE_BYTES >> 4)), b_desc = b0 + (uint64_t)(stage * (XE_TILE_BYTES >> 4));
 #pragma unroll
                         for (int ks = 0; ks < XE_BK / 16; ++ks)
-                            if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, p.idesc, (kc | ks) ? 1u : 0u);
+                            if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, idesc, (kc | ks) ? 1u : 0u);
                         if (issuer) tc_commit_pair(bar_empty + 8 * stage, 3);       // frees the slot in both CTAs
                         if (++stage == STAGES) { stage = 0; phase ^= 1; }
                     }
@@ -246,30 +275,31 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
         int as = 0;
         uint32_t aphase = 0, issued = 0;
         bool ok = true;
-        const float scale = (EPI == XE_F32 || EPI == XE_BF16) && p.scale ? *p.scale : 1.f;
         // the staging buffer that is free next (its earlier store has been read out of shared memory)
-        auto next_buffer = [&]() -> uint32_t {
+        auto next_buffer = [&](bool plain = false) -> uint32_t {
             const uint32_t buf = L::NBUF == 1 ? 0 : issued & 1;
-            if (issued >= (uint32_t)L::NBUF) {
+            if (plain) {                              // a use that no store follows: leave nothing outstanding behind it
+                if (lane == 0) tma_store_wait_read<0>();
+                __syncwarp();
+            } else if (issued >= (uint32_t)L::NBUF) {
                 if (lane == 0) tma_store_wait_read<L::NBUF - 1>();
                 __syncwarp();
             }
             ++issued;
             return buf;
         };
-        for (long long u = pair; ok && u < total; u += npairs) {
-            int sp, mp, nb, c0, c1;
-            decode(u, sp, mp, nb);
-            chunk_range(sp, c0, c1);
-            const long long row0 = (long long)(mp * 2 + (int)rank) * 128 + quarter * 32;
-            const long long row = row0 + lane, wcol = (long long)nb * XE_BN + half * XE_WCOLS;
+        for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+            Unit w;
+            const XeProblem& p = decode(u, w);
+            const long long row0 = (long long)(w.mp * 2 + (int)rank) * 128 + quarter * 32;
+            const long long row = row0 + lane, wcol = (long long)w.nb * XE_BN + half * XE_WCOLS;
 
             float z[XE_WCOLS];                        // this thread's row of the tile
-            for (int cb = c0; cb < c1; cb += p.block) {
-                if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
+            for (int cb = w.c0; cb < w.c1; cb += p.block) {
+                if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, pp.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * XE_BN + half * XE_WCOLS);
-                if (cb == c0) {
+                if (cb == w.c0) {
 #pragma unroll
                     for (int j = 0; j < XE_WCOLS / 32; ++j) tmem_ld_32x32(tsrc + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * j]));
                     tmem_ld_wait();
@@ -303,12 +333,13 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 __syncwarp();
                 if (lane == 0) {
                     for (int q = 0; q < planes; ++q)
-                        tma_store_3d(&tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)col0, (int)row0, q);
+                        tma_store_3d(&p.tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)col0, (int)row0, q);
                     tma_store_commit();
                 }
             };
 
             if constexpr (EPI == XE_F32 || EPI == XE_BF16) {
+                const float scale = xe_scale(p.scale);
 #pragma unroll
                 for (int i = 0; i < XE_WCOLS; ++i) z[i] *= scale;
             }
@@ -317,17 +348,31 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                 for (int chunk = 0; chunk < XE_WCOLS / 32; ++chunk) {
                     const long long col0 = wcol + chunk * 32;
                     if (col0 < p.n) {
-                        const uint32_t buf = next_buffer();
+                        const uint32_t buf = next_buffer(p.plain);
                         float4* dst = reinterpret_cast<float4*>(stage_gen + buf * L::BUF + lane * 128);
                         const float* v = &z[chunk * 32];
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             dst[j ^ (lane & 7)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        if (p.plain) {                // row by row, 128 contiguous bytes per store
+                            __syncwarp();
+                            float* o = static_cast<float*>(p.out_ptr) + row0 * p.out_pitch + col0 + lane;
+                            const int rows = p.m - row0 < 32 ? (int)(p.m - row0) : 32;
+                            if (col0 + lane < p.n) {
+                                const float* src = reinterpret_cast<const float*>(stage_gen + buf * L::BUF) + (lane & 3);
+                                for (int r = 0; r < rows; ++r) {
+                                    const float v = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
+                                    o[r * p.out_pitch] = p.add ? o[r * p.out_pitch] + v : v;
+                                }
+                            }
+                            __syncwarp();
+                            continue;
+                        }
                         fence_async_shared();
                         __syncwarp();
                         if (lane == 0) {
-                            if (p.add) tma_reduce_add_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, sp);
-                            else tma_store_3d(&tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, sp);
+                            if (p.add) tma_reduce_add_3d(&p.tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, w.sp);
+                            else tma_store_3d(&p.tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, w.sp);
                             tma_store_commit();
                         }
                     }
@@ -336,11 +381,24 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (wcol + h * 64 < p.n) {
-                        const uint32_t buf = next_buffer();
-                        uint32_t w[32];
+                        const uint32_t buf = next_buffer(p.plain);
+                        uint32_t pk[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                        stage64(w, buf, 0);
+                        for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                        stage64(pk, buf, 0);
+                        if (p.plain) {                // row by row, two columns of 32 per row
+                            __syncwarp();
+                            const int rows = p.m - row0 < 32 ? (int)(p.m - row0) : 32;
+                            const unsigned short* src = reinterpret_cast<const unsigned short*>(stage_gen + buf * L::BUF) + (lane & 7);
+                            unsigned short* o = static_cast<unsigned short*>(p.out_ptr) + row0 * p.out_pitch + wcol + h * 64 + lane;
+                            const bool in0 = wcol + h * 64 + lane < p.n, in1 = wcol + h * 64 + 32 + lane < p.n;
+                            for (int r = 0; r < rows; ++r) {
+                                if (in0) o[r * p.out_pitch] = src[r * 64 + ((lane >> 3) ^ (r & 7)) * 8];
+                                if (in1) o[r * p.out_pitch + 32] = src[r * 64 + (((lane >> 3) + 4) ^ (r & 7)) * 8];
+                            }
+                            __syncwarp();
+                            continue;
+                        }
                         store64(buf, wcol + h * 64, 1);
                     }
                 }
@@ -404,10 +462,10 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                         for (int h = 0; h < 2; ++h) {
                             if (wcol + h * 64 < p.n) {
                                 const uint32_t buf = next_buffer();
-                                uint32_t w[32];
+                                uint32_t pk[32];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                stage64(w, buf, 0);
+                                for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                stage64(pk, buf, 0);
                                 store64(buf, wcol + h * 64, 1);
                             }
                         }
@@ -428,11 +486,11 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     for (int h = 0; h < 2; ++h) {
                         if (wcol + h * 64 < p.n) {
                             const uint32_t buf = next_buffer();
-                            uint32_t w[32];
+                            uint32_t pk[32];
                             if constexpr (PLANES == 1) {
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                stage64(w, buf, 0);
+                                for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                stage64(pk, buf, 0);
                                 store64(buf, wcol + h * 64, 1);
                                 if (p.db_part) {
 #pragma unroll
@@ -458,11 +516,11 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                                 for (int q = 0; q < PLANES; ++q) {        // round, keep the remainder for the next plane
 #pragma unroll
                                     for (int i = 0; i < 32; ++i) {
-                                        w[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                        z[64 * h + 2 * i] -= __uint_as_float(w[i] << 16);
-                                        z[64 * h + 2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+                                        pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                        z[64 * h + 2 * i] -= __uint_as_float(pk[i] << 16);
+                                        z[64 * h + 2 * i + 1] -= __uint_as_float(pk[i] & 0xffff0000u);
                                     }
-                                    stage64(w, buf, q);
+                                    stage64(pk, buf, q);
                                 }
                                 store64(buf, wcol + h * 64, PLANES);
                             }
@@ -484,8 +542,8 @@ xe_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
     }
 }
 
-template <int EPI, int PLANES, bool A_MN, bool B_MN>
-int run(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap& tm_out, const XeParams& p, cudaStream_t st) {
+template <int EPI, int PLANES>
+int run(const XeParams& p, cudaStream_t st) {
     using L = XeSmem<EPI, PLANES>;
     static_assert(L::TOTAL <= 232448, "shared memory budget of one CTA exceeded");
     static std::once_flag once[64];
@@ -493,15 +551,13 @@ int run(const CUtensorMap& tm_a, const CUtensorMap& tm_b, const CUtensorMap& tm_
     WINO_CUDA_CHECK(cudaGetDevice(&dev));
     cudaError_t attr_err = cudaSuccess;
     std::call_once(once[dev & 63], [&] {
-        attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES, A_MN, B_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+        attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     });
     WINO_CUDA_CHECK(attr_err);
-    const long long total = (long long)p.mpairs * p.nblocks * p.splits;
-    long long pairs = sm_count() / 2;
-    if (total < pairs) pairs = total;
+    const long long total = p.prob[0].units + p.prob[1].units;
+    const long long pairs = total < sm_count() / 2 ? total : sm_count() / 2;
     count_launch();
-    xe_gemm_kernel<EPI, PLANES, A_MN, B_MN><<<(unsigned)(2 * pairs), XE_THREADS, L::TOTAL, st>>>(tm_a, tm_b, tm_out, p);
-    WINO_CUDA_CHECK(cudaGetLastError());
+    WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES>, dim3((unsigned)(2 * pairs)), dim3(XE_THREADS), L::TOTAL, st, true, p));
     return WINO_OK;
 }
 
@@ -514,59 +570,83 @@ int operand_map(CUtensorMap* map, const XeOperand& o) {
     return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1);
 }
 
-}  // namespace
-
-int xe_gemm(XeEpilogue epi, const XeOperand& a, const XeOperand& b, long long m, long long n, long long k, const XeOutput& out,
-            cudaStream_t st) {
-    CUtensorMap tm_a, tm_b, tm_out;
+int make_problem(const XeProduct& x, XeProblem* out) {
+    XeProblem& p = *out;
+    const XeOutput& o = x.out;
     int rc;
-    if ((rc = operand_map(&tm_a, a)) || (rc = operand_map(&tm_b, b))) return rc;
-    const bool f32 = epi == XE_F32;
-    if (epi == XE_STATS) {
-        tm_out = tm_a;
+    if ((rc = operand_map(&p.tm_a, x.a)) || (rc = operand_map(&p.tm_b, x.b))) return rc;
+    const bool f32 = x.epi == XE_F32;
+    const int es = f32 ? 4 : 2;
+    p.plain = x.epi != XE_STATS && (o.pitch * es) % 16 != 0;
+    if (p.plain && (o.splits > 1 || x.epi > XE_BF16)) return fail(WINO_E_BADARG, "xent: buffer rows must be multiples of 16 bytes");
+    if (x.epi == XE_STATS || p.plain) {
+        p.tm_out = p.tm_a;
     } else {
-        const int es = f32 ? 4 : 2;
-        const int planes = f32 ? out.splits : epi == XE_DZ ? a.planes : 1;
-        const unsigned long long dims[3] = {(unsigned long long)n, (unsigned long long)m, (unsigned long long)planes};
-        const unsigned long long strides[2] = {(unsigned long long)out.pitch * es, (unsigned long long)(out.pitch * m) * es};
+        const int planes = f32 ? o.splits : x.epi == XE_DZ ? x.a.planes : 1;
+        const unsigned long long dims[3] = {(unsigned long long)x.n, (unsigned long long)x.m, (unsigned long long)planes};
+        const unsigned long long strides[2] = {(unsigned long long)o.pitch * es, (unsigned long long)(o.pitch * x.m) * es};
         const unsigned box[3] = {(unsigned)(128 / es), 32u, 1u};
-        if ((rc = encode_tensor_map(&tm_out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, out.ptr, dims,
-                                    strides, box, 1)))
+        if ((rc = encode_tensor_map(&p.tm_out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1)))
             return rc;
     }
-    XeParams p = {};
-    p.m = m; p.n = n;
-    p.mpairs = (int)((m + XE_BM - 1) / XE_BM);
-    p.nblocks = (int)((n + XE_BN - 1) / XE_BN);
-    p.kchunks = (int)((k + XE_BK - 1) / XE_BK);
-    p.splits = out.splits;
-    p.block = a.planes == 3 ? 4 : 16;
-    if (a.planes == 3) {
+    p.m = x.m; p.n = x.n;
+    p.mpairs = (int)((x.m + XE_BM - 1) / XE_BM);
+    p.nblocks = (int)((x.n + XE_BN - 1) / XE_BN);
+    p.kchunks = (int)((x.k + XE_BK - 1) / XE_BK);
+    p.splits = o.splits;
+    p.tiles = (long long)p.mpairs * p.nblocks;
+    p.units = p.tiles * p.splits;
+    p.block = x.a.planes == 3 ? 4 : 16;
+    if (x.a.planes == 3) {
         static const unsigned char pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
         p.pairs = 6;
         for (int i = 0; i < 6; ++i) { p.pa[i] = pa[i]; p.pb[i] = pb[i]; }
     } else {
         p.pairs = 1;
+        p.pa[0] = p.pb[0] = 0;
     }
-    p.idesc = make_idesc(OP_BF16, XE_BN, XE_BM) | (a.along_rows ? 1u << 15 : 0u) | (b.along_rows ? 1u << 16 : 0u);
+    p.a_mn = x.a.along_rows;
+    p.b_mn = x.b.along_rows;
+    p.idesc = make_idesc(OP_BF16, XE_BN, XE_BM) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
+    p.add = o.add;
+    p.out_ptr = o.ptr; p.out_pitch = o.pitch;
+    p.scale = o.scale;
+    p.bias = o.bias; p.target = o.target; p.col_base = o.col_base;
+    p.stats = o.stats; p.zsum = o.zsum; p.zt = o.zt;
+    p.lse = o.lse; p.rowg = o.rowg; p.rule = o.rule;
+    p.db_part = o.db_part; p.db_pitch = o.db_pitch;
+    return WINO_OK;
+}
+
+}  // namespace
+
+int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
+    static_assert(sizeof(XeParams) <= 4096, "kernel parameters");
+    XeParams p;
+    int rc;
+    p.zero = prod[0].out.zero;
+    for (int i = 0; i < count; ++i)
+        if ((rc = make_problem(prod[i], &p.prob[i]))) return rc;
+    p.lead = 0;
+    if (count == 1) {
+        p.prob[1].units = 0;
+    } else {
+        // ring slots of a unit, and about six more for its epilogue; the product with the longer units goes first
+        auto cost = [](const XeProblem& q) { return (double)q.kchunks / q.splits * q.pairs + 6.0; };
+        if (cost(p.prob[0]) < cost(p.prob[1])) { const XeProblem t = p.prob[0]; p.prob[0] = p.prob[1]; p.prob[1] = t; }
+        const long long pairs = sm_count() / 2, over = p.prob[0].units % pairs;
+        if (over) {
+            const long long lead = (long long)(cost(p.prob[0]) / cost(p.prob[1]) + 0.5), most = p.prob[1].units / (pairs - over);
+            p.lead = (int)(lead < most ? lead : most);
+        }
+    }
     if ((rc = status_word(&p.status))) return rc;
-    p.add = out.add;
-    p.scale = out.scale;
-    p.bias = out.bias; p.target = out.target; p.col_base = out.col_base;
-    p.stats = out.stats; p.zsum = out.zsum; p.zt = out.zt;
-    p.lse = out.lse; p.rowg = out.rowg; p.rule = out.rule;
-    p.db_part = out.db_part; p.db_pitch = out.db_pitch;
-    if (!a.along_rows && !b.along_rows) {
-        if (epi == XE_F32) return run<XE_F32, 1, false, false>(tm_a, tm_b, tm_out, p, st);
-        if (epi == XE_STATS) return run<XE_STATS, 1, false, false>(tm_a, tm_b, tm_out, p, st);
-        if (epi == XE_STATS_E) return run<XE_STATS_E, 1, false, false>(tm_a, tm_b, tm_out, p, st);
-        if (epi == XE_DZ) return a.planes == 3 ? run<XE_DZ, 3, false, false>(tm_a, tm_b, tm_out, p, st) : run<XE_DZ, 1, false, false>(tm_a, tm_b, tm_out, p, st);
-    } else if (!a.along_rows) {
-        if (epi == XE_F32) return run<XE_F32, 1, false, true>(tm_a, tm_b, tm_out, p, st);
-        if (epi == XE_BF16) return run<XE_BF16, 1, false, true>(tm_a, tm_b, tm_out, p, st);
-    } else if (b.along_rows) {
-        if (epi == XE_F32) return run<XE_F32, 1, true, true>(tm_a, tm_b, tm_out, p, st);
-        if (epi == XE_BF16) return run<XE_BF16, 1, true, true>(tm_a, tm_b, tm_out, p, st);
+    switch (prod[0].epi) {
+        case XE_F32: return run<XE_F32, 1>(p, st);
+        case XE_BF16: return run<XE_BF16, 1>(p, st);
+        case XE_STATS: return run<XE_STATS, 1>(p, st);
+        case XE_STATS_E: return run<XE_STATS_E, 1>(p, st);
+        case XE_DZ: return prod[0].a.planes == 3 ? run<XE_DZ, 3>(p, st) : run<XE_DZ, 1>(p, st);
     }
     return fail(WINO_E_BADARG, "xent: no kernel for this product");
 }

@@ -10,42 +10,58 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODES, REDUCTION_CODES, XentDesc, check, lib
-from .conv import _TORCH_DTYPE, _code, _ptr
+from .conv import _TORCH_DTYPE, _code
+
+
+# The current stream's handle by device index.  torch.cuda.current_stream builds a Stream object first, 2 to 3 us of a call
+# that otherwise costs about 8; this is what it asks.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(fn, device_index, *args):
+    """fn(*args, stream) with the tensors' device current and that device's current stream."""
+    if torch.cuda.current_device() == device_index:
+        return check(fn(*args, _raw_stream(device_index)))
+    with torch.cuda.device(device_index):
+        return check(fn(*args, _raw_stream(device_index)))
 
 
 def _rows(t, what):
-    """(rows, cols, pitch) of a CUDA matrix whose rows are contiguous; any contiguous tensor counts as one long row."""
-    if not t.is_cuda:
-        raise ValueError("libwino needs CUDA tensors (%s)" % what)
+    """(rows, cols, pitch) of a matrix whose rows are contiguous; any contiguous tensor counts as one long row."""
     if t.is_contiguous():
-        return 1, t.numel(), t.numel()
+        n = t.numel()
+        return 1, n, n
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
         return t.shape[0], t.shape[1], t.stride(0)
     raise ValueError("%s must be contiguous, or a matrix with contiguous rows" % what)
 
 
-def _dropout(name, x, p, seed, offset, offset_dev, out):
-    dt = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16}.get(x.dtype)
+_DROPOUT_DTYPE = {torch.float32: _lib.FP32, torch.bfloat16: _lib.BF16}
+
+
+def _dropout(fn, x, p, seed, offset, offset_dev, out):
+    dt = _DROPOUT_DTYPE.get(x.dtype)
     if dt is None:
         raise ValueError("dropout takes float32 or bfloat16, not %s" % x.dtype)
+    if not x.is_cuda:
+        raise ValueError("libwino needs CUDA tensors")
     if not (0.0 <= p <= 1.0):
         raise ValueError("p must lie in [0, 1]")
     if not (0 <= seed < 2 ** 64 and 0 <= offset < 2 ** 64):
         raise ValueError("seed and offset are unsigned 64-bit integers")
+    rows, cols, ldx = _rows(x, "input")
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError("out must have the input's shape, dtype and device")
     if offset_dev is not None and (offset_dev.dtype != torch.int64 or offset_dev.numel() != 1 or offset_dev.device != x.device):
         raise ValueError("offset_dev must be one int64 on the input's device")
-    rows, cols, ldx = _rows(x, "input")
     orows, ocols, ldy = _rows(out, "output")
-    if (rows, cols) != (orows, ocols):      # one of the two is a strided matrix: take both by rows
+    if rows != orows or cols != ocols:      # one of the two is a strided matrix: take both by rows
         rows, cols = x.shape
         ldx, ldy = (t.stride(0) if not t.is_contiguous() else cols for t in (x, out))
-    with torch.cuda.device(x.device):
-        check(getattr(lib(), name)(dt, rows, cols, ldx, ldy, p, seed, offset, _ptr(offset_dev), _ptr(x), _ptr(out),
-                                   ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    _call(fn, x.get_device(), dt, rows, cols, ldx, ldy, p, seed, offset, None if offset_dev is None else offset_dev.data_ptr(),
+          x.data_ptr(), out.data_ptr())
     return out
 
 
@@ -55,12 +71,12 @@ def dropout(x, p, seed, offset=0, offset_dev=None, out=None):
     p is met to 2^-17 (``include/wino.h``: T = round(65536 p), scale 65536 / (65536 - T)).  The element index is that of
     the dense tensor, whatever its strides or type.  Draw another mask with another offset; ``offset_dev`` (one int64 on
     the device, added to offset when the kernel runs) does that for a captured graph.  ``out`` may be x."""
-    return _dropout("wino_dropout_forward", x, p, seed, offset, offset_dev, out)
+    return _dropout(lib().wino_dropout_forward, x, p, seed, offset, offset_dev, out)
 
 
 def dropout_backward(dy, p, seed, offset=0, offset_dev=None, out=None):
     """Gradient through ``dropout`` with the same p, seed and offset."""
-    return _dropout("wino_dropout_backward", dy, p, seed, offset, offset_dev, out)
+    return _dropout(lib().wino_dropout_backward, dy, p, seed, offset, offset_dev, out)
 
 
 class LinearXent:
@@ -92,44 +108,44 @@ class LinearXent:
             self.workspace = workspace
         else:
             self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
+        self._desc_ref, self._ws_size = ctypes.byref(s), self.workspace.numel() * self.workspace.element_size()
+        self._index = self.workspace.get_device()
+        self._like = torch.empty(0, dtype=torch.float32, device=self.workspace.device)
 
-    def _matrix(self, t, what, rows, ld, dtype=None):
+    def _matrix(self, t, what, rows, ld):
         d = self.desc.d
-        if not t.is_cuda or t.device != self.workspace.device:
+        if t.get_device() != self._index:
             raise ValueError("%s must be on the plan's device" % what)
         if t.dtype != self.io_dtype:
             raise ValueError("%s dtype %s, expected %s" % (what, t.dtype, self.io_dtype))
-        if tuple(t.shape) != (rows, d) or (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) != (ld or d)):
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != d or (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) != (ld or d)):
             raise ValueError("%s must be (%d, %d) with rows %d elements apart" % (what, rows, d, ld or d))
-        return t
+        return t.data_ptr()
 
     def _vector(self, t, what, count, dtype):
-        if not t.is_cuda or t.device != self.workspace.device or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
+        if t.get_device() != self._index or t.dtype != dtype or t.numel() != count or not t.is_contiguous():
             raise ValueError("%s must be %d contiguous %s values on the plan's device" % (what, count, dtype))
-        return t
+        return t.data_ptr()
 
     def _inputs(self, x, w, target, bias):
         s = self.desc
-        self._matrix(x, "x", s.n, s.ldx)
-        self._matrix(w, "w", s.v, s.ldw)
-        self._vector(target, "target", s.n, torch.int64)
+        if self._index < 0:
+            raise ValueError("libwino needs CUDA tensors")
         if bool(s.has_bias) != (bias is not None):
             raise ValueError("the plan was made with bias=%s" % bool(s.has_bias))
-        if bias is not None:
-            self._vector(bias, "bias", s.v, torch.float32)
+        return (self._matrix(x, "x", s.n, s.ldx), self._matrix(w, "w", s.v, s.ldw),
+                None if bias is None else self._vector(bias, "bias", s.v, torch.float32), self._vector(target, "target", s.n, torch.int64))
 
-    def _losses(self, device):
+    def _losses(self):
         s = self.desc
-        return torch.empty((s.n,) if s.reduction == _lib.NONE else (), dtype=torch.float32, device=device)
+        return self._like.new_empty((s.n,) if s.reduction == _lib.NONE else ())
 
     def forward(self, x, w, target, bias=None):
         """(loss, lse): loss is a scalar (or n values), lse_i = log sum_j exp z_ij (0 for an ignored row)."""
-        self._inputs(x, w, target, bias)
-        loss, lse = self._losses(x.device), torch.empty(self.desc.n, dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
-            check(lib().wino_xent_forward(ctypes.byref(self.desc), _ptr(x), _ptr(w), _ptr(bias), _ptr(target), _ptr(loss),
-                                          _ptr(lse), _ptr(self.workspace), self.workspace.numel() * self.workspace.element_size(),
-                                          ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        args = self._inputs(x, w, target, bias)
+        loss, lse = self._losses(), self._like.new_empty((self.desc.n,))
+        _call(lib().wino_xent_forward, self._index, self._desc_ref, *args, loss.data_ptr(), lse.data_ptr(), self.workspace.data_ptr(),
+              self._ws_size)
         return loss, lse
 
     def loss_and_grad(self, x, w, target, bias=None, dloss=None, dx=None, dw=None, need_dx=True, need_dw=True):
@@ -140,24 +156,21 @@ class LinearXent:
         s = self.desc
         if not self.grad:
             raise ValueError("the plan was made for forward alone (grad=False)")
-        self._inputs(x, w, target, bias)
+        args = self._inputs(x, w, target, bias)
         if dloss is not None:
-            self._vector(dloss, "dloss", s.n if s.reduction == _lib.NONE else 1, torch.float32)
+            dloss = self._vector(dloss, "dloss", s.n if s.reduction == _lib.NONE else 1, torch.float32)
 
-        def result(t, need, what, rows, ld):
+        def result(t, need, what, like, rows, ld):
             if not need:
-                return None
-            if t is None:
-                t = torch.empty((rows, ld or s.d), dtype=self.io_dtype, device=x.device)[:, :s.d]
-            return self._matrix(t, what, rows, ld)
+                return None, None
+            if t is None:                   # the input's own shape where both are dense
+                t = torch.empty_like(like) if not ld and like.is_contiguous() else like.new_empty((rows, ld or s.d))[:, :s.d]
+            return t, self._matrix(t, what, rows, ld)
 
-        dx = result(dx, need_dx, "dx", s.n, s.lddx)
-        dw = result(dw, need_dw, "dw", s.v, s.lddw)
-        db = torch.empty(s.v, dtype=torch.float32, device=x.device) if s.has_bias else None
-        loss = self._losses(x.device)
-        with torch.cuda.device(x.device):
-            check(lib().wino_xent_grad(ctypes.byref(s), _ptr(x), _ptr(w), _ptr(bias), _ptr(target), _ptr(dloss), _ptr(loss), None,
-                                       _ptr(dx), _ptr(dw), _ptr(db), _ptr(self.workspace),
-                                       self.workspace.numel() * self.workspace.element_size(),
-                                       ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        dx, dx_ptr = result(dx, need_dx, "dx", x, s.n, s.lddx)
+        dw, dw_ptr = result(dw, need_dw, "dw", w, s.v, s.lddw)
+        db = torch.empty_like(bias) if s.has_bias else None
+        loss = self._losses()
+        _call(lib().wino_xent_grad, self._index, self._desc_ref, *args, dloss, loss.data_ptr(), None, dx_ptr, dw_ptr,
+              None if db is None else db.data_ptr(), self.workspace.data_ptr(), self._ws_size)
         return loss, dx, dw, db
