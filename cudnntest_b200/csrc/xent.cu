@@ -85,8 +85,7 @@ struct RowArgs {
     float* lse_out;             // caller's, or NULL
     float* rowloss;             // scratch, or the caller's (WINO_NONE)
     float* rowg;                // a row's own weight in the gradient; 0: does not count
-    float* loss;                // mean or sum, written by the block that finishes last; NULL: left to the rows
-    int mean;
+    XeLoss loss;                // written by the block that finishes last; loss NULL: left to the rows, or to a later kernel
     int* count;                 // [0] rows that count, [1] blocks that are done (both set to 0 by the kernel before)
     int* status;
 };
@@ -108,30 +107,21 @@ __device__ __forceinline__ bool finish_row(const RowArgs& a, long long row, floa
     return counts;
 }
 
-// The block that finishes last sums the rows' losses (in the same order whichever block that is).  All threads call it.
+// The block that finishes last sums the rows' losses (in the same order whichever block that is).  All threads call it; the
+// block's losses were written by warp 0, so only that warp waits for its stores.
 template <int THREADS>
 __device__ __forceinline__ void finish_loss(const RowArgs& a) {
-    if (!a.loss) return;
+    if (!a.loss.loss) return;
     __shared__ int last;
-    __shared__ double rs[THREADS / 32];
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.count + 1, 1) == (int)gridDim.x - 1;
+    if (threadIdx.x < 32) {
+        __threadfence();
+        __syncwarp();
+        if (threadIdx.x == 0) last = atomicAdd(a.count + 1, 1) == (int)gridDim.x - 1;
+    }
     __syncthreads();
     if (!last) return;
     __threadfence();
-    double sum = 0;
-#pragma unroll 4
-    for (long long i = threadIdx.x; i < a.n; i += THREADS) sum += __ldcg(a.rowloss + i);
-#pragma unroll
-    for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    if (threadIdx.x % 32 == 0) rs[threadIdx.x / 32] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < THREADS / 32; ++i) sum += rs[i];
-        const int count = __ldcg(a.count);
-        *a.loss = (float)(a.mean ? sum / (count > 0 ? count : 1) : sum);
-    }
+    xe_sum_losses<THREADS>(a.loss);
 }
 
 // joins (maximum, sum) pairs
@@ -355,9 +345,9 @@ __global__ void __launch_bounds__(THREADS, (SPLIT && QUADS > 1 ? 512 : 1024) / T
     finish_loss<THREADS>(a);
 }
 
-// The same for any v, in two kernels: one block per row for the statistics (the sum of several parts replaces the first), ...
-template <bool SPLIT>
-__global__ void __launch_bounds__(256, SPLIT ? 1 : 4) xe_wide_rows_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, const RowArgs a) {
+// The same for any v, in two kernels.  Statistics of split logits, one block per row (the sum of the parts replaces the
+// first); of unsplit ones they come with the product (XE_STATS_Z).
+__global__ void __launch_bounds__(256) xe_wide_rows_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, const RowArgs a) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float red[3][8];
@@ -372,11 +362,11 @@ __global__ void __launch_bounds__(256, SPLIT ? 1 : 4) xe_wide_rows_kernel(float*
     // four groups of four columns at a time, so that their loads overlap and the running maximum moves once
     for (int c0 = threadIdx.x * 4; c0 < v; c0 += 4096) {
         float e[4][4], m2 = m;
-        gather_groups<SPLIT>(e, zr, a.n * pitch, splits, c0, 1024, v, bias);
+        gather_groups<true>(e, zr, a.n * pitch, splits, c0, 1024, v, bias);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int c = c0 + q * 1024;
-            if (SPLIT && c < v) *reinterpret_cast<float4*>(zr + c) = make_float4(e[q][0], e[q][1], e[q][2], e[q][3]);
+            if (c < v) *reinterpret_cast<float4*>(zr + c) = make_float4(e[q][0], e[q][1], e[q][2], e[q][3]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (c + i < v) zsum += e[q][i];
@@ -414,9 +404,9 @@ __global__ void __launch_bounds__(256, SPLIT ? 1 : 4) xe_wide_rows_kernel(float*
     finish_loss<256>(a);
 }
 
-// ... and dz, two classes per thread, 32 rows per block, with the block's column sums.  bias: NULL where z has it already
+// dz, two classes per thread, 32 rows per block, with the block's column sums (z has the bias already)
 template <int PLANES>
-__global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ bias, const float* __restrict__ lse,
+__global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ lse,
                                                          const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
                                                          __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
     pdl_launch_dependents();
@@ -427,13 +417,12 @@ __global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict
     const long long r0 = (long long)part * XE_ROWS_PER_PART;
     const long long r1 = r0 + XE_ROWS_PER_PART < n ? r0 + XE_ROWS_PER_PART : n;
     float s0 = 0.f, s1 = 0.f;
-    const float b0 = bias ? bias[c] : 0.f, b1 = bias && c + 1 < v ? bias[c + 1] : 0.f;
 #pragma unroll 8
     for (long long r = r0; r < r1; ++r) {
         const float2 q = *reinterpret_cast<const float2*>(z + r * zpitch + c);
         const float l = lse[r], g = rowg[r];
         const long long t = target[r];
-        float a = xe_ex2((q.x + b0 - l) * XE_LOG2E) * rule.pf - rule.smooth_all, b = xe_ex2((q.y + b1 - l) * XE_LOG2E) * rule.pf - rule.smooth_all;
+        float a = xe_ex2((q.x - l) * XE_LOG2E) * rule.pf - rule.smooth_all, b = xe_ex2((q.y - l) * XE_LOG2E) * rule.pf - rule.smooth_all;
         if (t == c) a -= rule.smooth_t;
         if (t == c + 1) b -= rule.smooth_t;
         a = g == 0.f ? 0.f : a * g;
@@ -545,8 +534,11 @@ __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict_
 }
 
 // ---- few products: FP32 arithmetic on the caller's matrices --------------------------------------------------
-// Below some millions of products a tensor-core launch is mostly set-up (8 us each with one tile), and the operands fit
-// the L2 many times over: three plain kernels take 2 to 4 us each.
+// Below some millions of products a tensor-core launch is mostly set-up, and the operands fit the L2 many times over.
+// Measured (GPU time of a call, BF16 / FP32X3, us): loss of 16 x 1024 x 1000 (16M products) 12.4 / 12.4 against 14.4 / 18.9 on
+// tensor cores, of 512 x 256 x 256 (32M) 20.6 / 26.7 against 14.4 / 16.5; gradient of 32 x 4096 x 64 (8M) 18.5 / 20.6 against
+// 22.7 / 28.8.  The gradient's sums run one after the other over rows or classes: with 256 of them 23.8 / 24.8 against
+// 18.5 / 24.7, with 1000 of them 65 against 29.
 template <typename T>
 __device__ __forceinline__ void load4(float (&v)[4], const T* p, int left, bool aligned) {
     if (aligned && left >= 4) {
@@ -612,8 +604,8 @@ __global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restric
 // out[o][k] = scale sum_c coef(o, c) M[c][k]: dx (o rows, c classes, M = W) and dW (o classes, c rows, M = x; and dbias),
 // from dz in floats.  A block makes eight o by 128 k; its eight warps share the sum over c, whose coefficients sit in
 // shared memory.  A row that does not count has nothing but zeros there and is not read.
-constexpr int XE_SMALL_MAX = 1024;                 // most rows, most classes
-constexpr int XE_SMALL_GRAD_SMEM = XE_SMALL_MAX * 8 * 4;
+constexpr int XE_SMALL_MAX = 128;                  // most rows, most classes
+constexpr int XE_SMALL_GRAD_SMEM = 8 * 8 * 128 * 4;
 template <typename T>
 struct SmallGrad {
     const T* x; const T* w;
@@ -623,12 +615,17 @@ struct SmallGrad {
     const float* dz;
     int n, d, v, dzpitch, kblocks, dx_blocks;
     XeScale scale;
+    XeLoss loss;                      // summed by the last block
 };
 template <typename T>
 __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a) {
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(16) float coef[];            // [c][8], then [warp][8][128] sums
+    if (a.loss.loss && blockIdx.x == gridDim.x - 1) {
+        xe_sum_losses<256>(a.loss);
+        return;
+    }
     const bool is_dw = (int)blockIdx.x >= a.dx_blocks;
     const int b = is_dw ? blockIdx.x - a.dx_blocks : blockIdx.x;
     const int o0 = b / a.kblocks * 8, k = (b % a.kblocks) * 128 + (threadIdx.x % 32) * 4, warp = threadIdx.x / 32;
@@ -693,7 +690,7 @@ unsigned loop_blocks(long long items) {
 }
 
 // ---- plan ----------------------------------------------------------------------------------------------------
-constexpr long long XE_SMALL_PRODUCTS = 4ll << 20;   // n v d up to which xe_small_* run
+constexpr long long XE_SMALL_PRODUCTS = 16ll << 20;   // n v d up to which xe_small_* run
 
 struct Plan {
     int planes, es, dp;
@@ -701,29 +698,12 @@ struct Plan {
     bool pack_x, pack_w;
     bool small;                          // FP32 arithmetic instead of tensor cores
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
-    int splits_z, splits_dx, splits_dw;
+    int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
     int zpitch, piece, pieces, dzpitch, parts;
     bool dx_direct, dw_direct;           // the product's epilogue stores the caller's matrix
     int dpitch;                          // of float dx / dw buffers in the scratch
-    size_t off_x, off_w, off_z, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_count, off_dz, off_db, off_dx, off_dw, total;
+    size_t off_x, off_w, off_z, off_stats, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_count, off_dz, off_db, off_dx, off_dw, total;
 };
-
-// Parts of a contraction of `chunks` ring slots (times `products` plane pairs), so that tiles * parts fills the CTA pairs in
-// as few whole turns as possible.  Estimated time: turns of the slots (0.28 us each on a pair) and of the epilogue (1.5 us),
-// and, for more than one part, writing and reading the floats of every part (5 TB/s) and, where `join` is set, a launch.
-int split_count(long long rows, long long cols, long long chunks, int products, bool join) {
-    const long long pairs = sm_count() / 2, tiles = ((rows + XE_BM - 1) / XE_BM) * ((cols + XE_BN - 1) / XE_BN);
-    if (tiles >= 4 * pairs || tiles == 0 || chunks == 1) return 1;
-    const double part_us = (double)rows * (double)cols * 8.0 / 5e6;
-    int best = 1;
-    double best_us = 1e30;
-    for (long long s = 1; s <= chunks && s <= 64 && (s == 1 || tiles * s <= 4 * pairs); ++s) {
-        const double us = (double)((tiles * s + pairs - 1) / pairs) * ((double)((chunks + s - 1) / s) * products * 0.28 + 1.5) +
-                          (s > 1 || !join ? part_us * (double)s : 0.0) + (s > 1 && join ? 3.0 : 0.0);
-        if (us < best_us) { best_us = us; best = (int)s; }
-    }
-    return best;
-}
 
 // rows of dz a block of xe_rows_kernel sums up: as many blocks as fit the GPU twice at 1024 threads an SM
 int row_blocks(long long n, int threads) {
@@ -733,6 +713,32 @@ int row_blocks(long long n, int threads) {
 constexpr int XE_ROWS_MAX_V = 512 * 4 * 4;          // widest row of xe_rows_kernel: wider ones spill, and one block an SM is
                                                     // slower than two kernels (1024 x 21841: 130 us against 92)
 int row_threads(int v) { return v <= 512 ? 128 : v <= 4096 ? 256 : 512; }
+
+// Parts of a contraction of `chunks` ring slots (times `products` plane pairs), and columns of a tile (256 or 128), so that
+// the CTA pairs are filled in as few whole turns as possible.  Estimated time: turns of the slots (0.28 us each on a pair;
+// 0.2 us for half the columns, which need 24 of the 32 KB) and of the epilogue (1.5 us; 0.75 us), and, for more than one part,
+// writing and reading the floats of every part (5 TB/s) and, where `join` is set, a launch.
+struct Cut {
+    int splits, bn;
+    double us;
+};
+Cut cut_product(long long rows, long long cols, long long chunks, int products, bool join) {
+    const long long pairs = sm_count() / 2;
+    const double part_us = (double)rows * (double)cols * 8.0 / 5e6;
+    Cut best = {1, XE_BN, 1e30};
+    if (rows == 0) return best;
+    for (int bn = XE_BN; bn >= 128; bn -= 128) {
+        const long long tiles = ((rows + XE_BM - 1) / XE_BM) * ((cols + bn - 1) / bn);
+        if (bn < XE_BN && tiles >= 8 * pairs) break;
+        const double slot = bn == XE_BN ? 0.28 : 0.2, end = bn == XE_BN ? 1.5 : 0.75;
+        for (long long s = 1; s <= chunks && s <= 64 && (s == 1 || tiles * s <= 4 * pairs); ++s) {
+            const double us = (double)((tiles * s + pairs - 1) / pairs) * ((double)((chunks + s - 1) / s) * products * slot + end) +
+                              (s > 1 || !join ? part_us * (double)s : 0.0) + (s > 1 && join ? 3.0 : 0.0);
+            if (us < best.us * 0.97) best = {(int)s, bn, us};
+        }
+    }
+    return best;
+}
 
 int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     if (!d) return fail(WINO_E_BADARG, "xent: NULL descriptor");
@@ -761,7 +767,8 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.pack_x = !bf16 || p.ldx % 8 != 0 || (grad && d->has_ignore);
     p.pack_w = !bf16 || p.ldw % 8 != 0;
     const long long kd = (d->d + XE_BK - 1) / XE_BK;
-    p.splits_z = split_count(n, v, kd, products, false);
+    const Cut cz = cut_product(n, v, kd, products, false);
+    p.splits_z = cz.splits;
     p.zpitch = round_up(d->v, 4);
     const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll;
     const bool fits = z_bytes * p.splits_z + (grad ? dz_bytes : 0) <= limit;
@@ -769,7 +776,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured 6.5 TB/s and 1.4 PFLOP/s the
     // product is the dearer one from d = 1000 (200) on.
     const bool few = n * v <= 64ll * XE_BM * XE_BN;
-    p.small = n > 0 && d->v <= XE_SMALL_MAX && (!grad || n <= XE_SMALL_MAX) && n * v <= XE_SMALL_PRODUCTS / d->d;
+    p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
@@ -777,7 +784,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     } else if (few && fits) p.kept = true;
     else if (grad && bf16 && !d->has_bias && dz_bytes <= limit) p.exps = true;
     else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
+    if (!grad && p.splits_z == 1 && !p.small) p.kept = false;          // statistics are all that is wanted
     if (!p.kept) p.splits_z = 1;
+    p.bn_z = p.kept && (p.splits_z > 1 || d->v <= XE_ROWS_MAX_V) ? cz.bn : XE_BN;                       // the other epilogues make statistics of 128 columns a warp
     p.piece = d->v;
     p.pieces = 1;
     if (grad && !p.kept && !p.exps) {
@@ -791,8 +800,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     }
     p.dzpitch = round_up(p.piece, 8);
     p.dpitch = round_up(d->d, 4);
-    p.splits_dx = split_count(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true);
-    p.splits_dw = split_count(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
+    Cut cx = cut_product(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true), cw = cut_product(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
+    p.splits_dx = cx.splits; p.splits_dw = cw.splits;
+    p.bn_dx = cx.bn; p.bn_dw = cw.bn;
     // more than one piece adds up in floats: in dx itself, or in the scratch
     p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
     p.dw_direct = p.splits_dw == 1;
@@ -810,8 +820,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.off_zt = take(un * 4);
     p.off_count = take(8);               // rows that count, blocks that are done
     const size_t vtiles = (size_t)((v + XE_STAT_COLS - 1) / XE_STAT_COLS);
-    p.off_zsum = take(p.kept || d->label_smoothing <= 0.f ? 0 : vtiles * un * 4);
-    p.off_z = take(p.kept ? un * p.zpitch * 4 * p.splits_z : vtiles * un * 8);
+    p.off_zsum = take(d->label_smoothing > 0.f ? vtiles * un * 4 : 0);
+    p.off_stats = take(vtiles * un * 8);
+    p.off_z = take(p.kept ? un * p.zpitch * 4 * p.splits_z : 0);
     p.off_x = take(p.pack_x ? un * p.dp * 2 * p.planes : 0);
     p.off_w = take(p.pack_w ? (size_t)v * p.dp * 2 * p.planes : 0);
     if (grad) {
@@ -855,7 +866,7 @@ int launch_rows(int planes, unsigned blocks, cudaStream_t st, const float* z, in
     if (planes < 0) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, false, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, false, false>);
     if (planes == 1) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, true, false>);
     if (planes == 3) return split ? go(xe_rows_kernel<THREADS, QUADS, 3, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 3, true, false>);
-    if constexpr (THREADS * QUADS * 4 <= XE_SMALL_MAX)
+    if constexpr (THREADS == 128)
         return split ? go(xe_rows_kernel<THREADS, QUADS, 0, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 0, true, false>);
     return fail(WINO_E_BADARG, "xent: no row kernel");
 }
@@ -868,7 +879,7 @@ int launch_small_logits(const void* x, long long ldx, const void* w, long long l
 
 template <typename T>
 int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* db, const wino_xent_desc& d, const Plan& p, const float* dz, const XeScale& scale,
-                      cudaStream_t st) {
+                      const XeLoss& loss, cudaStream_t st) {
     SmallGrad<T> a;
     a.x = (const T*)x; a.w = (const T*)w; a.dx = (T*)dx; a.dw = (T*)dw; a.db = db;
     a.ldx = p.ldx; a.ldw = p.ldw; a.lddx = p.lddx; a.lddw = p.lddw;
@@ -876,8 +887,9 @@ int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* d
     a.kblocks = (d.d + 127) / 128;
     a.dx_blocks = dx ? (d.n + 7) / 8 * a.kblocks : 0;
     a.scale = scale;
+    a.loss = loss;
     const int dw_blocks = dw || db ? (d.v + 7) / 8 * a.kblocks : 0;
-    return xe_launch(xe_small_grad_kernel<T>, (unsigned)(a.dx_blocks + dw_blocks), 256, XE_SMALL_GRAD_SMEM, st, a);
+    return xe_launch(xe_small_grad_kernel<T>, (unsigned)(a.dx_blocks + dw_blocks + (loss.loss ? 1 : 0)), 256, XE_SMALL_GRAD_SMEM, st, a);
 }
 
 int finish(const wino_xent_desc& d, const Plan& p, const float* buf, int splits, long long rows, void* out, long long ld, cudaStream_t st) {
@@ -941,9 +953,16 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     ra.smooth = s; ra.inv_v = (float)(1.0 / (double)v);
     ra.lse = f(p.off_lse); ra.lse_out = lse; ra.rowg = f(p.off_rowg);
     ra.rowloss = d.reduction == WINO_NONE ? loss : f(p.off_rowloss);
-    ra.loss = d.reduction == WINO_NONE ? nullptr : loss;
-    ra.mean = d.reduction == WINO_MEAN;
     ra.count = reinterpret_cast<int*>(ws + p.off_count);
+    // the sum of the losses goes to the rows' last block, or, where gradients follow and a warp is done with it in good
+    // time, to one that idles in their kernel
+    const bool products = grad && (dx || dw || db);
+    XeLoss sum;
+    sum.loss = d.reduction == WINO_NONE ? nullptr : loss;
+    sum.rowloss = ra.rowloss; sum.n = n; sum.count = ra.count;
+    sum.mean = d.reduction == WINO_MEAN;
+    const bool later = products && (dx || dw) && n <= 8192;
+    if (!later) ra.loss = sum;
     if ((rc = status_word(&ra.status))) return rc;
     const float* b = d.has_bias ? bias : nullptr;
     const bool wide = d.v > XE_ROWS_MAX_V;
@@ -953,12 +972,13 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     scale.count = ra.count;
     scale.dloss = d.reduction == WINO_NONE ? nullptr : dloss;
     scale.factor = dz_factor;
-    scale.mean = ra.mean;
+    scale.mean = sum.mean;
 
-    const bool products = grad && (dx || dw || db);
-    XeProduct pz = {p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
+    const bool kept_stats = p.kept && wide && p.splits_z == 1;
+    XeProduct pz = {kept_stats ? XE_STATS_Z : p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
+    pz.bn = p.bn_z;
     pz.out.zero = ra.count;
-    if (p.kept) {
+    if (p.kept && !kept_stats) {
         float* z = f(p.off_z);
         pz.out.ptr = z;
         pz.out.pitch = p.zpitch;
@@ -968,7 +988,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         else rc = launch_small_logits<float>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
         if (rc) return rc;
         if (wide) {
-            rc = xe_launch(p.splits_z > 1 ? xe_wide_rows_kernel<true> : xe_wide_rows_kernel<false>, (unsigned)n, 256, 0, st, z, p.splits_z, d.v, p.zpitch, b, ra);
+            rc = xe_launch(xe_wide_rows_kernel, (unsigned)n, 256, 0, st, z, p.splits_z, d.v, p.zpitch, b, ra);
         } else {
             const unsigned blocks = (unsigned)row_blocks(n, row_threads(d.v));
             auto rows_fn = d.v <= 512 ? launch_rows<128, 1> : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
@@ -979,10 +999,13 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     } else {
         pz.out.bias = b;
         pz.out.target = target;
-        pz.out.stats = reinterpret_cast<float2*>(ws + p.off_z);
+        pz.out.stats = reinterpret_cast<float2*>(ws + p.off_stats);
         pz.out.zsum = d.label_smoothing > 0.f ? f(p.off_zsum) : nullptr;
         pz.out.zt = f(p.off_zt);
-        if (p.exps) {
+        if (kept_stats) {
+            pz.out.ptr = f(p.off_z);
+            pz.out.pitch = p.zpitch;
+        } else if (p.exps) {
             pz.out.ptr = dz;
             pz.out.pitch = p.dzpitch;
         }
@@ -993,8 +1016,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
 
     if (!products) return WINO_OK;
     if (p.small)
-        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, st)
-                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, st);
+        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st)
+                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st);
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, vc = d.v - v0 < p.piece ? d.v - v0 : p.piece;
         XeOperand wp = ow;                 // the piece's rows of W
@@ -1002,8 +1025,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         wp.rows = vc;
         if (p.kept && wide) {
             const unsigned grid = (unsigned)((vc + 255) / 256) * (unsigned)p.parts;
-            if (p.planes == 1) rc = xe_launch(xe_wide_dz_kernel<1>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, p.splits_z > 1 ? nullptr : b, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
-            else rc = xe_launch(xe_wide_dz_kernel<3>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, p.splits_z > 1 ? nullptr : b, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
+            if (p.planes == 1) rc = xe_launch(xe_wide_dz_kernel<1>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
+            else rc = xe_launch(xe_wide_dz_kernel<3>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
         } else if (p.exps) {
             rc = xe_launch(xe_dz_from_exp_kernel, loop_blocks(n * ((p.dzpitch / 8 + 1023) / 1024) * 256), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt, ra.lse, ra.rowg, target, dzr);
         } else if (!p.kept) {
@@ -1025,9 +1048,11 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         const bool bf16 = p.planes == 1, first = i == 0, last = i == p.pieces - 1;
         XeProduct prod[2];
         int count = 0;
-        auto product = [&](const XeOperand& a, const XeOperand& b, long long rows, long long k, bool direct, int splits, bool add, void* out, long long ld, float* buf) {
+        auto product = [&](const XeOperand& a, const XeOperand& b, long long rows, long long k, bool direct, int splits, int bn, bool add, void* out,
+                           long long ld, float* buf) {
             XeProduct& q = prod[count++];
             q = {direct && bf16 ? XE_BF16 : XE_F32, a, b, rows, d.d, k, XeOutput()};
+            q.bn = bn;
             q.out.scale = scale;
             q.out.add = add;
             q.out.ptr = direct ? out : buf;
@@ -1039,19 +1064,20 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         if (dx) {
             XeOperand wr = wp;
             wr.along_rows = true;
-            product(odz, wr, n, vc, p.dx_direct, p.splits_dx, !first, dx, p.lddx, f(p.off_dx));
+            product(odz, wr, n, vc, p.dx_direct, p.splits_dx, p.bn_dx, !first, dx, p.lddx, f(p.off_dx));
         }
         if (dw) {
             XeOperand zr = odz, xr = ox;
             zr.along_rows = xr.along_rows = true;
-            product(zr, xr, vc, n, p.dw_direct, p.splits_dw, false, dw_at, p.lddw, f(p.off_dw));
+            product(zr, xr, vc, n, p.dw_direct, p.splits_dw, p.bn_dw, false, dw_at, p.lddw, f(p.off_dw));
         }
         // Both in one launch where their epilogues agree and one of them has few tiles: the other fills the SMs that it
         // leaves idle (256 x 25088 x 1000: 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU
         // runs at its power limit either way (8192 x 4096 x 50021: 8.2 ms apart, 8.4 ms together).
-        const long long cols = (d.d + XE_BN - 1) / XE_BN;
-        const long long tiles_x = (n + XE_BM - 1) / XE_BM * cols * p.splits_dx, tiles_w = ((long long)vc + XE_BM - 1) / XE_BM * cols * p.splits_dw;
-        if (count == 2 && prod[0].epi == prod[1].epi && (tiles_x < tiles_w ? tiles_x : tiles_w) < sm_count()) {
+        const long long tiles_x = (n + XE_BM - 1) / XE_BM * ((d.d + p.bn_dx - 1) / p.bn_dx) * p.splits_dx;
+        const long long tiles_w = ((long long)vc + XE_BM - 1) / XE_BM * ((d.d + p.bn_dw - 1) / p.bn_dw) * p.splits_dw;
+        if (first && later) prod[0].out.loss = sum;
+        if (count == 2 && prod[0].epi == prod[1].epi && p.bn_dx == p.bn_dw && (tiles_x < tiles_w ? tiles_x : tiles_w) < sm_count()) {
             if ((rc = xe_gemm(prod, 2, st))) return rc;
         } else {
             for (int k = 0; k < count; ++k)

@@ -23,7 +23,8 @@ enum XeEpilogue {
     XE_BF16 = 1,      // scale, round and store
     XE_STATS = 2,     // per row and 128 columns: maximum, sum of exponentials (and of logits); the target's logit
     XE_STATS_E = 3,   // the same, and the exponentials exp(z - maximum) themselves, rounded to BF16
-    XE_DZ = 4,        // the gradient of the logits, rounded to BF16 (or split into three BF16 planes), and its column sums
+    XE_STATS_Z = 4,   // the same as XE_STATS, and the logits themselves (with the bias) as floats
+    XE_DZ = 5,        // the gradient of the logits, rounded to BF16 (or split into three BF16 planes), and its column sums
 };
 constexpr int XE_STAT_COLS = 128;
 
@@ -50,13 +51,43 @@ __device__ __forceinline__ float xe_scale(const XeScale& s) {
     return s.factor * (s.dloss ? *s.dloss : 1.f) * (s.mean ? 1.f / (float)(n > 0 ? n : 1) : 1.f);
 }
 
+// the mean or sum of the rows' losses
+struct XeLoss {
+    float* loss = nullptr;            // NULL: nothing to do
+    const float* rowloss = nullptr;
+    long long n = 0;
+    const int* count = nullptr;       // rows that count
+    int mean = 0;
+};
+// by the first THREADS threads of a block, all of which call it (one warp: no barrier)
+template <int THREADS>
+__device__ __forceinline__ void xe_sum_losses(const XeLoss& a) {
+    __shared__ double rs[THREADS / 32];
+    const int tid = threadIdx.x % THREADS;
+    double sum = 0;
+#pragma unroll 8
+    for (long long i = tid; i < a.n; i += THREADS) sum += __ldcg(a.rowloss + i);
+#pragma unroll
+    for (int w = 16; w >= 1; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    if (THREADS > 32) {
+        if (tid % 32 == 0) rs[tid / 32] = sum;
+        __syncthreads();
+        if (tid == 0)
+            for (int i = 1; i < THREADS / 32; ++i) sum += rs[i];
+    }
+    if (tid == 0) {
+        const int count = __ldcg(a.count);
+        *a.loss = (float)(a.mean ? sum / (count > 0 ? count : 1) : sum);
+    }
+}
+
 struct XeOutput {
-    void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16, XE_STATS_E: m rows; XE_DZ: [planes][m][pitch] BF16
+    void* ptr = nullptr;            // XE_F32: [splits][m][pitch] floats; XE_BF16, XE_STATS_E, XE_STATS_Z: m rows; XE_DZ: [planes][m][pitch] BF16
     long long pitch = 0;
     int splits = 1;                 // parts of the contraction, one buffer each (XE_F32)
     bool add = false;               // XE_F32: add instead of store
     XeScale scale;                  // XE_F32, XE_BF16: what the product is multiplied by
-    // XE_STATS, XE_STATS_E, XE_DZ
+    // XE_STATS*, XE_DZ
     const float* bias = nullptr;    // of column 0 of this product
     const long long* target = nullptr;
     int col_base = 0;               // class number of column 0
@@ -69,6 +100,7 @@ struct XeOutput {
     float* db_part = nullptr;       // [m / 32][db_pitch] column sums of 32 rows each, or NULL
     long long db_pitch = 0;
     int* zero = nullptr;            // two device words set to 0, or NULL
+    XeLoss loss;                    // summed by a warp that has nothing else to do
 };
 
 // one product of a (m x k) and b (n x k)^T, contraction length k
@@ -77,8 +109,9 @@ struct XeProduct {
     XeOperand a, b;
     long long m, n, k;
     XeOutput out;
+    int bn = XE_BN;                   // columns of a tile: 256, or 128 (XE_F32, XE_BF16)
 };
-// one or two products in one launch; two must have the same epilogue, XE_F32 or XE_BF16
+// one or two products in one launch; two must have the same epilogue, XE_F32 or XE_BF16, and the same bn
 int xe_gemm(const XeProduct* prod, int count, cudaStream_t st);
 
 __device__ __forceinline__ float xe_ex2(float x) {

@@ -1,7 +1,7 @@
 // The products of the linear softmax cross entropy (sm_100a): logits z = x W^T, dx = dz W, dW = dz^T x, one kernel with
 // the step that follows fused into its epilogue.
 //
-// CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles), for the reason given in gemm_tc_pair.cu: half of B comes from the
+// CTA pairs (tcgen05.mma.cta_group::2, 256 x 256 tiles; 256 x 128 where tiles are few), for the reason given in gemm_tc_pair.cu: half of B comes from the
 // partner's shared memory, so a 64-deep slice costs 32 KB of L2 reads per SM.  Operands are BF16; what changes between the
 // three products is along which axis of the stored matrix the contraction runs:
 //   z : x and W along their columns (K-major);  dx: dz along its columns, W along its rows;  dW: dz and x along their rows.
@@ -16,8 +16,8 @@
 // fetched from tensor memory and added to the tile's sums in registers, rounded to nearest, while the next block runs in
 // the other accumulator.
 //
-// Roles as in gemm_tc_pair.cu: warp 0 TMA, warp 1 of the leader MMA, warps 2-9 epilogue: a warp holds 32 rows x 128 columns
-// of the tile in 128 registers a thread and gives the accumulator back before it works on them.  Tiles are walked in bands
+// Roles as in gemm_tc_pair.cu: warp 0 TMA, warp 1 of the leader MMA, warps 2-9 epilogue: a warp holds 32 rows x 128 (64)
+// columns of the tile in registers and gives the accumulator back before it works on them.  Tiles are walked in bands
 // of eight row blocks, rows fastest, so that the pairs working at a time share both operands through the L2.
 // Bound: tensor pipe for wide layers; the read of W (or the write of dW) where rows are few.
 #include <mutex>
@@ -33,15 +33,16 @@ constexpr int XE_THREADS = 320;
 constexpr int XE_TILE_BYTES = 128 * 128;             // a CTA's share of an operand per ring slot: 128 rows x 64 BF16
 constexpr int XE_STAGE_TILE = 32 * 128;              // epilogue staging: 32 rows x 128 bytes
 constexpr int XE_EPI_WARPS = 8;
-constexpr int XE_WCOLS = 128;                        // columns of an epilogue warp
 constexpr int XE_BAND = 8;
 
 enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
 
 struct alignas(64) XeProblem {
     CUtensorMap tm_a, tm_b, tm_out;
-    long long m, n, tiles, units;     // units: tiles * splits
-    int mpairs, nblocks, splits, kchunks, pairs;
+    long long m, n;
+    unsigned units, tiles;            // work units: tiles * splits
+    unsigned mpairs, nblocks, band;   // row blocks of 256, column blocks, tiles in a band of XE_BAND row blocks
+    int splits, kchunks, part, part_over, pairs;   // a part has `part` ring slots, the first part_over parts one more
     int block;                        // ring slots per block of the contraction (and plane pair)
     unsigned char pa[6], pb[6];       // planes of a and b, one entry per partial product
     int a_mn, b_mn;                   // contracted along the rows of the stored matrix
@@ -67,16 +68,18 @@ struct XeParams {
     XeProblem prob[2];
     int lead;                         // units of the second product that a pair without a last unit of the first takes ahead
     int* zero;
+    XeLoss loss;
     int* status;
 };
 
-template <int EPI, int PLANES>
+template <int EPI, int PLANES, int BN>
 struct XeSmem {
+    static constexpr int B_BYTES = BN / 2 * 128;                          // a CTA's half of the rows of b per ring slot
     static constexpr int STORE_TILES = EPI == XE_STATS ? 0 : PLANES;      // per staging buffer
-    static constexpr int STAGES = PLANES == 3 ? 4 : EPI == XE_STATS ? 6 : 5;
+    static constexpr int STAGES = PLANES == 3 ? 4 : EPI == XE_STATS || BN < 256 ? 6 : 5;
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = STAGES * XE_TILE_BYTES;
-    static constexpr int STORE_OFF = B_OFF + STAGES * XE_TILE_BYTES;
+    static constexpr int STORE_OFF = B_OFF + STAGES * B_BYTES;
     static constexpr int BUF = STORE_TILES * XE_STAGE_TILE;
     static constexpr int NBUF = PLANES == 3 ? 1 : 2;
     static constexpr int BAR_OFF = STORE_OFF + NBUF * XE_EPI_WARPS * BUF;
@@ -102,6 +105,10 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32
                  : "memory");
 }
 
+__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // v[i] of lane l -> lane i returns the sum over lanes of v[i] (halving exchange, 31 shuffles); v is used up
 __device__ __forceinline__ float column_sums(float* v, int lane) {
 #pragma unroll
@@ -121,9 +128,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&o);
 }
 
-template <int EPI, int PLANES>
+template <int EPI, int PLANES, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_gemm_kernel(const __grid_constant__ XeParams pp) {
-    using L = XeSmem<EPI, PLANES>;
+    using L = XeSmem<EPI, PLANES, BN>;
+    constexpr int WCOLS = BN / 2;                     // columns of an epilogue warp
     constexpr int STAGES = L::STAGES;
 
     extern __shared__ uint8_t smem_raw[];
@@ -139,6 +147,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_ctarank();          // 0 = leader (issues the MMAs, owns the "full" and "tempty" barriers)
 
+    if (threadIdx.x == 64) {       // descriptors on their way while the barriers are set up
+        prefetch_tensor_map(&pp.prob[0].tm_a);
+        prefetch_tensor_map(&pp.prob[0].tm_b);
+        if (EPI != XE_STATS && !pp.prob[0].plain) prefetch_tensor_map(&pp.prob[0].tm_out);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(bar_full + 8 * s, 1);
@@ -156,37 +169,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
     cluster_sync_all();            // barriers of both CTAs initialised before any remote arrive or TMA completion
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    pdl_wait();                    // everything before this ran under the predecessor
 
-    const long long pair = blockIdx.x / 2, npairs = gridDim.x / 2;
-    if (pp.zero && blockIdx.x == 0 && threadIdx.x < 2) pp.zero[threadIdx.x] = 0;
+    const unsigned pair = blockIdx.x / 2, npairs = gridDim.x / 2;
 
     // The i-th unit of this pair, -1 after the last.  Units of the first product go round the pairs; the pairs that its last
     // turn leaves out take `lead` units of the second product each in that time, the rest of which goes round all pairs.
-    const long long units0 = pp.prob[0].units, units1 = pp.prob[1].units, over = units0 % npairs;
-    const long long mine0 = units0 / npairs + (pair < over ? 1 : 0), ahead = over && pair >= over ? pp.lead : 0;
-    const long long base1 = over ? (npairs - over) * pp.lead : 0;
-    auto unit_at = [&](long long i) -> long long {
+    const unsigned units0 = pp.prob[0].units, units1 = pp.prob[1].units, over = units0 % npairs;
+    const unsigned mine0 = units0 / npairs + (pair < over ? 1 : 0), ahead = over && pair >= over ? pp.lead : 0;
+    const unsigned base1 = over ? (npairs - over) * pp.lead : 0;
+    auto unit_at = [&](unsigned i) -> long long {
         if (i < mine0) return pair + i * npairs;
         i -= mine0;
-        const long long u = i < ahead ? pair - over + i * (npairs - over) : base1 + pair + (i - ahead) * npairs;
-        return u < units1 ? units0 + u : -1;
+        const unsigned long long u = i < ahead ? pair - over + i * (npairs - over) : (unsigned long long)base1 + pair + (unsigned long long)(i - ahead) * npairs;
+        return u < units1 ? (long long)(units0 + u) : -1;
     };
 
     // work unit -> problem, part of the contraction (ring slots c0 ... c1), tile
     struct Unit { int sp, mp, nb, c0, c1; };
-    auto decode = [&](long long u, Unit& w) -> const XeProblem& {
-        const bool second = u >= pp.prob[0].units;
+    auto decode = [&](long long at, Unit& w) -> const XeProblem& {
+        const bool second = at >= units0;
         const XeProblem& p = pp.prob[second];
-        if (second) u -= pp.prob[0].units;
-        w.sp = (int)(u / p.tiles);
-        const long long t = u % p.tiles, band = (long long)XE_BAND * p.nblocks;
-        const int first = (int)(t / band) * XE_BAND;
-        const int height = p.mpairs - first < XE_BAND ? p.mpairs - first : XE_BAND;
-        w.mp = first + (int)((t % band) % height);
-        w.nb = (int)((t % band) / height);
-        w.c0 = (int)((long long)w.sp * p.kchunks / p.splits);
-        w.c1 = (int)((long long)(w.sp + 1) * p.kchunks / p.splits);
+        const unsigned u = second ? (unsigned)at - units0 : (unsigned)at, sp = u / p.tiles, t = u - sp * p.tiles;
+        const unsigned b = t / p.band, first = b * XE_BAND, left = p.mpairs - first, height = left < XE_BAND ? left : XE_BAND;
+        const unsigned in = t - b * p.band;
+        w.sp = (int)sp;
+        w.nb = (int)(in / height);
+        w.mp = (int)(first + in - w.nb * height);
+        w.c0 = (int)sp * p.part + ((int)sp < p.part_over ? (int)sp : p.part_over);
+        w.c1 = w.c0 + p.part + ((int)sp < p.part_over ? 1 : 0);
         return p;
     };
 
@@ -196,21 +206,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+        long long u;
+            for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
             Unit w;
             const XeProblem& p = decode(u, w);
+            if (i == 0) pdl_wait();        // all of the above ran under the predecessor; now its results are read
             const bool a_mn = p.a_mn, b_mn = p.b_mn;
             const int arow = (w.mp * 2 + (int)rank) * 128;             // this CTA's 128 rows of a
-            const int brow = w.nb * XE_BN + (int)rank * 128;           // this CTA's half of the rows of b
+            const int brow = w.nb * BN + (int)rank * (BN / 2);           // this CTA's half of the rows of b
             for (int cb = w.c0; ok && cb < w.c1; cb += p.block) {
                 const int ce = cb + p.block < w.c1 ? cb + p.block : w.c1;
                 for (int q = 0; ok && q < p.pairs; ++q) {
                     const int pa = p.pa[q], pb = p.pb[q];
                     for (int kc = cb; kc < ce; ++kc) {
                         if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, pp.status, XE_WAIT_EMPTY)) { ok = false; break; }
-                        if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 4 * XE_TILE_BYTES);
+                        if (rank == 0 && issuer) mbar_arrive_expect_tx(bar_full + 8 * stage, 2 * (XE_TILE_BYTES + L::B_BYTES));
                         if (issuer) {
-                            const uint32_t bar = full_leader + 8 * stage, as = a_ring + stage * XE_TILE_BYTES, bs = b_ring + stage * XE_TILE_BYTES;
+                            const uint32_t bar = full_leader + 8 * stage, as = a_ring + stage * XE_TILE_BYTES, bs = b_ring + stage * L::B_BYTES;
                             const int k0 = kc * XE_BK;
                             if (a_mn) {
                                 tma_load_3d_pair(as, &p.tm_a, bar, arow, k0, pa);
@@ -220,7 +232,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                             }
                             if (b_mn) {
                                 tma_load_3d_pair(bs, &p.tm_b, bar, brow, k0, pb);
-                                tma_load_3d_pair(bs + 8192, &p.tm_b, bar, brow + 64, k0, pb);
+                                if (BN == 256) tma_load_3d_pair(bs + 8192, &p.tm_b, bar, brow + 64, k0, pb);
                             } else {
                                 tma_load_3d_pair(bs, &p.tm_b, bar, k0, brow, pb);
                             }
@@ -237,7 +249,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             int stage = 0, as = 0;
             uint32_t phase = 0, aphase = 0;
             bool ok = true;
-            for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+            long long u;
+            for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
                 Unit w;
                 const XeProblem& p = decode(u, w);
                 // 16 contraction elements further on: 32 bytes in a K-major row, 16 rows (2 KiB) in an MN-major tile
@@ -249,11 +262,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                     const int steps = (cb + p.block < w.c1 ? p.block : w.c1 - cb) * p.pairs;
                     if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, pp.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t d_tmem = tmem_base + (uint32_t)(as * XE_BN);
+                    const uint32_t d_tmem = tmem_base + (uint32_t)(as * BN);
                     for (int kc = 0; kc < steps; ++kc) {
                         if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, pp.status, XE_WAIT_FULL)) { ok = false; break; }
                         tc_fence_after();
-                        const uint64_t a_desc = a0 + (uint64_t)(stage * (XE_TILE_BYTES >> 4)), b_desc = b0 + (uint64_t)(stage * (XE_TILE_BYTES >> 4));
+                        const uint64_t a_desc = a0 + (uint64_t)(stage * (XE_TILE_BYTES >> 4)), b_desc = b0 + (uint64_t)(stage * (L::B_BYTES >> 4));
 #pragma unroll
                         for (int ks = 0; ks < XE_BK / 16; ++ks)
                             if (issuer) tc_mma_pair<false>(d_tmem, a_desc + ks * a_step, b_desc + ks * b_step, idesc, (kc | ks) ? 1u : 0u);
@@ -266,15 +279,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                 }
             }
         }
+        if (blockIdx.x == 1 && pp.loss.loss) {        // the partner CTA's MMA warp has no other work
+            pdl_wait();
+            xe_sum_losses<32>(pp.loss);
+        }
     } else {
         const int quarter = warp % 4;                 // tensor-memory lanes [32*quarter, 32*quarter + 32)
-        const int half = (warp - 2) / 4;              // columns [128*half, 128*half + 128)
+        const int half = (warp - 2) / 4;              // columns [WCOLS*half, WCOLS*half + WCOLS)
         uint8_t* stage_gen = gen_base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
         const uint32_t stage_s = base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
         const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
         int as = 0;
         uint32_t aphase = 0, issued = 0;
         bool ok = true;
+        pdl_wait();                                   // before anything is read or stored (the MMA warp does neither)
+        if (pp.zero && blockIdx.x == 0 && warp == 2 && lane < 2) pp.zero[lane] = 0;
         // the staging buffer that is free next (its earlier store has been read out of shared memory)
         auto next_buffer = [&](bool plain = false) -> uint32_t {
             const uint32_t buf = L::NBUF == 1 ? 0 : issued & 1;
@@ -288,24 +307,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             ++issued;
             return buf;
         };
-        for (long long i = 0, u; ok && (u = unit_at(i)) >= 0; ++i) {
+        long long u;
+            for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
             Unit w;
             const XeProblem& p = decode(u, w);
             const long long row0 = (long long)(w.mp * 2 + (int)rank) * 128 + quarter * 32;
-            const long long row = row0 + lane, wcol = (long long)w.nb * XE_BN + half * XE_WCOLS;
+            const long long row = row0 + lane, wcol = (long long)w.nb * BN + half * WCOLS;
 
-            float z[XE_WCOLS];                        // this thread's row of the tile
+            float z[WCOLS];                        // this thread's row of the tile
             for (int cb = w.c0; cb < w.c1; cb += p.block) {
                 if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, pp.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * XE_BN + half * XE_WCOLS);
+                const uint32_t tsrc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * BN + half * WCOLS);
                 if (cb == w.c0) {
 #pragma unroll
-                    for (int j = 0; j < XE_WCOLS / 32; ++j) tmem_ld_32x32(tsrc + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * j]));
+                    for (int j = 0; j < WCOLS / 32; ++j) tmem_ld_32x32(tsrc + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * j]));
                     tmem_ld_wait();
                 } else {
 #pragma unroll
-                    for (int j = 0; j < XE_WCOLS / 16; ++j) {
+                    for (int j = 0; j < WCOLS / 16; ++j) {
                         uint32_t r[16];
                         tmem_ld_32x16(tsrc + j * 16, r);
                         tmem_ld_wait();
@@ -341,11 +361,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             if constexpr (EPI == XE_F32 || EPI == XE_BF16) {
                 const float scale = xe_scale(p.scale);
 #pragma unroll
-                for (int i = 0; i < XE_WCOLS; ++i) z[i] *= scale;
+                for (int i = 0; i < WCOLS; ++i) z[i] *= scale;
             }
-            if constexpr (EPI == XE_F32) {
+            // the warp's columns as floats, 32 at a time
+            auto store_floats = [&]() {
 #pragma unroll
-                for (int chunk = 0; chunk < XE_WCOLS / 32; ++chunk) {
+                for (int chunk = 0; chunk < WCOLS / 32; ++chunk) {
                     const long long col0 = wcol + chunk * 32;
                     if (col0 < p.n) {
                         const uint32_t buf = next_buffer(p.plain);
@@ -361,8 +382,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                             if (col0 + lane < p.n) {
                                 const float* src = reinterpret_cast<const float*>(stage_gen + buf * L::BUF) + (lane & 3);
                                 for (int r = 0; r < rows; ++r) {
-                                    const float v = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
-                                    o[r * p.out_pitch] = p.add ? o[r * p.out_pitch] + v : v;
+                                    const float x = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
+                                    o[r * p.out_pitch] = p.add ? o[r * p.out_pitch] + x : x;
                                 }
                             }
                             __syncwarp();
@@ -377,9 +398,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                         }
                     }
                 }
+            };
+            if constexpr (EPI == XE_F32) {
+                store_floats();
             } else if constexpr (EPI == XE_BF16) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < WCOLS / 64; ++h) {
                     if (wcol + h * 64 < p.n) {
                         const uint32_t buf = next_buffer(p.plain);
                         uint32_t pk[32];
@@ -403,12 +427,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                     }
                 }
             } else {
-                const bool live = row < p.m, whole = wcol + XE_WCOLS <= p.n;
+                const bool live = row < p.m, whole = wcol + WCOLS <= p.n;
                 if (p.bias) {
                     if (whole) {
                         const float4* b4 = reinterpret_cast<const float4*>(p.bias + wcol);
 #pragma unroll
-                        for (int j = 0; j < XE_WCOLS / 4; ++j) {
+                        for (int j = 0; j < WCOLS / 4; ++j) {
                             const float4 b = __ldg(b4 + j);
                             z[4 * j] += b.x;
                             z[4 * j + 1] += b.y;
@@ -417,7 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < XE_WCOLS; ++i)
+                        for (int i = 0; i < WCOLS; ++i)
                             if (wcol + i < p.n) z[i] += __ldg(p.bias + wcol + i);
                     }
                 }
@@ -425,34 +449,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                 int tc = -1;
                 if (live) {
                     const long long t = p.target[row] - p.col_base - wcol;
-                    if (t >= 0 && t < XE_WCOLS) tc = (int)t;
+                    if (t >= 0 && t < WCOLS) tc = (int)t;
                 }
                 const bool here = __any_sync(0xffffffffu, tc >= 0);
-                if constexpr (EPI == XE_STATS || EPI == XE_STATS_E) {
+                if constexpr (EPI == XE_STATS || EPI == XE_STATS_E || EPI == XE_STATS_Z) {
+                    if constexpr (EPI == XE_STATS_Z) store_floats();
                     if (here) {
                         float t = 0.f;
 #pragma unroll
-                        for (int i = 0; i < XE_WCOLS; ++i) t = i == tc ? z[i] : t;
+                        for (int i = 0; i < WCOLS; ++i) t = i == tc ? z[i] : t;
                         if (tc >= 0) p.zt[row] = t;
                     }
                     if (p.zsum) {
                         float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int i = 0; i < XE_WCOLS; ++i) t[i & 3] += whole || wcol + i < p.n ? z[i] : 0.f;
+                        for (int i = 0; i < WCOLS; ++i) t[i & 3] += whole || wcol + i < p.n ? z[i] : 0.f;
                         if (live) p.zsum[wcol / XE_STAT_COLS * p.m + row] = (t[0] + t[1]) + (t[2] + t[3]);
                     }
                     if (!whole) {
 #pragma unroll
-                        for (int i = 0; i < XE_WCOLS; ++i) z[i] = wcol + i < p.n ? z[i] : -INFINITY;
+                        for (int i = 0; i < WCOLS; ++i) z[i] = wcol + i < p.n ? z[i] : -INFINITY;
                     }
                     float cm[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-                    for (int i = 4; i < XE_WCOLS; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
+                    for (int i = 4; i < WCOLS; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
                     const float mx = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3]));
                     const float ref = mx == -INFINITY ? 0.f : mx;      // nothing but -inf: every term is 0
                     float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < XE_WCOLS; ++i) {
+                    for (int i = 0; i < WCOLS; ++i) {
                         z[i] = xe_ex2((z[i] - ref) * XE_LOG2E);
                         t[i & 3] += z[i];
                     }
@@ -476,11 +501,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                     const float gp = g * p.rule.pf, ga = g * p.rule.smooth_all;
                     // a row that does not count: exactly 0, whatever its logits
 #pragma unroll
-                    for (int i = 0; i < XE_WCOLS; ++i) z[i] = g == 0.f ? 0.f : gp * xe_ex2((z[i] - lse) * XE_LOG2E) - ga;
+                    for (int i = 0; i < WCOLS; ++i) z[i] = g == 0.f ? 0.f : gp * xe_ex2((z[i] - lse) * XE_LOG2E) - ga;
                     if (here) {
                         const float gt = g * p.rule.smooth_t;
 #pragma unroll
-                        for (int i = 0; i < XE_WCOLS; ++i) z[i] = i == tc ? z[i] - gt : z[i];
+                        for (int i = 0; i < WCOLS; ++i) z[i] = i == tc ? z[i] - gt : z[i];
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -542,31 +567,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
     }
 }
 
-template <int EPI, int PLANES>
+template <int EPI, int PLANES, int BN = XE_BN>
 int run(const XeParams& p, cudaStream_t st) {
-    using L = XeSmem<EPI, PLANES>;
+    using L = XeSmem<EPI, PLANES, BN>;
     static_assert(L::TOTAL <= 232448, "shared memory budget of one CTA exceeded");
     static std::once_flag once[64];
     int dev = 0;
     WINO_CUDA_CHECK(cudaGetDevice(&dev));
     cudaError_t attr_err = cudaSuccess;
     std::call_once(once[dev & 63], [&] {
-        attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
+        attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     });
     WINO_CUDA_CHECK(attr_err);
-    const long long total = p.prob[0].units + p.prob[1].units;
+    const long long total = (long long)p.prob[0].units + p.prob[1].units;
     const long long pairs = total < sm_count() / 2 ? total : sm_count() / 2;
     count_launch();
-    WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES>, dim3((unsigned)(2 * pairs)), dim3(XE_THREADS), L::TOTAL, st, true, p));
+    WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES, BN>, dim3((unsigned)(2 * pairs)), dim3(XE_THREADS), L::TOTAL, st, true, p));
     return WINO_OK;
 }
 
-// boxes of 64 columns (128 bytes, 128-byte swizzle): 128 rows for a K-major share, 64 rows (one contraction element each)
+// boxes of 64 columns (128 bytes, 128-byte swizzle): `share` rows for a K-major share, 64 rows (one contraction element each)
 // for an MN-major one
-int operand_map(CUtensorMap* map, const XeOperand& o) {
+int operand_map(CUtensorMap* map, const XeOperand& o, unsigned share) {
     const unsigned long long dims[3] = {(unsigned long long)o.cols, (unsigned long long)o.rows, (unsigned long long)o.planes};
     const unsigned long long strides[2] = {(unsigned long long)o.pitch * 2, (unsigned long long)o.plane_pitch * 2};
-    const unsigned box[3] = {64u, o.along_rows ? 64u : 128u, 1u};
+    const unsigned box[3] = {64u, o.along_rows ? 64u : share, 1u};
     return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1);
 }
 
@@ -574,8 +599,8 @@ int make_problem(const XeProduct& x, XeProblem* out) {
     XeProblem& p = *out;
     const XeOutput& o = x.out;
     int rc;
-    if ((rc = operand_map(&p.tm_a, x.a)) || (rc = operand_map(&p.tm_b, x.b))) return rc;
-    const bool f32 = x.epi == XE_F32;
+    if ((rc = operand_map(&p.tm_a, x.a, 128)) || (rc = operand_map(&p.tm_b, x.b, (unsigned)x.bn / 2))) return rc;
+    const bool f32 = x.epi == XE_F32 || x.epi == XE_STATS_Z;
     const int es = f32 ? 4 : 2;
     p.plain = x.epi != XE_STATS && (o.pitch * es) % 16 != 0;
     if (p.plain && (o.splits > 1 || x.epi > XE_BF16)) return fail(WINO_E_BADARG, "xent: buffer rows must be multiples of 16 bytes");
@@ -590,12 +615,17 @@ int make_problem(const XeProduct& x, XeProblem* out) {
             return rc;
     }
     p.m = x.m; p.n = x.n;
-    p.mpairs = (int)((x.m + XE_BM - 1) / XE_BM);
-    p.nblocks = (int)((x.n + XE_BN - 1) / XE_BN);
+    p.mpairs = (unsigned)((x.m + XE_BM - 1) / XE_BM);
+    p.nblocks = (unsigned)((x.n + x.bn - 1) / x.bn);
     p.kchunks = (int)((x.k + XE_BK - 1) / XE_BK);
     p.splits = o.splits;
-    p.tiles = (long long)p.mpairs * p.nblocks;
+    p.part = p.kchunks / p.splits;
+    p.part_over = p.kchunks % p.splits;
+    const unsigned long long tiles = (unsigned long long)p.mpairs * p.nblocks;
+    if (tiles * p.splits > 0x3fffffffull) return fail(WINO_E_UNSUPPORTED, "xent: more than 2^30 tiles");
+    p.tiles = (unsigned)tiles;
     p.units = p.tiles * p.splits;
+    p.band = XE_BAND * p.nblocks;
     p.block = x.a.planes == 3 ? 4 : 16;
     if (x.a.planes == 3) {
         static const unsigned char pa[6] = {2, 1, 0, 1, 0, 0}, pb[6] = {0, 1, 2, 0, 1, 0};
@@ -607,7 +637,7 @@ int make_problem(const XeProduct& x, XeProblem* out) {
     }
     p.a_mn = x.a.along_rows;
     p.b_mn = x.b.along_rows;
-    p.idesc = make_idesc(OP_BF16, XE_BN, XE_BM) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
+    p.idesc = make_idesc(OP_BF16, x.bn, XE_BM) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
     p.add = o.add;
     p.out_ptr = o.ptr; p.out_pitch = o.pitch;
     p.scale = o.scale;
@@ -625,6 +655,7 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
     XeParams p;
     int rc;
     p.zero = prod[0].out.zero;
+    p.loss = prod[0].out.loss;
     for (int i = 0; i < count; ++i)
         if ((rc = make_problem(prod[i], &p.prob[i]))) return rc;
     p.lead = 0;
@@ -634,7 +665,7 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
         // ring slots of a unit, and about six more for its epilogue; the product with the longer units goes first
         auto cost = [](const XeProblem& q) { return (double)q.kchunks / q.splits * q.pairs + 6.0; };
         if (cost(p.prob[0]) < cost(p.prob[1])) { const XeProblem t = p.prob[0]; p.prob[0] = p.prob[1]; p.prob[1] = t; }
-        const long long pairs = sm_count() / 2, over = p.prob[0].units % pairs;
+        const long long pairs = sm_count() / 2, over = (long long)p.prob[0].units % pairs;
         if (over) {
             const long long lead = (long long)(cost(p.prob[0]) / cost(p.prob[1]) + 0.5), most = p.prob[1].units / (pairs - over);
             p.lead = (int)(lead < most ? lead : most);
@@ -642,9 +673,10 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
     }
     if ((rc = status_word(&p.status))) return rc;
     switch (prod[0].epi) {
-        case XE_F32: return run<XE_F32, 1>(p, st);
-        case XE_BF16: return run<XE_BF16, 1>(p, st);
+        case XE_F32: return prod[0].bn == 128 ? run<XE_F32, 1, 128>(p, st) : run<XE_F32, 1>(p, st);
+        case XE_BF16: return prod[0].bn == 128 ? run<XE_BF16, 1, 128>(p, st) : run<XE_BF16, 1>(p, st);
         case XE_STATS: return run<XE_STATS, 1>(p, st);
+        case XE_STATS_Z: return run<XE_STATS_Z, 1>(p, st);
         case XE_STATS_E: return run<XE_STATS_E, 1>(p, st);
         case XE_DZ: return prod[0].a.planes == 3 ? run<XE_DZ, 3>(p, st) : run<XE_DZ, 1>(p, st);
     }

@@ -110,16 +110,21 @@ class LinearXent:
             self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
         self._desc_ref, self._ws_size = ctypes.byref(s), self.workspace.numel() * self.workspace.element_size()
         self._index = self.workspace.get_device()
+        self._forms = [(torch.Size((rows, d)), (ld or d, 1)) for rows, ld in ((n, ldx), (v, ldw), (n, lddx), (v, lddw))]
         self._like = torch.empty(0, dtype=torch.float32, device=self.workspace.device)
 
-    def _matrix(self, t, what, rows, ld):
-        d = self.desc.d
+    def _matrix(self, t, what, form):
+        """Device address of a matrix of the plan's rows and pitch; form: (shape, strides)."""
+        if t.shape == form[0] and t.stride() == form[1] and t.dtype == self.io_dtype and t.get_device() == self._index:
+            return t.data_ptr()
+        (rows, d), (ld, _) = form
         if t.get_device() != self._index:
             raise ValueError("%s must be on the plan's device" % what)
         if t.dtype != self.io_dtype:
             raise ValueError("%s dtype %s, expected %s" % (what, t.dtype, self.io_dtype))
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != d or (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) != (ld or d)):
-            raise ValueError("%s must be (%d, %d) with rows %d elements apart" % (what, rows, d, ld or d))
+        # the pitch of a single row and the step of a single column mean nothing
+        if tuple(t.shape) != (rows, d) or (d > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) != ld):
+            raise ValueError("%s must be (%d, %d) with rows %d elements apart" % (what, rows, d, ld))
         return t.data_ptr()
 
     def _vector(self, t, what, count, dtype):
@@ -133,7 +138,7 @@ class LinearXent:
             raise ValueError("libwino needs CUDA tensors")
         if bool(s.has_bias) != (bias is not None):
             raise ValueError("the plan was made with bias=%s" % bool(s.has_bias))
-        return (self._matrix(x, "x", s.n, s.ldx), self._matrix(w, "w", s.v, s.ldw),
+        return (self._matrix(x, "x", self._forms[0]), self._matrix(w, "w", self._forms[1]),
                 None if bias is None else self._vector(bias, "bias", s.v, torch.float32), self._vector(target, "target", s.n, torch.int64))
 
     def _losses(self):
@@ -160,15 +165,19 @@ class LinearXent:
         if dloss is not None:
             dloss = self._vector(dloss, "dloss", s.n if s.reduction == _lib.NONE else 1, torch.float32)
 
-        def result(t, need, what, like, rows, ld):
+        def result(t, need, what, like, form):
             if not need:
                 return None, None
-            if t is None:                   # the input's own shape where both are dense
-                t = torch.empty_like(like) if not ld and like.is_contiguous() else like.new_empty((rows, ld or s.d))[:, :s.d]
-            return t, self._matrix(t, what, rows, ld)
+            if t is not None:
+                return t, self._matrix(t, what, form)
+            if form[1][0] == s.d and like.stride() == form[1]:       # both dense
+                t = torch.empty_like(like)
+            else:
+                t = like.new_empty((form[0][0], form[1][0]))[:, :s.d]
+            return t, t.data_ptr()
 
-        dx, dx_ptr = result(dx, need_dx, "dx", x, s.n, s.lddx)
-        dw, dw_ptr = result(dw, need_dw, "dw", w, s.v, s.lddw)
+        dx, dx_ptr = result(dx, need_dx, "dx", x, self._forms[2])
+        dw, dw_ptr = result(dw, need_dw, "dw", w, self._forms[3])
         db = torch.empty_like(bias) if s.has_bias else None
         loss = self._losses()
         _call(lib().wino_xent_grad, self._index, self._desc_ref, *args, dloss, loss.data_ptr(), None, dx_ptr, dw_ptr,

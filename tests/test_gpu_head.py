@@ -123,6 +123,15 @@ CASES = [
     (2304, 300, 2050, "fp32", {}),
     (2304, 1024, 2050, "bf16", dict(bias=False)),                 # logits kept as exponentials
     (2500, 24, 2303, "bf16", dict(bias=False)),
+    (600, 1100, 9001, "bf16", {}),                                # rows too wide for one kernel: statistics with the product
+    (1100, 300, 9000, "fp32", {}),
+    (20, 4096, 9001, "bf16", {}),                                 # the same with a split contraction
+    (20, 1025, 9002, "fp32", {}),
+    (100, 3000, 8000, "bf16", {}),                                # the widest row of the one-kernel path, and narrower ones
+    (100, 900, 4000, "fp32", {}),
+    (700, 1500, 1900, "bf16", {}),
+    (1000, 40, 100, "fp32", {}),                                  # plain FP32 kernels up to their most rows and classes
+    (3, 1001, 1024, "bf16", {}),
     (300, 2200, 700, "bf16", dict(bias=False)),                   # blocks of the contraction: 1024 + 1024 + 152
     (2100, 700, 2400, "fp32", {}),                                # 256 + 256 + 188, logits recomputed below
     (4000, 64, 5, "bf16", {}),                                    # long contraction of dW over rows, few classes
@@ -293,10 +302,22 @@ def test_outputs_stay_inside_their_rows(dtype, n, d, v, pad):
     c.check(got, ref, "mean", np.full(n, 1.0 / n))
     for b, rows in ((bx, n), (bw, v)):
         assert (b[rows:] == 5).all() and (b[:rows, d:] == 5).all()
+    fresh = plan.loss_and_grad(c.x, c.w, c.target, c.bias)                       # allocated by the call
+    assert all(torch.equal(a, b) for a, b in zip(fresh, got)) and fresh[1].shape == c.x.shape and (n < 2 or fresh[1].stride(0) == d + pad)
     only = plan.loss_and_grad(c.x, c.w, c.target, c.bias, need_dx=False)
     assert only[1] is None and torch.equal(only[2], got[2]) and torch.equal(only[3], got[3])
     only = plan.loss_and_grad(c.x, c.w, c.target, c.bias, need_dw=False)
     assert only[2] is None and torch.equal(only[1], got[1])
+
+
+def test_results_have_the_pitch_of_the_plan():
+    """Inputs and results of the same wide pitch: what the call allocates is laid out by the plan, not like the input."""
+    torch = _torch()
+    import cudnntest_b200 as cb
+    c = Case(50, 40, 60, "bf16", seed=5, ldx=64, ldw=64)
+    got = c.plan(lddx=64, lddw=64, reduction="mean").loss_and_grad(c.x, c.w, c.target, c.bias)
+    assert got[1].stride() == (64, 1) and got[2].stride() == (64, 1)
+    c.check(got, c.oracle("mean"), "mean", np.full(50, 1.0 / 50))
 
 
 def test_python_checks():
