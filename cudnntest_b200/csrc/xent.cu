@@ -15,6 +15,7 @@
 // rows FP64.
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "xent.cuh"
 
@@ -39,6 +40,44 @@ struct PackJob {
     __nv_bfloat16* dst;
     const long long* target;            // rows that do not count become zero where target is given
 };
+// four neighbouring elements, `left` of which exist, by the widest loads that the address allows
+template <typename T> using Wide = std::conditional_t<sizeof(T) == 4, float4, uint2>;
+template <typename T> using Pair = std::conditional_t<sizeof(T) == 4, float2, uint32_t>;
+template <typename T>
+__device__ __forceinline__ void load4(T (&v)[4], const T* p, int left) {
+    const unsigned at = (unsigned)(uintptr_t)p;
+    if (left < 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = e < left ? p[e] : from_float<T>(0.f);
+    } else if (at % (4 * sizeof(T)) == 0) {
+        const Wide<T> q = *reinterpret_cast<const Wide<T>*>(p);
+        memcpy(v, &q, sizeof(q));
+    } else if (at % (2 * sizeof(T)) == 0) {
+        const Pair<T> q[2] = {reinterpret_cast<const Pair<T>*>(p)[0], reinterpret_cast<const Pair<T>*>(p)[1]};
+        memcpy(v, q, sizeof(q));
+    } else {
+        v[0] = p[0];
+        const Pair<T> q = *reinterpret_cast<const Pair<T>*>(p + 1);
+        memcpy(v + 1, &q, sizeof(q));
+        v[3] = p[3];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void load4_aligned(float (&v)[4], const T* p) {
+    const Wide<T> q = *reinterpret_cast<const Wide<T>*>(p);
+    T t[4];
+    memcpy(t, &q, sizeof(q));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_float<T>(t[e]);
+}
+template <typename T>
+__device__ __forceinline__ void load4f(float (&v)[4], const T* p, int left) {
+    T t[4];
+    load4(t, p, left);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = to_float<T>(t[e]);
+}
+
 // src (rows x cols, pitch ld) -> PLANES x rows x pitch BF16, four columns per thread, for up to two matrices
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) xe_pack_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
@@ -55,13 +94,8 @@ __global__ void __launch_bounds__(256) xe_pack_kernel(const PackJob j0, const Pa
         const bool live = !j.target || row_counts(rule, j.target[r]);
         const T* src = static_cast<const T*>(j.src) + r * j.ld + c;
         T v[4];
-        if (live && sizeof(T) == 4 && c + 4 <= cols && ((uintptr_t)src & 15) == 0) {
-            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = live && c + e < cols ? src[e] : from_float<T>(0.f);
-        }
-        __nv_bfloat16 part[PLANES][4];
+        load4(v, src, live ? cols - c : 0);
+        alignas(8) __nv_bfloat16 part[PLANES][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (PLANES == 3) xe_split3(to_float<T>(v[e]), part[0][e], part[1][e], part[2][e]);
@@ -107,12 +141,16 @@ __device__ __forceinline__ bool finish_row(const RowArgs& a, long long row, floa
     return counts;
 }
 
-// The block that finishes last sums the rows' losses (in the same order whichever block that is).  All threads call it; the
-// block's losses were written by warp 0, so only that warp waits for its stores.
-template <int THREADS>
+// The block that finishes last sums the rows' losses (in the same order whichever block that is).  All threads call it; where
+// warp 0 has written the block's losses, only that warp waits for its stores, else all do (EVERY_WARP).
+template <int THREADS, bool EVERY_WARP = false>
 __device__ __forceinline__ void finish_loss(const RowArgs& a) {
     if (!a.loss.loss) return;
     __shared__ int last;
+    if (EVERY_WARP) {
+        __threadfence();
+        __syncthreads();
+    }
     if (threadIdx.x < 32) {
         __threadfence();
         __syncwarp();
@@ -245,11 +283,25 @@ __device__ __forceinline__ void gather_groups(float (&e)[COUNT][4], const float*
     }
 }
 
+// four columns of dz: floats (PLANES 0) or BF16 planes; d is used up
+template <int PLANES>
+__device__ __forceinline__ void store_dz(float (&d)[4], void* dz, long long n, long long row, int pitch, int c) {
+    if constexpr (PLANES == 0) *reinterpret_cast<float4*>(static_cast<float*>(dz) + row * pitch + c) = make_float4(d[0], d[1], d[2], d[3]);
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(d[0], d[1]), hi = __floats2bfloat162_rn(d[2], d[3]);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(dz) + (p * n + row) * pitch + c) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        d[0] -= __low2float(lo); d[1] -= __high2float(lo);
+        d[2] -= __low2float(hi); d[3] -= __high2float(hi);
+    }
+}
+
 // Kept logits -> lse, loss and dz (PLANES BF16 planes; 0: floats, which may replace the first part of the logits) in one go.  A block takes a run of rows; a thread holds the same 4 * QUADS columns of each
 // in registers, from the sum of the parts to dz, and their column sums over the run.  v <= 4 * THREADS * QUADS.
-// 1024 threads an SM (64 registers), half of that where the parts of several groups of columns are in flight.
+// 1024 threads an SM (64 registers), fewer where the parts of the columns have to be in flight.
 template <int THREADS, int QUADS, int PLANES, bool GRAD, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, (SPLIT && QUADS > 1 ? 512 : 1024) / THREADS) xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
+__global__ void __launch_bounds__(THREADS, (!SPLIT ? 1024 : QUADS > 1 ? 512 : 768) / THREADS) xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
                                                           const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
     pdl_launch_dependents();
     pdl_wait();
@@ -319,15 +371,7 @@ __global__ void __launch_bounds__(THREADS, (SPLIT && QUADS > 1 ? 512 : 1024) / T
                         d[k] = g == 0.f || c + k >= v ? 0.f : d[k] * g;      // a row that does not count: exactly 0, whatever its logits
                         sums[q][k] += d[k];
                     }
-                    if constexpr (PLANES == 0) *reinterpret_cast<float4*>(static_cast<float*>(dz) + row * dpitch + c) = make_float4(d[0], d[1], d[2], d[3]);
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p) {
-                        const __nv_bfloat162 lo = __floats2bfloat162_rn(d[0], d[1]), hi = __floats2bfloat162_rn(d[2], d[3]);
-                        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(dz) + (p * a.n + row) * dpitch + c) =
-                            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-                        d[0] -= __low2float(lo); d[1] -= __high2float(lo);
-                        d[2] -= __low2float(hi); d[3] -= __high2float(hi);
-                    }
+                    store_dz<PLANES>(d, dz, a.n, row, dpitch, c);
                 }
             }
         }
@@ -345,43 +389,118 @@ __global__ void __launch_bounds__(THREADS, (SPLIT && QUADS > 1 ? 512 : 1024) / T
     finish_loss<THREADS>(a);
 }
 
-// The same for any v, in two kernels.  Statistics of split logits, one block per row (the sum of the parts replaces the
-// first); of unsplit ones they come with the product (XE_STATS_Z).
-__global__ void __launch_bounds__(256) xe_wide_rows_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, const RowArgs a) {
+// The same with a warp per row and no barriers, for v <= 512: lanes hold up to four groups of four columns.  A warp walks its
+// run of rows; the block's warps add up their column sums at the end.
+constexpr int XE_WARP_ROWS = 8;                    // warps per block
+template <int PLANES, bool GRAD, bool SPLIT>
+__global__ void __launch_bounds__(256) xe_warp_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
+                                                           const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int QUADS = 4;
+    __shared__ __align__(16) float block_sums[XE_WARP_ROWS][128 * QUADS];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const long long warps = (long long)gridDim.x * XE_WARP_ROWS, w0 = (long long)blockIdx.x * XE_WARP_ROWS + warp;
+    const long long r0 = w0 * a.n / warps, r1 = (w0 + 1) * a.n / warps, plane = a.n * zpitch;
+    float sums[QUADS][4];
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[q][k] = 0.f;
+    int live = 0;
+    for (long long row = r0; row < r1; ++row) {
+        const bool counts = row_counts(a.rule, a.target[row]);
+        const int t = counts ? (int)a.target[row] : -1;
+        float e[QUADS][4], m = -INFINITY, zsum = 0.f, zt = 0.f;
+        gather_groups<SPLIT>(e, z + row * zpitch, plane, splits, lane * 4, 128, v, bias);
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = q * 128 + lane * 4 + k;
+                m = fmaxf(m, e[q][k]);
+                if (c < v) zsum += e[q][k];
+                if (c == t) zt = e[q][k];
+            }
+#pragma unroll
+        for (int w = 16; w >= 1; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        const float ref = m == -INFINITY ? 0.f : m;
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += xe_ex2((e[q][k] - ref) * XE_LOG2E);
+#pragma unroll
+        for (int w = 16; w >= 1; w >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, w);
+            zsum += __shfl_xor_sync(0xffffffffu, zsum, w);
+        }
+        if (counts) zt = __shfl_sync(0xffffffffu, zt, t % 128 / 4);
+        const float lse = m + logf(s);
+        if (lane == 0) live += finish_row(a, row, lse, zsum, zt);
+        if constexpr (GRAD) {
+            const float g = counts ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
+#pragma unroll
+            for (int q = 0; q < QUADS; ++q) {
+                const int c = q * 128 + lane * 4;
+                if (c < v) {
+                    float d[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        d[k] = xe_ex2((e[q][k] - lse) * XE_LOG2E) * rule.pf - rule.smooth_all;
+                        if (c + k == t) d[k] -= rule.smooth_t;
+                        d[k] = g == 0.f || c + k >= v ? 0.f : d[k] * g;      // a row that does not count: exactly 0, whatever its logits
+                        sums[q][k] += d[k];
+                    }
+                    store_dz<PLANES>(d, dz, a.n, row, dpitch, c);
+                }
+            }
+        }
+    }
+    if (lane == 0 && live) atomicAdd(a.count, live);
+    if constexpr (GRAD && PLANES > 0) {
+        if (db_part) {
+#pragma unroll
+            for (int q = 0; q < QUADS; ++q)
+                *reinterpret_cast<float4*>(&block_sums[warp][q * 128 + lane * 4]) = make_float4(sums[q][0], sums[q][1], sums[q][2], sums[q][3]);
+            __syncthreads();
+            for (int c = threadIdx.x; c < v; c += 256) {
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < XE_WARP_ROWS; ++w) s += block_sums[w][c];
+                db_part[(long long)blockIdx.x * dpitch + c] = s;
+            }
+        }
+    }
+    finish_loss<256, true>(a);
+}
+
+// The same for any v, in three kernels.  Statistics of split logits, 1024 columns of a row per block (the sum of the parts with
+// the bias replaces the first); of unsplit ones they come with the product (XE_STATS_Z).
+constexpr int XE_CHUNK = 1024;
+__global__ void __launch_bounds__(256) xe_wide_stats_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, long long n,
+                                                            const long long* __restrict__ target, float2* __restrict__ stats, float* __restrict__ zsums,
+                                                            float* __restrict__ zt) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float red[3][8];
-    __shared__ float zt_s;
-    const long long row = blockIdx.x;
-    const bool counts = row_counts(a.rule, a.target[row]);
-    const int t = counts ? (int)a.target[row] : -1;
+    const int chunks = (v + XE_CHUNK - 1) / XE_CHUNK, chunk = (int)(blockIdx.x % (unsigned)chunks);
+    const long long row = blockIdx.x / (unsigned)chunks;
+    const int c = chunk * XE_CHUNK + threadIdx.x * 4;
+    const long long t = target[row];
     float* zr = z + row * pitch;
-    float m = -INFINITY, s = 0.f, zsum = 0.f;
-    if (threadIdx.x == 0) zt_s = 0.f;
-    __syncthreads();
-    // four groups of four columns at a time, so that their loads overlap and the running maximum moves once
-    for (int c0 = threadIdx.x * 4; c0 < v; c0 += 4096) {
-        float e[4][4], m2 = m;
-        gather_groups<true>(e, zr, a.n * pitch, splits, c0, 1024, v, bias);
+    float e[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, zsum = 0.f;
+    if (c < v) {
+        gather_logits(e, zr, n * pitch, splits, c, v, bias);
+        *reinterpret_cast<float4*>(zr + c) = make_float4(e[0], e[1], e[2], e[3]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = c0 + q * 1024;
-            if (c < v) *reinterpret_cast<float4*>(zr + c) = make_float4(e[q][0], e[q][1], e[q][2], e[q][3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (c + i < v) zsum += e[q][i];
-                if (c + i == t) zt_s = e[q][i];
-                m2 = fmaxf(m2, e[q][i]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            if (c + i < v) zsum += e[i];
+            if (c + i == t) zt[row] = e[i];
         }
-        const float ref = m2 == -INFINITY ? 0.f : m2;
-        s *= xe_ex2((m - ref) * XE_LOG2E);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s += xe_ex2((e[q][i] - ref) * XE_LOG2E);
-        m = m2;
     }
+    float m = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), ref = m == -INFINITY ? 0.f : m;
+    float s = (xe_ex2((e[0] - ref) * XE_LOG2E) + xe_ex2((e[1] - ref) * XE_LOG2E)) + (xe_ex2((e[2] - ref) * XE_LOG2E) + xe_ex2((e[3] - ref) * XE_LOG2E));
 #pragma unroll
     for (int w = 16; w >= 1; w >>= 1) {
         const float m2 = __shfl_xor_sync(0xffffffffu, m, w), s2 = __shfl_xor_sync(0xffffffffu, s, w);
@@ -399,16 +518,17 @@ __global__ void __launch_bounds__(256) xe_wide_rows_kernel(float* __restrict__ z
             join(m, s, red[0][i], red[1][i]);
             zsum += red[2][i];
         }
-        if (finish_row(a, row, m + logf(s), zsum, zt_s)) atomicAdd(a.count, 1);
+        stats[chunk * n + row] = make_float2(m, s);
+        if (zsums) zsums[chunk * n + row] = zsum;
     }
-    finish_loss<256>(a);
 }
 
-// dz, two classes per thread, 32 rows per block, with the block's column sums (z has the bias already)
+// dz (PLANES 0: floats, which may replace z), two classes per thread, 32 rows per block, with the block's column sums; z has
+// the bias already
 template <int PLANES>
-__global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict__ z, int v, int zpitch, long long n, const float* __restrict__ lse,
+__global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* z, int v, int zpitch, long long n, const float* __restrict__ lse,
                                                          const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
-                                                         __nv_bfloat16* __restrict__ dz, int dpitch, float* __restrict__ db_part) {
+                                                         void* dz, int dpitch, float* __restrict__ db_part) {
     pdl_launch_dependents();
     pdl_wait();
     const unsigned cblocks = (unsigned)(v + 255) / 256, part = blockIdx.x / cblocks;
@@ -429,10 +549,11 @@ __global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* __restrict
         b = g == 0.f || c + 1 >= v ? 0.f : b * g;
         s0 += a;
         s1 += b;
+        if constexpr (PLANES == 0) *reinterpret_cast<float2*>(static_cast<float*>(dz) + r * dpitch + c) = make_float2(a, b);
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
             const __nv_bfloat162 o = __floats2bfloat162_rn(a, b);
-            *reinterpret_cast<__nv_bfloat162*>(dz + (p * n + r) * dpitch + c) = o;
+            *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(dz) + (p * n + r) * dpitch + c) = o;
             a -= __low2float(o);
             b -= __high2float(o);
         }
@@ -491,21 +612,24 @@ __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __re
     }
 }
 
-// dbias from the column sums of runs of rows, 32 columns per block
+// dbias from the column sums of runs of rows (or from the rows of a float dz): COLS columns and 512 / COLS runs at a time
+// per block; eight columns where there are few of them, 32 (whole lines) where there are many
+template <int COLS>
 __global__ void __launch_bounds__(512) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, const XeScale scale, float* __restrict__ db) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ float red[16][32];
-    const int l = threadIdx.x % 32, g = threadIdx.x / 32, c = blockIdx.x * 32 + l;
+    constexpr int RUNS = 512 / COLS;
+    __shared__ float red[RUNS][COLS];
+    const int l = threadIdx.x % COLS, g = threadIdx.x / COLS, c = blockIdx.x * COLS + l;
     float s = 0.f;
     if (c < cols) {
 #pragma unroll 8
-        for (int i = g; i < parts; i += 16) s += part[(long long)i * pitch + c];
+        for (int i = g; i < parts; i += RUNS) s += part[(long long)i * pitch + c];
     }
     red[g][l] = s;
     __syncthreads();
     if (g == 0 && c < cols) {
-        for (int i = 1; i < 16; ++i) s += red[i][l];
+        for (int i = 1; i < RUNS; ++i) s += red[i][l];
         db[c] = s * xe_scale(scale);
     }
 }
@@ -522,8 +646,9 @@ __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict_
         const long long r = i / quads;
         const int c = (int)(i - r * quads) * 4;
         float4 q = *reinterpret_cast<const float4*>(part + r * pitch + c);
+#pragma unroll 8
         for (int s = 1; s < splits; ++s) {
-            const float4 o = *reinterpret_cast<const float4*>(part + s * plane + r * pitch + c);
+            const float4 o = __ldg(reinterpret_cast<const float4*>(part + s * plane + r * pitch + c));
             q.x += o.x; q.y += o.y; q.z += o.z; q.w += o.w;
         }
         const float e[4] = {q.x, q.y, q.z, q.w};
@@ -539,23 +664,6 @@ __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict_
 // tensor cores, of 512 x 256 x 256 (32M) 20.6 / 26.7 against 14.4 / 16.5; gradient of 32 x 4096 x 64 (8M) 18.5 / 20.6 against
 // 22.7 / 28.8.  The gradient's sums run one after the other over rows or classes: with 256 of them 23.8 / 24.8 against
 // 18.5 / 24.7, with 1000 of them 65 against 29.
-template <typename T>
-__device__ __forceinline__ void load4(float (&v)[4], const T* p, int left, bool aligned) {
-    if (aligned && left >= 4) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 q = *reinterpret_cast<const float4*>(p);
-            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-        } else {
-            const uint2 q = *reinterpret_cast<const uint2*>(p);
-            v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xffff0000u);
-            v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = e < left ? to_float<T>(p[e]) : 0.f;
-    }
-}
-
 // logits: a warp multiplies one class with eight rows, lanes along the features; blockIdx.z: part of the features
 constexpr int XE_SMALL_ROWS = 8, XE_SMALL_SLICE = 2048;
 template <typename T>
@@ -579,9 +687,9 @@ __global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restric
 #pragma unroll 2
         for (int k = k0 + lane * 4; k < k1; k += 128) {
             float a[4], b[XE_SMALL_ROWS][4];
-            load4(a, w + j * ldw + k, 4, true);
+            load4_aligned(a, w + j * ldw + k);
 #pragma unroll
-            for (int r = 0; r < XE_SMALL_ROWS; ++r) load4(b[r], row[r] + k, 4, true);
+            for (int r = 0; r < XE_SMALL_ROWS; ++r) load4_aligned(b[r], row[r] + k);
 #pragma unroll
             for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] += (a[0] * b[r][0] + a[1] * b[r][1]) + (a[2] * b[r][2] + a[3] * b[r][3]);
         }
@@ -646,7 +754,6 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
     if (!out) return;
     const T* m = is_dw ? a.x : a.w;
     const long long ldm = is_dw ? a.ldx : a.ldw, ldo = is_dw ? a.lddw : a.lddx;
-    const bool aligned = ldm % 4 == 0;
     float acc[8][4];
 #pragma unroll
     for (int o = 0; o < 8; ++o)
@@ -659,7 +766,7 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
             const float f[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
             if (p.x == 0.f && p.y == 0.f && p.z == 0.f && p.w == 0.f && q.x == 0.f && q.y == 0.f && q.z == 0.f && q.w == 0.f) continue;
             float v[4];
-            load4(v, m + c * ldm + k, a.d - k, aligned);
+            load4f(v, m + c * ldm + k, a.d - k);
 #pragma unroll
             for (int o = 0; o < 8; ++o)
 #pragma unroll
@@ -684,6 +791,207 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
     }
 }
 
+// ---- few rows: FP32 products on the caller's matrices ----------------------------------------------------------
+// FP32X3 with up to 16 rows: the products are a read of W (twice) and a write of dW; splitting W into BF16 parts first would move it
+// three times more, and a 256-row tensor-core tile would be mostly empty.  In all three kernels a lane owns four features,
+// 32 apart (single elements then make whole lines at any pitch and alignment), whose values of all rows (x, or the sums of dx) it
+// holds in registers as packed pairs, and a warp walks over classes, one piece of 128 features of W or dW per class.
+// ROWS (4, 8 or 16) rows cost ROWS * 4 multiplications a lane and piece, which the FP32 pipe does faster than HBM delivers it.
+constexpr int XF_ROWS = 16, XF_COLS = 128, XF_CLASSES = 128;      // most rows; features and classes of a block
+struct FewArgs {
+    const float* x; const float* w;
+    float* out;                           // z, dx or its parts, dW
+    const float* dz;
+    long long ldx, ldw, ldo, plane;       // plane: elements between the parts of z or dx
+    int n, d, v, dzpitch, splits;
+    const float* rowg;                    // rows of weight 0 are not read
+    XeScale scale;
+    int* zero;
+};
+// features k, k + 32, k + 64, k + 96 of one row
+__device__ __forceinline__ void few_load(float (&v)[4], const float* row, int k, int d) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = k + 32 * e < d ? row[k + 32 * e] : 0.f;
+}
+template <int ROWS>
+__device__ __forceinline__ void few_load_x(float2 (&xr)[ROWS][2], const FewArgs& p, int k, bool weigh) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        float v[4];
+        const bool in = r < p.n && !(weigh && p.rowg[r] == 0.f);
+        few_load(v, p.x + (in ? r * p.ldx : 0), k, in ? p.d : 0);
+        xr[r][0] = make_float2(v[0], v[1]);
+        xr[r][1] = make_float2(v[2], v[3]);
+    }
+}
+
+// z: a block multiplies 128 classes with a part of the features, 128 at a time; the lanes' sums of a class meet in a halving
+// exchange and add up in shared memory
+template <int ROWS>
+__global__ void __launch_bounds__(128) xe_few_logits_kernel(const FewArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float zs[XF_CLASSES][ROWS + 1];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, j0 = blockIdx.x * XF_CLASSES;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 2) p.zero[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < XF_CLASSES * (ROWS + 1); i += 128) (&zs[0][0])[i] = 0.f;
+    __syncthreads();
+    const int slices = (p.d + XF_COLS - 1) / XF_COLS, s0 = (int)((long long)blockIdx.y * slices / p.splits), s1 = (int)((long long)(blockIdx.y + 1) * slices / p.splits);
+    const float* w = p.w;
+    const int count = p.v - j0 < XF_CLASSES ? p.v - j0 : XF_CLASSES;
+    for (int s = s0; s < s1; ++s) {
+        const int k = s * XF_COLS + lane;
+        float2 xr[ROWS][2];
+        few_load_x<ROWS>(xr, p, k, false);
+        constexpr int AHEAD = 4;                                   // pieces of W in flight per warp
+        float wv[AHEAD][4];
+        for (int c0 = warp; c0 < count; c0 += 4 * AHEAD) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int c = c0 + 4 * q;
+                few_load(wv[q], w + (c < count ? (j0 + c) * p.ldw : 0), k, c < count ? p.d : 0);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int c = c0 + 4 * q;
+                if (c >= count) break;
+                float t[ROWS];
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    float2 m = __fmul2_rn(xr[r][0], make_float2(wv[q][0], wv[q][1]));
+                    m = __ffma2_rn(xr[r][1], make_float2(wv[q][2], wv[q][3]), m);
+                    t[r] = m.x + m.y;
+                }
+                // t[r] of lane l -> lane r (mod ROWS) holds the sum over lanes
+#pragma unroll
+                for (int h = ROWS / 2; h >= 1; h >>= 1) {
+                    const bool up = lane & h;
+#pragma unroll
+                    for (int r = 0; r < h; ++r) {
+                        const float send = up ? t[r] : t[r + h], keep = up ? t[r + h] : t[r];
+                        t[r] = keep + __shfl_xor_sync(0xffffffffu, send, h);
+                    }
+                }
+#pragma unroll
+                for (int h = ROWS; h <= 16; h <<= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], h);
+                if (lane < ROWS) zs[c][lane] += t[0];              // this warp's class: nobody else's
+            }
+        }
+    }
+    __syncthreads();
+    float* z = p.out + blockIdx.y * p.plane;
+    for (int i = threadIdx.x; i < XF_CLASSES * p.n; i += 128) {
+        const int r = i / XF_CLASSES, c = i % XF_CLASSES;
+        if (c < count) z[r * p.ldo + j0 + c] = zs[c][r];
+    }
+}
+
+// dz of 128 classes, [class][row], from rows of floats
+template <int ROWS>
+__device__ __forceinline__ void few_stage_dz(float (&ds)[XF_CLASSES][ROWS], const FewArgs& p, int j0) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int j = j0 + threadIdx.x;
+        ds[threadIdx.x][r] = r < p.n && j < p.v ? p.dz[(long long)r * p.dzpitch + j] : 0.f;
+    }
+}
+
+// dx = dz W: a block takes 128 features and a part of the classes; its warps' sums meet in shared memory
+template <int ROWS>
+__global__ void __launch_bounds__(128) xe_few_dx_kernel(const FewArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ __align__(16) float ds[XF_CLASSES][ROWS];
+    __shared__ float sums[4][XF_COLS];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * XF_COLS + lane;
+    const int tiles = (p.v + XF_CLASSES - 1) / XF_CLASSES, t0 = (int)((long long)blockIdx.y * tiles / p.splits), t1 = (int)((long long)(blockIdx.y + 1) * tiles / p.splits);
+    const float* w = p.w;
+    float2 acc[ROWS][2];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) acc[r][0] = acc[r][1] = make_float2(0.f, 0.f);
+    for (int t = t0; t < t1; ++t) {
+        const int j0 = t * XF_CLASSES, count = p.v - j0 < XF_CLASSES ? p.v - j0 : XF_CLASSES;
+        __syncthreads();
+        few_stage_dz<ROWS>(ds, p, j0);
+        __syncthreads();
+        constexpr int AHEAD = 4;
+        float wv[AHEAD][4];
+        for (int c0 = warp; c0 < count; c0 += 4 * AHEAD) {
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int c = c0 + 4 * q;
+                few_load(wv[q], w + (c < count ? (j0 + c) * p.ldw : 0), k, c < count ? p.d : 0);
+            }
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int c = c0 + 4 * q < count ? c0 + 4 * q : c0;        // past the last: zeros of W
+                const float2 lo = make_float2(wv[q][0], wv[q][1]), hi = make_float2(wv[q][2], wv[q][3]);
+#pragma unroll
+                for (int r = 0; r < ROWS; r += 4) {
+                    const float4 g = *reinterpret_cast<const float4*>(&ds[c][r]);
+                    const float gv[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[r + e][0] = __ffma2_rn(make_float2(gv[e], gv[e]), lo, acc[r + e][0]);
+                        acc[r + e][1] = __ffma2_rn(make_float2(gv[e], gv[e]), hi, acc[r + e][1]);
+                    }
+                }
+            }
+        }
+    }
+    const float scale = xe_scale(p.scale);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        __syncthreads();
+        sums[warp][lane] = acc[r][0].x;
+        sums[warp][lane + 32] = acc[r][0].y;
+        sums[warp][lane + 64] = acc[r][1].x;
+        sums[warp][lane + 96] = acc[r][1].y;
+        __syncthreads();
+        const int kk = blockIdx.x * XF_COLS + threadIdx.x;
+        if (r < p.n && kk < p.d) {
+            const float s = ((sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x])) * scale;
+            const long long at = blockIdx.y * p.plane + r * p.ldo + kk;
+            p.out[at] = s;
+        }
+    }
+}
+
+// dW = dz^T x: a block makes 128 classes x 128 features
+template <int ROWS>
+__global__ void __launch_bounds__(128) xe_few_dw_kernel(const FewArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ __align__(16) float ds[XF_CLASSES][ROWS];
+    const unsigned kblocks = (unsigned)(p.d + XF_COLS - 1) / XF_COLS;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = (int)(blockIdx.x % kblocks) * XF_COLS + lane, j0 = (int)(blockIdx.x / kblocks) * XF_CLASSES;
+    const int count = p.v - j0 < XF_CLASSES ? p.v - j0 : XF_CLASSES;
+    float2 xr[ROWS][2];
+    few_load_x<ROWS>(xr, p, k, true);
+    few_stage_dz<ROWS>(ds, p, j0);
+    const float scale = xe_scale(p.scale);
+    __syncthreads();
+#pragma unroll 2
+    for (int c = warp; c < count; c += 4) {
+        float2 lo = make_float2(0.f, 0.f), hi = lo;
+#pragma unroll
+        for (int r = 0; r < ROWS; r += 4) {
+            const float4 g = *reinterpret_cast<const float4*>(&ds[c][r]);
+            const float gv[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                lo = __ffma2_rn(make_float2(gv[e], gv[e]), xr[r + e][0], lo);
+                hi = __ffma2_rn(make_float2(gv[e], gv[e]), xr[r + e][1], hi);
+            }
+        }
+        const float v[4] = {lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale};
+        float* o = p.out + (long long)(j0 + c) * p.ldo + k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (k + 32 * e < p.d) o[32 * e] = v[e];
+    }
+}
+
 unsigned loop_blocks(long long items) {
     const long long b = (items + 255) / 256, most = 16ll * sm_count();
     return (unsigned)(b < 1 ? 1 : b < most ? b : most);
@@ -696,7 +1004,7 @@ struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
-    bool small;                          // FP32 arithmetic instead of tensor cores
+    bool small, few;                     // FP32 arithmetic instead of tensor cores: xe_small_*, xe_few_*
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
     int zpitch, piece, pieces, dzpitch, parts;
@@ -705,14 +1013,28 @@ struct Plan {
     size_t off_x, off_w, off_z, off_stats, off_zsum, off_zt, off_lse, off_rowloss, off_rowg, off_count, off_dz, off_db, off_dx, off_dw, total;
 };
 
-// rows of dz a block of xe_rows_kernel sums up: as many blocks as fit the GPU twice at 1024 threads an SM
-int row_blocks(long long n, int threads) {
-    const long long most = 2048ll / threads * sm_count();
-    return (int)(n < most ? n : most);
+// parts of the contraction of an xe_few_* product: `tiles` blocks without splitting, `steps` pieces of the contraction;
+// about eight blocks an SM
+int few_split_count(long long tiles, long long steps) {
+    const long long want = 8ll * sm_count();
+    long long s = tiles > 0 ? (want + tiles - 1) / tiles : 1;
+    if (s > steps) s = steps;
+    if (s > 64) s = 64;
+    return (int)(s < 1 ? 1 : s);
+}
+
+// blocks of xe_rows_kernel or xe_warp_rows_kernel, each with a run of rows: no more than fit the GPU at once (1024 threads an
+// SM), and at least four rows each once every SM has a block, for the sake of the partial column sums
+int row_blocks(long long n, int v) {
+    if (v <= 512) {
+        const long long most = 4ll * sm_count(), b = (n + XE_WARP_ROWS - 1) / XE_WARP_ROWS;
+        return (int)(b < most ? b : most);
+    }
+    const long long most = (v <= 4096 ? 4ll : 2ll) * sm_count(), few = sm_count(), b = n / 4 < few ? (n < few ? n : few) : n / 4;
+    return (int)(b < most ? b : most);
 }
 constexpr int XE_ROWS_MAX_V = 512 * 4 * 4;          // widest row of xe_rows_kernel: wider ones spill, and one block an SM is
                                                     // slower than two kernels (1024 x 21841: 130 us against 92)
-int row_threads(int v) { return v <= 512 ? 128 : v <= 4096 ? 256 : 512; }
 
 // Parts of a contraction of `chunks` ring slots (times `products` plane pairs), and columns of a tile (256 or 128), so that
 // the CTA pairs are filled in as few whole turns as possible.  Estimated time: turns of the slots (0.28 us each on a pair;
@@ -775,16 +1097,23 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
     // logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured 6.5 TB/s and 1.4 PFLOP/s the
     // product is the dearer one from d = 1000 (200) on.
-    const bool few = n * v <= 64ll * XE_BM * XE_BN;
+    const bool few_tiles = n * v <= 64ll * XE_BM * XE_BN;
+    const long long class_tiles = (v + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
+    const int few_splits = few_split_count(class_tiles, col_tiles);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
+    p.few = !bf16 && !p.small && n > 0 && n <= XF_ROWS && z_bytes * few_splits <= limit;
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
         p.splits_z = (d->d + XE_SMALL_SLICE - 1) / XE_SMALL_SLICE;
-    } else if (few && fits) p.kept = true;
+    } else if (p.few) {
+        p.kept = true;
+        p.pack_x = p.pack_w = false;
+        p.splits_z = few_splits;
+    } else if (few_tiles && fits) p.kept = true;
     else if (grad && bf16 && !d->has_bias && dz_bytes <= limit) p.exps = true;
     else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
-    if (!grad && p.splits_z == 1 && !p.small) p.kept = false;          // statistics are all that is wanted
+    if (!grad && p.splits_z == 1 && !p.small && !p.few) p.kept = false;          // statistics are all that is wanted
     if (!p.kept) p.splits_z = 1;
     p.bn_z = p.kept && (p.splits_z > 1 || d->v <= XE_ROWS_MAX_V) ? cz.bn : XE_BN;                       // the other epilogues make statistics of 128 columns a warp
     p.piece = d->v;
@@ -804,9 +1133,13 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.splits_dx = cx.splits; p.splits_dw = cw.splits;
     p.bn_dx = cx.bn; p.bn_dw = cw.bn;
     // more than one piece adds up in floats: in dx itself, or in the scratch
+    if (p.few) {
+        p.splits_dx = few_split_count(col_tiles, class_tiles);
+        p.splits_dw = 1;
+    }
     p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
     p.dw_direct = p.splits_dw == 1;
-    p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, row_threads(d->v)) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
+    p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, d->v) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;
@@ -866,9 +1199,17 @@ int launch_rows(int planes, unsigned blocks, cudaStream_t st, const float* z, in
     if (planes < 0) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, false, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, false, false>);
     if (planes == 1) return split ? go(xe_rows_kernel<THREADS, QUADS, 1, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 1, true, false>);
     if (planes == 3) return split ? go(xe_rows_kernel<THREADS, QUADS, 3, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 3, true, false>);
-    if constexpr (THREADS == 128)
-        return split ? go(xe_rows_kernel<THREADS, QUADS, 0, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 0, true, false>);
-    return fail(WINO_E_BADARG, "xent: no row kernel");
+    return split ? go(xe_rows_kernel<THREADS, QUADS, 0, true, true>) : go(xe_rows_kernel<THREADS, QUADS, 0, true, false>);
+}
+
+int launch_warp_rows(int planes, unsigned blocks, cudaStream_t st, const float* z, int splits, int v, int zpitch, const float* bias, const RowArgs& ra,
+                     const XeDzRule& rule, void* dz, int dpitch, float* db_part) {
+    auto go = [&](auto kernel) { return xe_launch(kernel, blocks, 32 * XE_WARP_ROWS, 0, st, z, splits, v, zpitch, bias, ra, rule, dz, dpitch, db_part); };
+    const bool split = splits > 1;
+    if (planes < 0) return split ? go(xe_warp_rows_kernel<1, false, true>) : go(xe_warp_rows_kernel<1, false, false>);
+    if (planes == 1) return split ? go(xe_warp_rows_kernel<1, true, true>) : go(xe_warp_rows_kernel<1, true, false>);
+    if (planes == 3) return split ? go(xe_warp_rows_kernel<3, true, true>) : go(xe_warp_rows_kernel<3, true, false>);
+    return split ? go(xe_warp_rows_kernel<0, true, true>) : go(xe_warp_rows_kernel<0, true, false>);
 }
 
 template <typename T>
@@ -892,10 +1233,62 @@ int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* d
     return xe_launch(xe_small_grad_kernel<T>, (unsigned)(a.dx_blocks + dw_blocks + (loss.loss ? 1 : 0)), 256, XE_SMALL_GRAD_SMEM, st, a);
 }
 
+int launch_db(const float* part, int parts, int pitch, int cols, const XeScale& scale, float* db, cudaStream_t st) {
+    if (cols < 4096) return xe_launch(xe_db_kernel<8>, (unsigned)(cols + 7) / 8, 512, 0, st, part, parts, pitch, cols, scale, db);
+    return xe_launch(xe_db_kernel<32>, (unsigned)(cols + 31) / 32, 512, 0, st, part, parts, pitch, cols, scale, db);
+}
+
 int finish(const wino_xent_desc& d, const Plan& p, const float* buf, int splits, long long rows, void* out, long long ld, cudaStream_t st) {
     const unsigned blocks = loop_blocks(rows * ((d.d + 3) / 4));
     if (d.dtype == WINO_BF16) return xe_launch(xe_finish_kernel<__nv_bfloat16>, blocks, 256, 0, st, buf, splits, rows, d.d, p.dpitch, (__nv_bfloat16*)out, ld);
     return xe_launch(xe_finish_kernel<float>, blocks, 256, 0, st, buf, splits, rows, d.d, p.dpitch, (float*)out, ld);
+}
+
+FewArgs few_args(const void* x, const void* w, const wino_xent_desc& d, const Plan& p) {
+    FewArgs a = {};
+    a.x = (const float*)x; a.w = (const float*)w;
+    a.ldx = p.ldx; a.ldw = p.ldw;
+    a.n = d.n; a.d = d.d; a.v = d.v; a.dzpitch = p.zpitch;
+    return a;
+}
+
+// the kernel for 4, 8 or 16 rows
+template <typename Pick>
+int few_launch(int n, dim3 grid, cudaStream_t st, const FewArgs& a, Pick pick) {
+    if (n <= 4) return xe_launch(pick(std::integral_constant<int, 4>()), grid, 128, 0, st, a);
+    if (n <= 8) return xe_launch(pick(std::integral_constant<int, 8>()), grid, 128, 0, st, a);
+    return xe_launch(pick(std::integral_constant<int, 16>()), grid, 128, 0, st, a);
+}
+
+int launch_few_logits(const void* x, const void* w, const wino_xent_desc& d, const Plan& p, float* z, int* zero, cudaStream_t st) {
+    FewArgs a = few_args(x, w, d, p);
+    a.out = z; a.ldo = p.zpitch; a.plane = (long long)d.n * p.zpitch;
+    a.splits = p.splits_z;
+    a.zero = zero;
+    const dim3 grid((unsigned)((d.v + XF_CLASSES - 1) / XF_CLASSES), (unsigned)a.splits);
+    return few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_logits_kernel<decltype(rows)::value>; });
+}
+
+int launch_few_grad(const void* x, const void* w, void* dx, void* dw, const wino_xent_desc& d, const Plan& p, const float* dz, float* buf, const float* rowg,
+                    const XeScale& scale, cudaStream_t st) {
+    FewArgs a = few_args(x, w, d, p);
+    a.dz = dz; a.rowg = rowg; a.scale = scale;
+    const unsigned kblocks = (unsigned)((d.d + XF_COLS - 1) / XF_COLS), jblocks = (unsigned)((d.v + XF_CLASSES - 1) / XF_CLASSES);
+    int rc;
+    if (dx) {
+        a.out = p.dx_direct ? (float*)dx : buf; a.ldo = p.dx_direct ? p.lddx : p.dpitch; a.plane = (long long)d.n * p.dpitch;
+        a.splits = p.splits_dx;
+        const dim3 grid(kblocks, (unsigned)a.splits);
+        rc = few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_dx_kernel<decltype(rows)::value>; });
+        if (rc || (!p.dx_direct && (rc = finish(d, p, buf, p.splits_dx, d.n, dx, p.lddx, st)))) return rc;
+    }
+    if (dw) {
+        a.out = (float*)dw; a.ldo = p.lddw;
+        const dim3 grid(kblocks * jblocks);
+        rc = few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_dw_kernel<decltype(rows)::value>; });
+        if (rc) return rc;
+    }
+    return WINO_OK;
 }
 
 int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, const float* bias, const long long* target, const float* dloss, float* loss,
@@ -961,7 +1354,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     sum.loss = d.reduction == WINO_NONE ? nullptr : loss;
     sum.rowloss = ra.rowloss; sum.n = n; sum.count = ra.count;
     sum.mean = d.reduction == WINO_MEAN;
-    const bool later = products && (dx || dw) && n <= 8192;
+    const bool later = products && (dx || dw) && n <= 1024 && !p.few;
     if (!later) ra.loss = sum;
     if ((rc = status_word(&ra.status))) return rc;
     const float* b = d.has_bias ? bias : nullptr;
@@ -974,7 +1367,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     scale.factor = dz_factor;
     scale.mean = sum.mean;
 
-    const bool kept_stats = p.kept && wide && p.splits_z == 1;
+    const bool kept_stats = p.kept && wide && p.splits_z == 1 && !p.few;
     XeProduct pz = {kept_stats ? XE_STATS_Z : p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
     pz.bn = p.bn_z;
     pz.out.zero = ra.count;
@@ -983,17 +1376,22 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         pz.out.ptr = z;
         pz.out.pitch = p.zpitch;
         pz.out.splits = p.splits_z;
-        if (!p.small) rc = xe_gemm(&pz, 1, st);
+        if (p.few) rc = launch_few_logits(x, w, d, p, z, ra.count, st);
+        else if (!p.small) rc = xe_gemm(&pz, 1, st);
         else if (p.es == 2) rc = launch_small_logits<__nv_bfloat16>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
         else rc = launch_small_logits<float>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
         if (rc) return rc;
         if (wide) {
-            rc = xe_launch(xe_wide_rows_kernel, (unsigned)n, 256, 0, st, z, p.splits_z, d.v, p.zpitch, b, ra);
+            const unsigned chunks = (unsigned)((v + XE_CHUNK - 1) / XE_CHUNK);
+            float2* stats = reinterpret_cast<float2*>(ws + p.off_stats);
+            float* zsum = d.label_smoothing > 0.f ? f(p.off_zsum) : nullptr;
+            if ((rc = xe_launch(xe_wide_stats_kernel, chunks * (unsigned)n, 256, 0, st, z, p.splits_z, d.v, p.zpitch, b, n, target, stats, zsum, f(p.off_zt)))) return rc;
+            rc = xe_launch(xe_rows_from_stats_kernel, (unsigned)((n + 31) / 32), 256, 0, st, stats, zsum, f(p.off_zt), (int)chunks, ra);
         } else {
-            const unsigned blocks = (unsigned)row_blocks(n, row_threads(d.v));
-            auto rows_fn = d.v <= 512 ? launch_rows<128, 1> : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
+            const unsigned blocks = (unsigned)row_blocks(n, d.v);
+            auto rows_fn = d.v <= 512 ? launch_warp_rows : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
                          : d.v <= 4096 ? launch_rows<256, 4> : launch_rows<512, 4>;
-            if (p.small && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, nullptr);
+            if ((p.small || p.few) && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, nullptr);
             else rc = rows_fn(products ? p.planes : -1, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, dz, p.dzpitch, db_part);
         }
     } else {
@@ -1018,6 +1416,15 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     if (p.small)
         return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st)
                          : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st);
+    if (p.few) {
+        float* z = f(p.off_z);
+        if (wide) {
+            const unsigned grid = (unsigned)((v + 255) / 256) * (unsigned)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
+            if ((rc = xe_launch(xe_wide_dz_kernel<0>, grid, 128, 0, st, z, d.v, p.zpitch, n, ra.lse, ra.rowg, target, dzr, z, p.zpitch, nullptr))) return rc;
+        }
+        if (db && (rc = launch_db(z, (int)n, p.zpitch, d.v, scale, db, st))) return rc;
+        return launch_few_grad(x, w, dx, dw, d, p, z, f(p.off_dx), ra.rowg, scale, st);
+    }
     for (int i = 0; i < p.pieces; ++i) {
         const int v0 = i * p.piece, vc = d.v - v0 < p.piece ? d.v - v0 : p.piece;
         XeOperand wp = ow;                 // the piece's rows of W
@@ -1039,10 +1446,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             if ((rc = xe_gemm(&pd, 1, st))) return rc;
         }
         if (rc) return rc;
-        if (db) {
-            rc = xe_launch(xe_db_kernel, (unsigned)(vc + 31) / 32, 512, 0, st, db_part, p.parts, p.dzpitch, vc, scale, db + v0);
-            if (rc) return rc;
-        }
+        if (db && (rc = launch_db(db_part, p.parts, p.dzpitch, vc, scale, db + v0, st))) return rc;
 
         const XeOperand odz = {dz, n, vc, p.dzpitch, n * p.dzpitch, p.planes, false};
         const bool bf16 = p.planes == 1, first = i == 0, last = i == p.pieces - 1;
@@ -1071,13 +1475,12 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             zr.along_rows = xr.along_rows = true;
             product(zr, xr, vc, n, p.dw_direct, p.splits_dw, p.bn_dw, false, dw_at, p.lddw, f(p.off_dw));
         }
-        // Both in one launch where their epilogues agree and one of them has few tiles: the other fills the SMs that it
-        // leaves idle (256 x 25088 x 1000: 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU
+        // Both in one launch where one of them has few tiles: the other fills the SMs that it leaves idle (256 x 25088 x 1000: 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU
         // runs at its power limit either way (8192 x 4096 x 50021: 8.2 ms apart, 8.4 ms together).
         const long long tiles_x = (n + XE_BM - 1) / XE_BM * ((d.d + p.bn_dx - 1) / p.bn_dx) * p.splits_dx;
         const long long tiles_w = ((long long)vc + XE_BM - 1) / XE_BM * ((d.d + p.bn_dw - 1) / p.bn_dw) * p.splits_dw;
         if (first && later) prod[0].out.loss = sum;
-        if (count == 2 && prod[0].epi == prod[1].epi && p.bn_dx == p.bn_dw && (tiles_x < tiles_w ? tiles_x : tiles_w) < sm_count()) {
+        if (count == 2 && p.bn_dx == p.bn_dw && (tiles_x < tiles_w ? tiles_x : tiles_w) < sm_count()) {
             if ((rc = xe_gemm(prod, 2, st))) return rc;
         } else {
             for (int k = 0; k < count; ++k)

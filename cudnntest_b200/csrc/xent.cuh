@@ -111,7 +111,7 @@ struct XeProduct {
     XeOutput out;
     int bn = XE_BN;                   // columns of a tile: 256, or 128 (XE_F32, XE_BF16)
 };
-// one or two products in one launch; two must have the same epilogue, XE_F32 or XE_BF16, and the same bn
+// one or two products in one launch; two must have the same bn and epilogues XE_F32 or XE_BF16
 int xe_gemm(const XeProduct* prod, int count, cudaStream_t st);
 
 __device__ __forceinline__ float xe_ex2(float x) {

@@ -47,7 +47,7 @@ struct alignas(64) XeProblem {
     unsigned char pa[6], pb[6];       // planes of a and b, one entry per partial product
     int a_mn, b_mn;                   // contracted along the rows of the stored matrix
     uint32_t idesc;
-    int add;
+    int add, bf16;                    // XE_F32, XE_BF16 (one kernel for both)
     int plain;                        // rows that TMA cannot store: out_ptr, out_pitch
     void* out_ptr;
     long long out_pitch;
@@ -75,14 +75,14 @@ struct XeParams {
 template <int EPI, int PLANES, int BN>
 struct XeSmem {
     static constexpr int B_BYTES = BN / 2 * 128;                          // a CTA's half of the rows of b per ring slot
-    static constexpr int STORE_TILES = EPI == XE_STATS ? 0 : PLANES;      // per staging buffer
-    static constexpr int STAGES = PLANES == 3 ? 4 : EPI == XE_STATS || BN < 256 ? 6 : 5;
+    static constexpr int STAGES = EPI == XE_STATS || BN < 256 ? 6 : 5;
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = STAGES * XE_TILE_BYTES;
     static constexpr int STORE_OFF = B_OFF + STAGES * B_BYTES;
-    static constexpr int BUF = STORE_TILES * XE_STAGE_TILE;
-    static constexpr int NBUF = PLANES == 3 ? 1 : 2;
-    static constexpr int BAR_OFF = STORE_OFF + NBUF * XE_EPI_WARPS * BUF;
+    static constexpr int BUF = EPI == XE_STATS ? 0 : XE_STAGE_TILE;
+    static constexpr int NBUF = EPI >= XE_STATS ? 1 : 2;                  // staging tiles per epilogue warp
+    static constexpr int BIAS_OFF = STORE_OFF + NBUF * XE_EPI_WARPS * BUF;               // 128 floats per epilogue warp
+    static constexpr int BAR_OFF = BIAS_OFF + (EPI >= XE_STATS ? XE_EPI_WARPS * 512 : 0);
     static constexpr int SLOT_OFF = BAR_OFF + 8 * (2 * STAGES + 4);
     static constexpr int TOTAL = SLOT_OFF + 16 + 1024;
 };
@@ -103,6 +103,25 @@ __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32
     asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
                  "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
+}
+
+// packed FP32 pairs: one issue slot for two columns, each rounded like the scalar operation
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {
+    const float2 r = __fadd2_rn(make_float2(a, b), make_float2(c, d));
+    a = r.x; b = r.y;
+}
+__device__ __forceinline__ void mul2(float& a, float& b, float c) {
+    const float2 r = __fmul2_rn(make_float2(a, b), make_float2(c, c));
+    a = r.x; b = r.y;
+}
+__device__ __forceinline__ void fma2(float& a, float& b, float c, float d) {
+    const float2 r = __ffma2_rn(make_float2(a, b), make_float2(c, c), make_float2(d, d));
+    a = r.x; b = r.y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
@@ -289,6 +308,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
         uint8_t* stage_gen = gen_base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
         const uint32_t stage_s = base + L::STORE_OFF + (warp - 2) * L::NBUF * L::BUF;
         const uint32_t tempty_leader = mapa_shared(bar_tempty, 0);
+        float* bias_s = reinterpret_cast<float*>(gen_base + L::BIAS_OFF + (warp - 2) * 512);
         int as = 0;
         uint32_t aphase = 0, issued = 0;
         bool ok = true;
@@ -313,6 +333,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             const XeProblem& p = decode(u, w);
             const long long row0 = (long long)(w.mp * 2 + (int)rank) * 128 + quarter * 32;
             const long long row = row0 + lane, wcol = (long long)w.nb * BN + half * WCOLS;
+
+            // what the epilogue reads, on its way while the products run
+            constexpr bool SOFTMAX = EPI >= XE_STATS;
+            const bool live = row < p.m, whole = wcol + WCOLS <= p.n;
+            long long target = -1;
+            float lse = 0.f, g = 0.f;
+            if constexpr (SOFTMAX) {
+                if (live) target = p.target[row];
+                if constexpr (EPI == XE_DZ) {
+                    if (live) { lse = p.lse[row]; g = p.rowg[row]; }
+                }
+                if (p.bias) {                         // four columns per lane, to be read by all lanes
+                    const float* b = p.bias + wcol + lane * 4;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    const long long left = p.n - wcol - lane * 4;
+                    if (left >= 4) v = __ldg(reinterpret_cast<const float4*>(b));
+                    else if (left > 0) { v.x = b[0]; v.y = left > 1 ? b[1] : 0.f; v.z = left > 2 ? b[2] : 0.f; }
+                    __syncwarp();
+                    reinterpret_cast<float4*>(bias_s)[lane] = v;
+                    __syncwarp();
+                }
+            }
 
             float z[WCOLS];                        // this thread's row of the tile
             for (int cb = w.c0; cb < w.c1; cb += p.block) {
@@ -343,22 +385,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             if (row0 >= p.m || wcol >= p.n) continue;
 
             // 64 columns of values, packed as BF16 pairs, to plane `plane` of the output
-            auto stage64 = [&](const uint32_t (&w)[32], uint32_t buf, int plane) {
-                uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + plane * XE_STAGE_TILE + lane * 128);
+            auto stage64 = [&](const uint32_t (&w)[32], uint32_t buf) {
+                uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + lane * 128);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) dst[j ^ (lane & 7)] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
             };
-            auto store64 = [&](uint32_t buf, long long col0, int planes) {
+            auto store64 = [&](uint32_t buf, long long col0, int plane) {
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) {
-                    for (int q = 0; q < planes; ++q)
-                        tma_store_3d(&p.tm_out, stage_s + buf * L::BUF + q * XE_STAGE_TILE, (int)col0, (int)row0, q);
+                    tma_store_3d(&p.tm_out, stage_s + buf * L::BUF, (int)col0, (int)row0, plane);
                     tma_store_commit();
                 }
             };
 
-            if constexpr (EPI == XE_F32 || EPI == XE_BF16) {
+            if constexpr (EPI == XE_F32) {
                 const float scale = xe_scale(p.scale);
 #pragma unroll
                 for (int i = 0; i < WCOLS; ++i) z[i] *= scale;
@@ -381,9 +422,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                             const int rows = p.m - row0 < 32 ? (int)(p.m - row0) : 32;
                             if (col0 + lane < p.n) {
                                 const float* src = reinterpret_cast<const float*>(stage_gen + buf * L::BUF) + (lane & 3);
-                                for (int r = 0; r < rows; ++r) {
-                                    const float x = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
-                                    o[r * p.out_pitch] = p.add ? o[r * p.out_pitch] + x : x;
+                                const long long pitch = p.out_pitch;
+                                if (rows == 32 && !p.add) {
+#pragma unroll
+                                    for (int r = 0; r < 32; ++r) o[r * pitch] = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
+                                } else {
+                                    for (int r = 0; r < rows; ++r) {
+                                        const float x = src[r * 32 + ((lane >> 2) ^ (r & 7)) * 4];
+                                        o[r * pitch] = p.add ? o[r * pitch] + x : x;
+                                    }
                                 }
                             }
                             __syncwarp();
@@ -400,8 +447,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                 }
             };
             if constexpr (EPI == XE_F32) {
-                store_floats();
-            } else if constexpr (EPI == XE_BF16) {
+                if (!p.bf16) {
+                    store_floats();
+                    continue;
+                }
 #pragma unroll
                 for (int h = 0; h < WCOLS / 64; ++h) {
                     if (wcol + h * 64 < p.n) {
@@ -409,48 +458,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                         uint32_t pk[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                        stage64(pk, buf, 0);
+                        stage64(pk, buf);
                         if (p.plain) {                // row by row, two columns of 32 per row
                             __syncwarp();
                             const int rows = p.m - row0 < 32 ? (int)(p.m - row0) : 32;
                             const unsigned short* src = reinterpret_cast<const unsigned short*>(stage_gen + buf * L::BUF) + (lane & 7);
                             unsigned short* o = static_cast<unsigned short*>(p.out_ptr) + row0 * p.out_pitch + wcol + h * 64 + lane;
                             const bool in0 = wcol + h * 64 + lane < p.n, in1 = wcol + h * 64 + 32 + lane < p.n;
-                            for (int r = 0; r < rows; ++r) {
-                                if (in0) o[r * p.out_pitch] = src[r * 64 + ((lane >> 3) ^ (r & 7)) * 8];
-                                if (in1) o[r * p.out_pitch + 32] = src[r * 64 + (((lane >> 3) + 4) ^ (r & 7)) * 8];
+                            const long long pitch = p.out_pitch;
+                            if (rows == 32 && __all_sync(0xffffffffu, in1)) {
+#pragma unroll
+                                for (int r = 0; r < 32; ++r) {
+                                    o[r * pitch] = src[r * 64 + ((lane >> 3) ^ (r & 7)) * 8];
+                                    o[r * pitch + 32] = src[r * 64 + (((lane >> 3) + 4) ^ (r & 7)) * 8];
+                                }
+                            } else {
+                                for (int r = 0; r < rows; ++r) {
+                                    if (in0) o[r * pitch] = src[r * 64 + ((lane >> 3) ^ (r & 7)) * 8];
+                                    if (in1) o[r * pitch + 32] = src[r * 64 + (((lane >> 3) + 4) ^ (r & 7)) * 8];
+                                }
                             }
                             __syncwarp();
                             continue;
                         }
-                        store64(buf, wcol + h * 64, 1);
+                        store64(buf, wcol + h * 64, 0);
                     }
                 }
             } else {
-                const bool live = row < p.m, whole = wcol + WCOLS <= p.n;
                 if (p.bias) {
-                    if (whole) {
-                        const float4* b4 = reinterpret_cast<const float4*>(p.bias + wcol);
 #pragma unroll
-                        for (int j = 0; j < WCOLS / 4; ++j) {
-                            const float4 b = __ldg(b4 + j);
-                            z[4 * j] += b.x;
-                            z[4 * j + 1] += b.y;
-                            z[4 * j + 2] += b.z;
-                            z[4 * j + 3] += b.w;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < WCOLS; ++i)
-                            if (wcol + i < p.n) z[i] += __ldg(p.bias + wcol + i);
+                    for (int j = 0; j < WCOLS / 4; ++j) {
+                        const float4 b = reinterpret_cast<const float4*>(bias_s)[j];
+                        add2(z[4 * j], z[4 * j + 1], b.x, b.y);
+                        add2(z[4 * j + 2], z[4 * j + 3], b.z, b.w);
                     }
                 }
                 // column of the target among this warp's, -1 when it lies elsewhere
-                int tc = -1;
-                if (live) {
-                    const long long t = p.target[row] - p.col_base - wcol;
-                    if (t >= 0 && t < WCOLS) tc = (int)t;
-                }
+                const long long tl = target - p.col_base - wcol;
+                const int tc = live && tl >= 0 && tl < WCOLS ? (int)tl : -1;
                 const bool here = __any_sync(0xffffffffu, tc >= 0);
                 if constexpr (EPI == XE_STATS || EPI == XE_STATS_E || EPI == XE_STATS_Z) {
                     if constexpr (EPI == XE_STATS_Z) store_floats();
@@ -472,14 +517,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                     }
                     float cm[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-                    for (int i = 4; i < WCOLS; ++i) cm[i & 3] = fmaxf(cm[i & 3], z[i]);
-                    const float mx = fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3]));
+                    for (int i = 4; i < WCOLS; i += 2) cm[i / 2 & 3] = max3(cm[i / 2 & 3], z[i], z[i + 1]);
+                    const float mx = fmaxf(max3(cm[0], cm[1], cm[2]), cm[3]);
                     const float ref = mx == -INFINITY ? 0.f : mx;      // nothing but -inf: every term is 0
                     float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = 0; i < WCOLS; ++i) {
-                        z[i] = xe_ex2((z[i] - ref) * XE_LOG2E);
-                        t[i & 3] += z[i];
+                    for (int i = 0; i < WCOLS; i += 2) {
+                        add2(z[i], z[i + 1], -ref, -ref);
+                        mul2(z[i], z[i + 1], XE_LOG2E);
+                        z[i] = xe_ex2(z[i]);
+                        z[i + 1] = xe_ex2(z[i + 1]);
+                        add2(t[i & 2], t[(i & 2) + 1], z[i], z[i + 1]);
                     }
                     if (live) p.stats[wcol / XE_STAT_COLS * p.m + row] = make_float2(mx, (t[0] + t[1]) + (t[2] + t[3]));
                     if constexpr (EPI == XE_STATS_E) {
@@ -490,18 +538,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                                 uint32_t pk[32];
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                stage64(pk, buf, 0);
-                                store64(buf, wcol + h * 64, 1);
+                                stage64(pk, buf);
+                                store64(buf, wcol + h * 64, 0);
                             }
                         }
                     }
                 } else {
-                    float lse = 0.f, g = 0.f;
-                    if (live) { lse = p.lse[row]; g = p.rowg[row]; }
                     const float gp = g * p.rule.pf, ga = g * p.rule.smooth_all;
-                    // a row that does not count: exactly 0, whatever its logits
 #pragma unroll
-                    for (int i = 0; i < WCOLS; ++i) z[i] = g == 0.f ? 0.f : gp * xe_ex2((z[i] - lse) * XE_LOG2E) - ga;
+                    for (int i = 0; i < WCOLS; i += 2) {
+                        add2(z[i], z[i + 1], -lse, -lse);
+                        mul2(z[i], z[i + 1], XE_LOG2E);
+                        z[i] = xe_ex2(z[i]);
+                        z[i + 1] = xe_ex2(z[i + 1]);
+                        fma2(z[i], z[i + 1], gp, -ga);
+                    }
+                    if (__any_sync(0xffffffffu, g == 0.f)) {          // a row that does not count: exactly 0, whatever its logits
+#pragma unroll
+                        for (int i = 0; i < WCOLS; ++i) z[i] = g == 0.f ? 0.f : z[i];
+                    }
                     if (here) {
                         const float gt = g * p.rule.smooth_t;
 #pragma unroll
@@ -510,45 +565,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (wcol + h * 64 < p.n) {
-                            const uint32_t buf = next_buffer();
-                            uint32_t pk[32];
-                            if constexpr (PLANES == 1) {
+                            auto sums = [&]() {       // of this warp's 32 rows
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                stage64(pk, buf, 0);
-                                store64(buf, wcol + h * 64, 1);
-                                if (p.db_part) {
+                                for (int k = 0; k < 2; ++k) {
+                                    const long long col = wcol + h * 64 + k * 32 + lane;
+                                    float c[32];
 #pragma unroll
-                                    for (int k = 0; k < 2; ++k) {
-                                        const long long col = wcol + h * 64 + k * 32 + lane;
-                                        const float cs = column_sums(&z[64 * h + 32 * k], lane);
-                                        if (col < p.n) p.db_part[(row0 / 32) * p.db_pitch + col] = cs;
-                                    }
+                                    for (int i = 0; i < 32; ++i) c[i] = z[64 * h + 32 * k + i];
+                                    const float cs = column_sums(c, lane);
+                                    if (col < p.n) p.db_part[(row0 / 32) * p.db_pitch + col] = cs;
                                 }
-                            } else {
-                                if (p.db_part) {
+                            };
+                            if (PLANES > 1 && p.db_part) sums();
 #pragma unroll
-                                    for (int k = 0; k < 2; ++k) {
-                                        float c[32];
+                            for (int q = 0; q < PLANES; ++q) {        // round; several planes: keep the remainder for the next
+                                const uint32_t buf = next_buffer();
+                                uint4* dst = reinterpret_cast<uint4*>(stage_gen + buf * L::BUF + lane * 128);
 #pragma unroll
-                                        for (int i = 0; i < 32; ++i) c[i] = z[64 * h + 32 * k + i];
-                                        const long long col = wcol + h * 64 + k * 32 + lane;
-                                        const float cs = column_sums(c, lane);
-                                        if (col < p.n) p.db_part[(row0 / 32) * p.db_pitch + col] = cs;
+                                for (int j = 0; j < 8; ++j) {
+                                    uint32_t w4[4];
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        float& v0 = z[64 * h + 8 * j + 2 * i];
+                                        float& v1 = z[64 * h + 8 * j + 2 * i + 1];
+                                        w4[i] = pack_bf16(v0, v1);
+                                        if (q + 1 < PLANES) {
+                                            v0 -= __uint_as_float(w4[i] << 16);
+                                            v1 -= __uint_as_float(w4[i] & 0xffff0000u);
+                                        }
                                     }
+                                    dst[j ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
                                 }
-#pragma unroll
-                                for (int q = 0; q < PLANES; ++q) {        // round, keep the remainder for the next plane
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i) {
-                                        pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
-                                        z[64 * h + 2 * i] -= __uint_as_float(pk[i] << 16);
-                                        z[64 * h + 2 * i + 1] -= __uint_as_float(pk[i] & 0xffff0000u);
-                                    }
-                                    stage64(pk, buf, q);
-                                }
-                                store64(buf, wcol + h * 64, PLANES);
+                                store64(buf, wcol + h * 64, q);
                             }
+                            if (PLANES == 1 && p.db_part) sums();
                         }
                     }
                 }
@@ -639,6 +689,7 @@ int make_problem(const XeProduct& x, XeProblem* out) {
     p.b_mn = x.b.along_rows;
     p.idesc = make_idesc(OP_BF16, x.bn, XE_BM) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u);
     p.add = o.add;
+    p.bf16 = x.epi == XE_BF16;
     p.out_ptr = o.ptr; p.out_pitch = o.pitch;
     p.scale = o.scale;
     p.bias = o.bias; p.target = o.target; p.col_base = o.col_base;
@@ -673,8 +724,8 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
     }
     if ((rc = status_word(&p.status))) return rc;
     switch (prod[0].epi) {
-        case XE_F32: return prod[0].bn == 128 ? run<XE_F32, 1, 128>(p, st) : run<XE_F32, 1>(p, st);
-        case XE_BF16: return prod[0].bn == 128 ? run<XE_BF16, 1, 128>(p, st) : run<XE_BF16, 1>(p, st);
+        case XE_F32:
+        case XE_BF16: return prod[0].bn == 128 ? run<XE_F32, 1, 128>(p, st) : run<XE_F32, 1>(p, st);
         case XE_STATS: return run<XE_STATS, 1>(p, st);
         case XE_STATS_Z: return run<XE_STATS_Z, 1>(p, st);
         case XE_STATS_E: return run<XE_STATS_E, 1>(p, st);

@@ -2,9 +2,10 @@
 
 Tolerances are element-wise bounds, added up from the roundings that happen, not measured:
   * a rounding to BF16 is off by at most 2^-8 of the value, one to FP32 by 2^-24;
-  * a sum of K terms on the tensor cores or in FP32 is off by at most (steps + 16) 2^-23 sum |terms|, one step per 16 terms
-    (one truncation of the accumulator, and the alignment of the 16 products);
-  * FP32X3 leaves out products below 2^-25 of a term, six partial products take six times the steps;
+  * a sum of K terms on the tensor cores is off by at most (steps + 16) 2^-23 sum |terms|, one step per 16 terms (one
+    truncation of the accumulator, and the alignment of the 16 products); FP32X3 leaves out products below 2^-25 of a term,
+    and its six partial products take six times the steps;
+  * a sum in FP32 arithmetic by K 2^-24 sum |terms|, one rounding per term;
   * ex2.approx is off by at most 2^-22, and exp(z - lse) by the errors of z and lse on top.
 """
 import numpy as np
@@ -25,8 +26,8 @@ def _torch():
 
 def _sum_eps(k, dtype):
     """Relative (to the sum of magnitudes) error of a product with contraction length k."""
-    steps = -(-k // 16)
-    return (steps + 16) * 2.0 ** -23 if dtype == "bf16" else (6 * steps + 16) * 2.0 ** -23 + 2.0 ** -23
+    steps = max(-(-k // 16) * (1 if dtype == "bf16" else 6), k / 2)
+    return (steps + 17) * 2.0 ** -23
 
 
 class Case:
@@ -132,6 +133,13 @@ CASES = [
     (700, 1500, 1900, "bf16", {}),
     (1000, 40, 100, "fp32", {}),                                  # plain FP32 kernels up to their most rows and classes
     (3, 1001, 1024, "bf16", {}),
+    (16, 1001, 3000, "fp32", {}),                                 # few rows: FP32 arithmetic on the caller's matrices
+    (9, 1001, 3000, "bf16", dict(bias=False)),
+    (8, 1002, 3000, "bf16", {}),
+    (3, 260, 70001, "fp32", dict(ldx=264, ldw=261)),
+    (13, 6001, 130, "fp32", {}),
+    (17, 1001, 3000, "fp32", {}),                                 # one row more than that
+    (64, 1001, 3000, "fp32", {}),
     (300, 2200, 700, "bf16", dict(bias=False)),                   # blocks of the contraction: 1024 + 1024 + 152
     (2100, 700, 2400, "fp32", {}),                                # 256 + 256 + 188, logits recomputed below
     (4000, 64, 5, "bf16", {}),                                    # long contraction of dW over rows, few classes
@@ -158,7 +166,8 @@ def test_gradient_against_definition(n, d, v, dtype, kw, reduction):
     cb.device_status()
 
 
-@pytest.mark.parametrize("n,d,v,dtype", [(40, 4096, 1000, "bf16"), (300, 96, 700, "fp32"), (2305, 40, 2100, "bf16"), (2305, 40, 2100, "fp32")])
+@pytest.mark.parametrize("n,d,v,dtype", [(40, 4096, 1000, "bf16"), (300, 96, 700, "fp32"), (2305, 40, 2100, "bf16"), (2305, 40, 2100, "fp32"),
+                                         (15, 2300, 700, "fp32"), (7, 2301, 700, "bf16"), (100, 64, 100, "bf16")])
 @pytest.mark.parametrize("ignored", [0.3, 1.0])
 @pytest.mark.parametrize("ignore_index", [-100, 3, 2 ** 62])
 def test_ignored_rows_leave_no_trace(n, d, v, dtype, ignored, ignore_index):
@@ -288,7 +297,7 @@ def test_no_rows():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-@pytest.mark.parametrize("n,d,v", [(300, 200, 700), (2305, 40, 2100)])
+@pytest.mark.parametrize("n,d,v", [(300, 200, 700), (2305, 40, 2100), (14, 201, 7000), (100, 60, 100)])
 @pytest.mark.parametrize("pad", [0, 1, 8])
 def test_outputs_stay_inside_their_rows(dtype, n, d, v, pad):
     """dx and dw inside wider buffers with guard rows: nothing but the results is written; left-out products cost nothing."""
