@@ -78,6 +78,45 @@ __device__ __forceinline__ void load4f(float (&v)[4], const T* p, int left) {
     for (int e = 0; e < 4; ++e) v[e] = to_float<T>(t[e]);
 }
 
+// The same for BF16 rows that start anywhere: a warp copies 256 columns of a row, neighbouring lanes neighbouring elements (PAIRS:
+// pairs of them, where every row starts on 4 bytes), so that both sides are whole lines whatever the pitch
+template <bool PAIRS>
+__global__ void __launch_bounds__(256) xe_pack_rows_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x % 32;
+    const unsigned chunks = (unsigned)(pitch + 255) / 256;
+    const long long items0 = j0.rows * chunks, total = items0 + j1.rows * chunks;
+    for (long long w = (long long)blockIdx.x * 8 + threadIdx.x / 32; w < total; w += (long long)gridDim.x * 8) {
+        const bool second = w >= items0;
+        const PackJob& j = second ? j1 : j0;
+        const long long i = second ? w - items0 : w, r = i < (1ll << 32) ? (long long)((unsigned)i / chunks) : i / chunks;
+        const int c0 = (int)(i - r * chunks) * 256;
+        const bool live = !j.target || row_counts(rule, j.target[r]);
+        const unsigned short* src = static_cast<const unsigned short*>(j.src) + r * j.ld + c0;
+        unsigned short* dst = reinterpret_cast<unsigned short*>(j.dst) + r * pitch + c0;
+        const int have = live ? cols - c0 : 0, want = pitch - c0;
+        if (PAIRS) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = (e * 32 + lane) * 2;
+                v[e] = c + 2 <= have ? *reinterpret_cast<const uint32_t*>(src + c) : c < have ? src[c] : 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if ((e * 32 + lane) * 2 < want) *reinterpret_cast<uint32_t*>(dst + (e * 32 + lane) * 2) = v[e];
+        } else {
+            unsigned short v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e * 32 + lane < have ? src[e * 32 + lane] : (unsigned short)0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e * 32 + lane < want) dst[e * 32 + lane] = v[e];
+        }
+    }
+}
+
 // src (rows x cols, pitch ld) -> PLANES x rows x pitch BF16, four columns per thread, for up to two matrices
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) xe_pack_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
@@ -399,6 +438,9 @@ __global__ void __launch_bounds__(256) xe_warp_rows_kernel(const float* z, int s
     pdl_wait();
     constexpr int QUADS = 4;
     __shared__ __align__(16) float block_sums[XE_WARP_ROWS][128 * QUADS];
+    __shared__ int block_live;
+    if (threadIdx.x == 0) block_live = 0;
+    __syncthreads();
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const long long warps = (long long)gridDim.x * XE_WARP_ROWS, w0 = (long long)blockIdx.x * XE_WARP_ROWS + warp;
     const long long r0 = w0 * a.n / warps, r1 = (w0 + 1) * a.n / warps, plane = a.n * zpitch;
@@ -457,8 +499,11 @@ __global__ void __launch_bounds__(256) xe_warp_rows_kernel(const float* z, int s
             }
         }
     }
-    if (lane == 0 && live) atomicAdd(a.count, live);
-    if constexpr (GRAD && PLANES > 0) {
+    // one atomic per block: thousands of warps on one address would queue for longer than the rows take
+    if (lane == 0 && live) atomicAdd(&block_live, live);
+    __syncthreads();
+    if (threadIdx.x == 0 && block_live) atomicAdd(a.count, block_live);
+    if constexpr (GRAD) {
         if (db_part) {
 #pragma unroll
             for (int q = 0; q < QUADS; ++q)
@@ -792,19 +837,22 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
 }
 
 // ---- few rows: FP32 products on the caller's matrices ----------------------------------------------------------
-// FP32X3 with up to 16 rows: the products are a read of W (twice) and a write of dW; splitting W into BF16 parts first would move it
+// FP32X3 with up to 16 rows, or up to 16 classes (for which read: x as W, and the other way round): the products are a read of
+// W (twice) and a write of dW; splitting W into BF16 parts first would move it
 // three times more, and a 256-row tensor-core tile would be mostly empty.  In all three kernels a lane owns four features,
 // 32 apart (single elements then make whole lines at any pitch and alignment), whose values of all rows (x, or the sums of dx) it
 // holds in registers as packed pairs, and a warp walks over classes, one piece of 128 features of W or dW per class.
 // ROWS (4, 8 or 16) rows cost ROWS * 4 multiplications a lane and piece, which the FP32 pipe does faster than HBM delivers it.
 constexpr int XF_ROWS = 16, XF_COLS = 128, XF_CLASSES = 128;      // most rows; features and classes of a block
 struct FewArgs {
-    const float* x; const float* w;
+    const float* x; const float* w;       // the matrix of few rows (n), and the long one (v rows); classes and rows may change
+                                          // places: then x is W, w is x, and dx and dW change places as well
     float* out;                           // z, dx or its parts, dW
     const float* dz;
     long long ldx, ldw, ldo, plane;       // plane: elements between the parts of z or dx
-    int n, d, v, dzpitch, splits;
-    const float* rowg;                    // rows of weight 0 are not read
+    long long zr, zj;                     // z and dz: elements from one row of x to the next, from one row of w to the next
+    int n, d, v, splits;
+    const float* xg; const float* wg;     // rows of x or w of weight 0 are not read, or NULL
     XeScale scale;
     int* zero;
 };
@@ -818,7 +866,7 @@ __device__ __forceinline__ void few_load_x(float2 (&xr)[ROWS][2], const FewArgs&
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         float v[4];
-        const bool in = r < p.n && !(weigh && p.rowg[r] == 0.f);
+        const bool in = r < p.n && !(weigh && p.xg && p.xg[r] == 0.f);
         few_load(v, p.x + (in ? r * p.ldx : 0), k, in ? p.d : 0);
         xr[r][0] = make_float2(v[0], v[1]);
         xr[r][1] = make_float2(v[2], v[3]);
@@ -882,7 +930,7 @@ __global__ void __launch_bounds__(128) xe_few_logits_kernel(const FewArgs p) {
     float* z = p.out + blockIdx.y * p.plane;
     for (int i = threadIdx.x; i < XF_CLASSES * p.n; i += 128) {
         const int r = i / XF_CLASSES, c = i % XF_CLASSES;
-        if (c < count) z[r * p.ldo + j0 + c] = zs[c][r];
+        if (c < count) z[r * p.zr + (j0 + c) * p.zj] = zs[c][r];
     }
 }
 
@@ -892,7 +940,7 @@ __device__ __forceinline__ void few_stage_dz(float (&ds)[XF_CLASSES][ROWS], cons
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         const int j = j0 + threadIdx.x;
-        ds[threadIdx.x][r] = r < p.n && j < p.v ? p.dz[(long long)r * p.dzpitch + j] : 0.f;
+        ds[threadIdx.x][r] = r < p.n && j < p.v ? p.dz[r * p.zr + j * p.zj] : 0.f;
     }
 }
 
@@ -920,7 +968,8 @@ __global__ void __launch_bounds__(128) xe_few_dx_kernel(const FewArgs p) {
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) {
                 const int c = c0 + 4 * q;
-                few_load(wv[q], w + (c < count ? (j0 + c) * p.ldw : 0), k, c < count ? p.d : 0);
+                const bool in = c < count && !(p.wg && p.wg[j0 + c] == 0.f);
+                few_load(wv[q], w + (in ? (j0 + c) * p.ldw : 0), k, in ? p.d : 0);
             }
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) {
@@ -1004,7 +1053,8 @@ struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
-    bool small, few;                     // FP32 arithmetic instead of tensor cores: xe_small_*, xe_few_*
+    bool small, few, few_rows;           // FP32 arithmetic instead of tensor cores: xe_small_*, xe_few_* (of rows, else of classes)
+    int splits_few;                      // of the gradient of the matrix of few rows
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
     int zpitch, piece, pieces, dzpitch, parts;
@@ -1098,10 +1148,11 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured 6.5 TB/s and 1.4 PFLOP/s the
     // product is the dearer one from d = 1000 (200) on.
     const bool few_tiles = n * v <= 64ll * XE_BM * XE_BN;
-    const long long class_tiles = (v + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
-    const int few_splits = few_split_count(class_tiles, col_tiles);
+    p.few_rows = n <= XF_ROWS;
+    const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
+    const int few_splits = few_split_count(long_tiles, col_tiles);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
-    p.few = !bf16 && !p.small && n > 0 && n <= XF_ROWS && z_bytes * few_splits <= limit;
+    p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && z_bytes * few_splits <= limit;
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
@@ -1133,10 +1184,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.splits_dx = cx.splits; p.splits_dw = cw.splits;
     p.bn_dx = cx.bn; p.bn_dw = cw.bn;
     // more than one piece adds up in floats: in dx itself, or in the scratch
-    if (p.few) {
-        p.splits_dx = few_split_count(col_tiles, class_tiles);
-        p.splits_dw = 1;
-    }
+    p.splits_few = few_split_count(col_tiles, long_tiles);
     p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
     p.dw_direct = p.splits_dw == 1;
     p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, d->v) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
@@ -1161,8 +1209,8 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     if (grad) {
         p.off_dz = take(un * p.dzpitch * 2 * p.planes);
         p.off_db = take(d->has_bias ? (size_t)p.parts * p.dzpitch * 4 : 0);
-        p.off_dx = take(p.dx_direct ? 0 : un * p.dpitch * 4 * p.splits_dx);
-        p.off_dw = take(p.dw_direct ? 0 : (size_t)p.piece * p.dpitch * 4 * p.splits_dw);
+        p.off_dx = take(p.few ? (size_t)(p.few_rows ? n : v) * p.dpitch * 4 * p.splits_few : p.dx_direct ? 0 : un * p.dpitch * 4 * p.splits_dx);
+        p.off_dw = take(p.few || p.dw_direct ? 0 : (size_t)p.piece * p.dpitch * 4 * p.splits_dw);
     }
     p.total = off + 256;
     *out = p;
@@ -1244,11 +1292,20 @@ int finish(const wino_xent_desc& d, const Plan& p, const float* buf, int splits,
     return xe_launch(xe_finish_kernel<float>, blocks, 256, 0, st, buf, splits, rows, d.d, p.dpitch, (float*)out, ld);
 }
 
-FewArgs few_args(const void* x, const void* w, const wino_xent_desc& d, const Plan& p) {
+FewArgs few_args(const void* x, const void* w, const wino_xent_desc& d, const Plan& p, const float* rowg) {
     FewArgs a = {};
-    a.x = (const float*)x; a.w = (const float*)w;
-    a.ldx = p.ldx; a.ldw = p.ldw;
-    a.n = d.n; a.d = d.d; a.v = d.v; a.dzpitch = p.zpitch;
+    a.d = d.d;
+    if (p.few_rows) {
+        a.x = (const float*)x; a.w = (const float*)w;
+        a.ldx = p.ldx; a.ldw = p.ldw;
+        a.n = d.n; a.v = d.v; a.zr = p.zpitch; a.zj = 1;
+        a.xg = rowg;
+    } else {
+        a.x = (const float*)w; a.w = (const float*)x;
+        a.ldx = p.ldw; a.ldw = p.ldx;
+        a.n = d.v; a.v = d.n; a.zr = 1; a.zj = p.zpitch;
+        a.wg = rowg;
+    }
     return a;
 }
 
@@ -1261,31 +1318,35 @@ int few_launch(int n, dim3 grid, cudaStream_t st, const FewArgs& a, Pick pick) {
 }
 
 int launch_few_logits(const void* x, const void* w, const wino_xent_desc& d, const Plan& p, float* z, int* zero, cudaStream_t st) {
-    FewArgs a = few_args(x, w, d, p);
-    a.out = z; a.ldo = p.zpitch; a.plane = (long long)d.n * p.zpitch;
+    FewArgs a = few_args(x, w, d, p, nullptr);
+    a.out = z; a.plane = (long long)d.n * p.zpitch;
     a.splits = p.splits_z;
     a.zero = zero;
-    const dim3 grid((unsigned)((d.v + XF_CLASSES - 1) / XF_CLASSES), (unsigned)a.splits);
-    return few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_logits_kernel<decltype(rows)::value>; });
+    const dim3 grid((unsigned)((a.v + XF_CLASSES - 1) / XF_CLASSES), (unsigned)a.splits);
+    return few_launch(a.n, grid, st, a, [](auto rows) { return xe_few_logits_kernel<decltype(rows)::value>; });
 }
 
 int launch_few_grad(const void* x, const void* w, void* dx, void* dw, const wino_xent_desc& d, const Plan& p, const float* dz, float* buf, const float* rowg,
                     const XeScale& scale, cudaStream_t st) {
-    FewArgs a = few_args(x, w, d, p);
-    a.dz = dz; a.rowg = rowg; a.scale = scale;
-    const unsigned kblocks = (unsigned)((d.d + XF_COLS - 1) / XF_COLS), jblocks = (unsigned)((d.v + XF_CLASSES - 1) / XF_CLASSES);
+    FewArgs a = few_args(x, w, d, p, rowg);
+    a.dz = dz; a.scale = scale;
+    const unsigned kblocks = (unsigned)((d.d + XF_COLS - 1) / XF_COLS), jblocks = (unsigned)((a.v + XF_CLASSES - 1) / XF_CLASSES);
+    void* few = p.few_rows ? dx : dw;              // the gradient of the matrix of few rows, and of the long one
+    void* full = p.few_rows ? dw : dx;
+    const long long ld_few = p.few_rows ? p.lddx : p.lddw, ld_full = p.few_rows ? p.lddw : p.lddx;
     int rc;
-    if (dx) {
-        a.out = p.dx_direct ? (float*)dx : buf; a.ldo = p.dx_direct ? p.lddx : p.dpitch; a.plane = (long long)d.n * p.dpitch;
-        a.splits = p.splits_dx;
+    if (few) {
+        const bool direct = p.splits_few == 1;
+        a.out = direct ? (float*)few : buf; a.ldo = direct ? ld_few : p.dpitch; a.plane = (long long)a.n * p.dpitch;
+        a.splits = p.splits_few;
         const dim3 grid(kblocks, (unsigned)a.splits);
-        rc = few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_dx_kernel<decltype(rows)::value>; });
-        if (rc || (!p.dx_direct && (rc = finish(d, p, buf, p.splits_dx, d.n, dx, p.lddx, st)))) return rc;
+        rc = few_launch(a.n, grid, st, a, [](auto rows) { return xe_few_dx_kernel<decltype(rows)::value>; });
+        if (rc || (!direct && (rc = finish(d, p, buf, a.splits, a.n, few, ld_few, st)))) return rc;
     }
-    if (dw) {
-        a.out = (float*)dw; a.ldo = p.lddw;
+    if (full) {
+        a.out = (float*)full; a.ldo = ld_full;
         const dim3 grid(kblocks * jblocks);
-        rc = few_launch(d.n, grid, st, a, [](auto rows) { return xe_few_dw_kernel<decltype(rows)::value>; });
+        rc = few_launch(a.n, grid, st, a, [](auto rows) { return xe_few_dw_kernel<decltype(rows)::value>; });
         if (rc) return rc;
     }
     return WINO_OK;
@@ -1330,7 +1391,11 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             ow = {ws + p.off_w, v, d.d, p.dp, v * p.dp, p.planes, false};
         }
         const unsigned blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * (p.dp / 4));
-        if (d.dtype == WINO_BF16) rc = xe_launch(xe_pack_kernel<__nv_bfloat16, 1>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
+        if (d.dtype == WINO_BF16 && ((p.pack_x && p.ldx % 8) || (p.pack_w && p.ldw % 8))) {
+            const bool pairs = !(p.pack_x && p.ldx % 2) && !(p.pack_w && p.ldw % 2);
+            const unsigned row_blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * ((p.dp + 255) / 256) * 32);
+            rc = xe_launch(pairs ? xe_pack_rows_kernel<true> : xe_pack_rows_kernel<false>, row_blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
+        } else if (d.dtype == WINO_BF16) rc = xe_launch(xe_pack_kernel<__nv_bfloat16, 1>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
         else rc = xe_launch(xe_pack_kernel<float, 3>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
         if (rc) return rc;
     }
@@ -1391,7 +1456,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             const unsigned blocks = (unsigned)row_blocks(n, d.v);
             auto rows_fn = d.v <= 512 ? launch_warp_rows : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
                          : d.v <= 4096 ? launch_rows<256, 4> : launch_rows<512, 4>;
-            if ((p.small || p.few) && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, nullptr);
+            // floats in the place of the logits; column sums where there are more rows than the products' kernels add up
+            if ((p.small || p.few) && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, p.few && !p.few_rows ? db_part : nullptr);
             else rc = rows_fn(products ? p.planes : -1, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, dz, p.dzpitch, db_part);
         }
     } else {
@@ -1422,7 +1488,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             const unsigned grid = (unsigned)((v + 255) / 256) * (unsigned)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
             if ((rc = xe_launch(xe_wide_dz_kernel<0>, grid, 128, 0, st, z, d.v, p.zpitch, n, ra.lse, ra.rowg, target, dzr, z, p.zpitch, nullptr))) return rc;
         }
-        if (db && (rc = launch_db(z, (int)n, p.zpitch, d.v, scale, db, st))) return rc;
+        if (db && (rc = p.few_rows ? launch_db(z, (int)n, p.zpitch, d.v, scale, db, st) : launch_db(db_part, p.parts, p.zpitch, d.v, scale, db, st))) return rc;
         return launch_few_grad(x, w, dx, dw, d, p, z, f(p.off_dx), ra.rowg, scale, st);
     }
     for (int i = 0; i < p.pieces; ++i) {
