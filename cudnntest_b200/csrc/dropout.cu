@@ -58,7 +58,6 @@ __device__ __forceinline__ uint32_t drop_pair(uint32_t v, uint32_t r, const Drop
 // width apart, and has all their loads in flight before the first generator runs.
 template <bool BF16, int GROUPS>
 __global__ void __launch_bounds__(DO_THREADS) dropout_vec_kernel(const void* xin, void* yout, const DropoutArgs a, long long groups_per_row) {
-    pdl_launch_dependents();
     pdl_wait();
     const long long g0 = (long long)blockIdx.x * (DO_THREADS * GROUPS) + threadIdx.x;
     const long long total = a.rows * groups_per_row;
@@ -113,7 +112,6 @@ __global__ void __launch_bounds__(DO_THREADS) dropout_vec_kernel(const void* xin
 // lane l then handles elements l, l + 32, ... so that accesses stay coalesced; the bits come over by shuffles.
 template <typename T>
 __global__ void __launch_bounds__(DO_THREADS) dropout_any_kernel(const T* x, T* y, const DropoutArgs a) {
-    pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x % 32;
     const long long warp = (long long)blockIdx.x * (DO_THREADS / 32) + threadIdx.x / 32;

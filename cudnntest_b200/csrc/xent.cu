@@ -82,7 +82,6 @@ __device__ __forceinline__ void load4f(float (&v)[4], const T* p, int left) {
 // pairs of them, where every row starts on 4 bytes), so that both sides are whole lines whatever the pitch
 template <bool PAIRS>
 __global__ void __launch_bounds__(256) xe_pack_rows_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
-    pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x % 32;
     const unsigned chunks = (unsigned)(pitch + 255) / 256;
@@ -120,7 +119,6 @@ __global__ void __launch_bounds__(256) xe_pack_rows_kernel(const PackJob j0, con
 // src (rows x cols, pitch ld) -> PLANES x rows x pitch BF16, four columns per thread, for up to two matrices
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256) xe_pack_kernel(const PackJob j0, const PackJob j1, int cols, int pitch, const RowRule rule) {
-    pdl_launch_dependents();
     pdl_wait();
     const unsigned quads = (unsigned)pitch / 4;
     const long long items0 = j0.rows * quads, total = items0 + j1.rows * quads;
@@ -211,7 +209,6 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // 32 rows x 8 threads per row over the column tiles' statistics, eight tiles in flight per thread
 __global__ void __launch_bounds__(256) xe_rows_from_stats_kernel(const float2* __restrict__ stats, const float* __restrict__ zsum,
                                                                  const float* __restrict__ zt, int tiles, const RowArgs a) {
-    pdl_launch_dependents();
     pdl_wait();
     __shared__ float2 red[8][32];
     __shared__ float redz[8][32];
@@ -342,7 +339,6 @@ __device__ __forceinline__ void store_dz(float (&d)[4], void* dz, long long n, l
 template <int THREADS, int QUADS, int PLANES, bool GRAD, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, (!SPLIT ? 1024 : QUADS > 1 ? 512 : 768) / THREADS) xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
                                                           const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
-    pdl_launch_dependents();
     pdl_wait();
     constexpr int WARPS = THREADS / 32;
     __shared__ float red[2][3][WARPS];          // two sets, used by turns: a row's second barrier frees the other set
@@ -434,7 +430,6 @@ constexpr int XE_WARP_ROWS = 8;                    // warps per block
 template <int PLANES, bool GRAD, bool SPLIT>
 __global__ void __launch_bounds__(256) xe_warp_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
                                                            const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
-    pdl_launch_dependents();
     pdl_wait();
     constexpr int QUADS = 4;
     __shared__ __align__(16) float block_sums[XE_WARP_ROWS][128 * QUADS];
@@ -526,7 +521,6 @@ constexpr int XE_CHUNK = 1024;
 __global__ void __launch_bounds__(256) xe_wide_stats_kernel(float* __restrict__ z, int splits, int v, int pitch, const float* __restrict__ bias, long long n,
                                                             const long long* __restrict__ target, float2* __restrict__ stats, float* __restrict__ zsums,
                                                             float* __restrict__ zt) {
-    pdl_launch_dependents();
     pdl_wait();
     __shared__ float red[3][8];
     const int chunks = (v + XE_CHUNK - 1) / XE_CHUNK, chunk = (int)(blockIdx.x % (unsigned)chunks);
@@ -574,7 +568,6 @@ template <int PLANES>
 __global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* z, int v, int zpitch, long long n, const float* __restrict__ lse,
                                                          const float* __restrict__ rowg, const long long* __restrict__ target, const XeDzRule rule,
                                                          void* dz, int dpitch, float* __restrict__ db_part) {
-    pdl_launch_dependents();
     pdl_wait();
     const unsigned cblocks = (unsigned)(v + 255) / 256, part = blockIdx.x / cblocks;
     const int c = (int)((blockIdx.x % cblocks) * 128 + threadIdx.x) * 2;
@@ -611,7 +604,6 @@ __global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* z, int v, 
 __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __restrict__ dz, int pitch, long long n, const float2* __restrict__ stats,
                                                              const float* __restrict__ zt, const float* __restrict__ lse, const float* __restrict__ rowg,
                                                              const long long* __restrict__ target, const XeDzRule rule) {
-    pdl_launch_dependents();
     pdl_wait();
     // a block takes 256 x 4 groups of a row at a time: one division per block, four loads in flight per thread
     const int octs = pitch / 8, spans = (octs + 1023) / 1024;
@@ -661,7 +653,6 @@ __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __re
 // per block; eight columns where there are few of them, 32 (whole lines) where there are many
 template <int COLS>
 __global__ void __launch_bounds__(512) xe_db_kernel(const float* __restrict__ part, int parts, int pitch, int cols, const XeScale scale, float* __restrict__ db) {
-    pdl_launch_dependents();
     pdl_wait();
     constexpr int RUNS = 512 / COLS;
     __shared__ float red[RUNS][COLS];
@@ -683,7 +674,6 @@ __global__ void __launch_bounds__(512) xe_db_kernel(const float* __restrict__ pa
 template <typename T>
 __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict__ part, int splits, long long rows, int cols, int pitch, T* __restrict__ out,
                                                         long long ld) {
-    pdl_launch_dependents();
     pdl_wait();
     const int quads = (cols + 3) / 4;
     const long long total = rows * quads, plane = rows * pitch;
@@ -714,7 +704,6 @@ constexpr int XE_SMALL_ROWS = 8, XE_SMALL_SLICE = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int n, int d, int v,
                                                               int zpitch, float* __restrict__ z, int* zero) {
-    pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x % 32, j = blockIdx.x * 8 + threadIdx.x / 32, r0 = blockIdx.y * XE_SMALL_ROWS;
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
@@ -772,7 +761,6 @@ struct SmallGrad {
 };
 template <typename T>
 __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a) {
-    pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(16) float coef[];            // [c][8], then [warp][8][128] sums
     if (a.loss.loss && blockIdx.x == gridDim.x - 1) {
@@ -877,7 +865,6 @@ __device__ __forceinline__ void few_load_x(float2 (&xr)[ROWS][2], const FewArgs&
 // exchange and add up in shared memory
 template <int ROWS>
 __global__ void __launch_bounds__(128) xe_few_logits_kernel(const FewArgs p) {
-    pdl_launch_dependents();
     pdl_wait();
     __shared__ float zs[XF_CLASSES][ROWS + 1];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, j0 = blockIdx.x * XF_CLASSES;
@@ -947,7 +934,6 @@ __device__ __forceinline__ void few_stage_dz(float (&ds)[XF_CLASSES][ROWS], cons
 // dx = dz W: a block takes 128 features and a part of the classes; its warps' sums meet in shared memory
 template <int ROWS>
 __global__ void __launch_bounds__(128) xe_few_dx_kernel(const FewArgs p) {
-    pdl_launch_dependents();
     pdl_wait();
     __shared__ __align__(16) float ds[XF_CLASSES][ROWS];
     __shared__ float sums[4][XF_COLS];
@@ -1009,7 +995,6 @@ __global__ void __launch_bounds__(128) xe_few_dx_kernel(const FewArgs p) {
 // dW = dz^T x: a block makes 128 classes x 128 features
 template <int ROWS>
 __global__ void __launch_bounds__(128) xe_few_dw_kernel(const FewArgs p) {
-    pdl_launch_dependents();
     pdl_wait();
     __shared__ __align__(16) float ds[XF_CLASSES][ROWS];
     const unsigned kblocks = (unsigned)(p.d + XF_COLS - 1) / XF_COLS;
@@ -1145,8 +1130,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll;
     const bool fits = z_bytes * p.splits_z + (grad ? dz_bytes : 0) <= limit;
     // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
-    // logit (18 in three parts) against 2 d flops (12 d) for another product: at the measured 6.5 TB/s and 1.4 PFLOP/s the
-    // product is the dearer one from d = 1000 (200) on.
+    // logit (18 in three parts), exponentials 6, against 2 d flops (12 d) for another product.  Measured, with gradients, kept
+    // against computed again: floats 4096 x d x 20000 BF16 d = 512 363 / 316 us, 1024 498 / 500, 2048 841 / 941; FP32X3
+    // 4096 x d x 12000 d = 128 484 / 465, 256 572 / 571, 512 891 / 995; exponentials d = 256 253 / 242, 512 303 / 304, 1024 440 / 495.
     const bool few_tiles = n * v <= 64ll * XE_BM * XE_BN;
     p.few_rows = n <= XF_ROWS;
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
@@ -1162,7 +1148,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
         p.pack_x = p.pack_w = false;
         p.splits_z = few_splits;
     } else if (few_tiles && fits) p.kept = true;
-    else if (grad && bf16 && !d->has_bias && dz_bytes <= limit) p.exps = true;
+    else if (grad && bf16 && !d->has_bias && dz_bytes <= limit && d->d >= 512) p.exps = true;
     else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
     if (!grad && p.splits_z == 1 && !p.small && !p.few) p.kept = false;          // statistics are all that is wanted
     if (!p.kept) p.splits_z = 1;
@@ -1217,8 +1203,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     return WINO_OK;
 }
 
-// Every kernel of a call is launched with programmatic serialisation and waits for its predecessor itself: its blocks are
-// set up while that one ends (five launches of the 256 x 25088 x 1000 gradient: PDL_MEASURE).
+// Every kernel of a call is launched with programmatic serialisation and waits for its predecessor itself, so that its blocks
+// are set up as that one's leave.  Measured per call: 256 x 25088 x 1000 with gradients 70.8 -> 63.6 us, 512 x 2048 x 8000
+// 85.8 -> 75.0 us.  No kernel lets its successor in any earlier: blocks that wait hold registers and shared memory (64.4 us, 83.3 us).
 template <typename... KArgs, typename... Args>
 int xe_launch(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, cudaStream_t st, Args... args) {
     count_launch();
