@@ -4,7 +4,8 @@
 //  :368-386 softmaxForward = cudnnSoftmaxForward ACCURATE / MODE_CHANNEL, :668-704 the call sequence and the arg-max;
 //  weights "vggData/fc14.bin", "fc14.bias.bin", ... as float32, [outputs][inputs], vggCUDNN.cu:39-44, :178-180).
 // It sits outside the convolution hot path: the three products are plain library GEMMs (cuBLAS, FP32), the bias /
-// ReLU / softmax / flatten steps are small kernels here.  The reference's arg-max keeps its running index across
+// ReLU / softmax / flatten steps are small kernels here.  The cross entropy of the batch (label of image i: class i modulo 1000,
+// the index the reference expects, vggCUDNN.cu:203-262) comes from wino_xent_forward on fc16's input and weights.  The reference's arg-max keeps its running index across
 // images (Network.h:690-700, `id` is never reset); here every image starts from class 0.
 #pragma once
 
@@ -82,6 +83,13 @@ struct ClassifierTail {
     float *flat = nullptr, *a14 = nullptr, *a15 = nullptr, *logits = nullptr, *prob = nullptr;
     void* nchw = nullptr;       // the last convolution output relaid out to NCHW (storage dtype)
     int* top1_d = nullptr;
+    wino_xent_desc xent = {};   // per-image cross entropy of fc16's softmax
+    long long* label_d = nullptr;
+    float* loss_d = nullptr;
+    void* xent_ws = nullptr;
+    size_t xent_bytes = 0;
+
+    int label(int img) const { return img % kOut[2]; }
 
     void init(int batch) {
         n = batch;
@@ -108,6 +116,16 @@ struct ClassifierTail {
         HCHECK_CUDA(cudaMalloc(&logits, (size_t)n * kOut[2] * 4));
         HCHECK_CUDA(cudaMalloc(&prob, (size_t)n * kOut[2] * 4));
         HCHECK_CUDA(cudaMalloc(&top1_d, n * sizeof(int)));
+        xent.n = n; xent.d = kIn[2]; xent.v = kOut[2];
+        xent.dtype = WINO_FP32X3; xent.has_bias = 1; xent.reduction = WINO_NONE;
+        xent_bytes = wino_xent_workspace_bytes(&xent, 0);
+        if (!xent_bytes) { fprintf(stderr, "libwino: %s\n", wino_last_error_string()); exit(3); }
+        std::vector<long long> labels(n);
+        for (int i = 0; i < n; ++i) labels[i] = label(i);
+        HCHECK_CUDA(cudaMalloc(&label_d, n * sizeof(long long)));
+        HCHECK_CUDA(cudaMalloc(&loss_d, n * sizeof(float)));
+        HCHECK_CUDA(cudaMalloc(&xent_ws, xent_bytes));
+        HCHECK_CUDA(cudaMemcpy(label_d, labels.data(), n * sizeof(long long), cudaMemcpyHostToDevice));
     }
 
     // y[n][out] = x[n][in] . W[out][in]^T (+ bias, optional ReLU)
@@ -137,9 +155,18 @@ struct ClassifierTail {
         HCHECK_CUDA(cudaGetLastError());
     }
 
+    // cross entropy of every image (after forward)
+    std::vector<float> losses() {
+        HCHECK_WINO(wino_xent_forward(&xent, a15, w_d[2], b_d[2], label_d, loss_d, nullptr, xent_ws, xent_bytes, nullptr));
+        HCHECK_WINO(wino_device_status());
+        std::vector<float> l(n);
+        HCHECK_CUDA(cudaMemcpy(l.data(), loss_d, n * sizeof(float), cudaMemcpyDeviceToHost));
+        return l;
+    }
+
     // Host restatement (double accumulation) of the tail for one image from the device's flattened input; returns the
-    // largest |p - p_ref| over the 1000 classes and whether the arg-max agrees.
-    double check_image(int img, bool* top1_ok) {
+    // largest |p - p_ref| over the 1000 classes, whether the arg-max agrees, and the image's cross entropy.
+    double check_image(int img, bool* top1_ok, double* loss = nullptr) {
         std::vector<float> x(kIn[0]), p(kOut[2]);
         HCHECK_CUDA(cudaMemcpy(x.data(), flat + (size_t)img * kIn[0], x.size() * 4, cudaMemcpyDeviceToHost));
         HCHECK_CUDA(cudaMemcpy(p.data(), prob + (size_t)img * kOut[2], p.size() * 4, cudaMemcpyDeviceToHost));
@@ -165,6 +192,7 @@ struct ClassifierTail {
         double worst = 0;
         for (int i = 0; i < kOut[2]; ++i) worst = std::fmax(worst, std::fabs(std::exp(cur[i] - mx) / sum - (double)p[i]));
         *top1_ok = arg == dev_top1;
+        if (loss) *loss = mx + std::log(sum) - cur[label(img)];
         return worst;
     }
 

@@ -15,7 +15,7 @@
 // block-end pooling as its own pass, wino_maxpool2x2, the way the reference sequences it, Network.h:314-366, :603-669).  With tail=1 the classifier tail of the
 // reference (fc14 + ReLU, fc15 + ReLU, fc16, softmax, arg-max: Network.h:668-704) runs after the last round on the
 // output of conv13 (classifier_tail.h: cuBLAS GEMMs + small kernels), is checked against a host restatement for two
-// images and reports the top-1 classes.  The pretrained weights (./vggData/*.bin) and ImageNet batches the reference
+// images and reports the top-1 classes and the batch's cross entropy (wino_xent_forward).  The pretrained weights (./vggData/*.bin) and ImageNet batches the reference
 // reads are not shipped; they are used if present, otherwise weights are seeded He-normal and the input
 // uniform[-1,1] (so the classes mean nothing, the arithmetic is what is checked).  Prints "time:<ms> ms" per round
 // and a JSON summary.
@@ -241,14 +241,21 @@ int main(int argc, char** argv) {
         float tail_ms;
         HCHECK_CUDA(cudaEventElapsedTime(&tail_ms, e0, e1));
         bool ok0 = false, ok1 = false;
-        const double err0 = ct.check_image(0, &ok0), err1 = ct.check_image(n - 1, &ok1);
+        double loss0 = 0, loss1 = 0;
+        const double err0 = ct.check_image(0, &ok0, &loss0), err1 = ct.check_image(n - 1, &ok1, &loss1);
+        const std::vector<float> losses = ct.losses();
+        double mean_loss = 0;
+        for (float l : losses) mean_loss += l / n;
+        const double lerr0 = std::fabs(losses[0] - loss0) / (1 + std::fabs(loss0)), lerr1 = std::fabs(losses[n - 1] - loss1) / (1 + std::fabs(loss1));
         const std::vector<int> top1 = ct.top1();
         for (int i = 0; i < n && i < 8; ++i) printf("Batch %d Resulting weights from Softmax:%d\n", i, top1[i]);
         char buf[512];
-        snprintf(buf, sizeof(buf), ", \"tail_ms\": %.4f, \"tail_weights\": \"%s\", \"tail_max_abs_err\": %.3e, \"tail_top1_agree\": %s, \"top1_first\": %d",
-                 tail_ms, ct.from_files ? "vggData/*.bin" : "seeded", err0 > err1 ? err0 : err1, (ok0 && ok1) ? "true" : "false", top1[0]);
+        snprintf(buf, sizeof(buf), ", \"tail_ms\": %.4f, \"tail_weights\": \"%s\", \"tail_max_abs_err\": %.3e, \"tail_top1_agree\": %s, \"top1_first\": %d, "
+                 "\"tail_loss\": %.6f, \"tail_loss_max_err\": %.3e",
+                 tail_ms, ct.from_files ? "vggData/*.bin" : "seeded", err0 > err1 ? err0 : err1, (ok0 && ok1) ? "true" : "false", top1[0], mean_loss,
+                 lerr0 > lerr1 ? lerr0 : lerr1);
         tail_json = buf;
-        if (!(err0 <= 1e-4 && err1 <= 1e-4)) printf("classifier tail error\n");
+        if (!(err0 <= 1e-4 && err1 <= 1e-4 && lerr0 <= 1e-4 && lerr1 <= 1e-4)) printf("classifier tail error\n");
     }
     printf("{\"harness\": \"netTest\", \"mode\": %d, \"batch\": %d, \"layout\": \"%s\", \"dtype\": \"%s\", \"ms_avg\": %.4f, \"ms_min\": %.4f, "
            "\"images_per_s\": %.1f, \"tflops_direct_equiv\": %.2f, \"what\": \"%s\"%s}\n",

@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from .conv import WinoConv, act_shape, make_desc
+from .head import LinearXent, dropout, dropout_backward
 
 # (input channels, filters, input side, pool after)
 VGG16_CONV = [
@@ -148,3 +149,41 @@ class VGG16ConvStack:
             y = self.forward(x)
         self.launches_per_forward = _lib.lib().wino_launch_count() - before
         return graph, y
+
+
+class ClassifierHead:
+    """A linear classifier on the stack's output: dropout, one fully connected layer, softmax cross entropy.
+
+    What a program fits on frozen convolutions, and the last layer of the reference's network (fc16 + softmax,
+    netTest/cudnn_test_0124/VGG_Batched/Network.h:668-704) with the dropout that its training puts before it.  Takes the
+    output of ``VGG16ConvStack`` as it comes, flattened per image in the stack's NHWC or NCHW order (CHWN has the images
+    innermost: relay it out first).  Weights are seeded; ``weight`` (classes, features) and ``bias`` may be overwritten."""
+
+    def __init__(self, batch, features, classes, dtype="bf16", p=0.5, ignore_index=None, label_smoothing=0.0, seed=0xC0DE0041,
+                 device="cuda"):
+        self.batch, self.features, self.classes, self.p, self.seed, self.steps = batch, features, classes, p, seed, 0
+        common = dict(dtype=dtype, bias=True, reduction="mean", ignore_index=ignore_index, label_smoothing=label_smoothing, device=device)
+        self.plan = LinearXent(batch, features, classes, **common)
+        self.eval_plan = LinearXent(batch, features, classes, grad=False, workspace=self.plan.workspace, **common)
+        gen = torch.Generator(device="cpu").manual_seed(seed)
+        self.weight = (torch.randn((classes, features), generator=gen) * math.sqrt(1.0 / features)).to(self.plan.io_dtype).to(device)
+        self.bias = torch.zeros(classes, dtype=torch.float32, device=device)
+
+    def _flat(self, features):
+        x = features.reshape(self.batch, -1)
+        if x.shape[1] != self.features:
+            raise ValueError("%d features per image, the head was made for %d" % (x.shape[1], self.features))
+        return x
+
+    def loss(self, features, target):
+        """Mean cross entropy, without dropout."""
+        return self.eval_plan.forward(self._flat(features), self.weight, target, self.bias)[0]
+
+    def loss_and_grad(self, features, target, need_dx=False):
+        """(loss, gradient of the features or None, of the weight, of the bias); every call draws its own dropout mask."""
+        x, step = self._flat(features), self.steps
+        self.steps += 1
+        h = dropout(x, self.p, self.seed, step)
+        loss, dh, dw, db = self.plan.loss_and_grad(h, self.weight, target, self.bias, need_dx=need_dx)
+        dx = dropout_backward(dh, self.p, self.seed, step, out=dh).view(features.shape) if need_dx else None
+        return loss, dx, dw, db

@@ -520,3 +520,55 @@ def test_gradient_against_differences(n, d, v):
         third = ((2 * zu.max(1)) ** 3).sum()
         moved_rounding = 2 * F32 * float(base.abs().max()) / h * float(grad.abs().sum())
         assert abs(got - want) <= h * h * third + row / h + moved_rounding + 1e-5 * abs(want), which
+
+
+# ---- where the framework itself calls them -----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "fp32x3"])
+@pytest.mark.parametrize("layout", ["NHWC", "NCHW"])
+def test_classifier_head_on_the_convolution_stack(dtype, layout):
+    """The stack's features through the head: loss and gradients against the definition on those features; the mask of a
+    call follows from its number."""
+    torch = _torch()
+    from cudnntest_b200 import vgg
+    layers = [(3, 64, 16, False), (64, 64, 16, True), (64, 128, 8, True)]
+    stack = vgg.VGG16ConvStack(20, layout=layout, dtype=dtype, layers=layers)
+    head_ = vgg.ClassifierHead(20, 128 * 4 * 4, 30, dtype=dtype, ignore_index=-1, label_smoothing=0.1)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(stack.in_shape, generator=gen, device="cuda").to(stack.io_dtype)
+    feats = stack(x).clone()
+    target = torch.arange(20, device="cuda")
+    target[4] = -1
+    plain = head_.loss(feats, target)
+    for step in range(2):
+        loss, dx, dw, db = head_.loss_and_grad(feats, target, need_dx=True)
+        keep = head.dropout_keep(0, feats.numel(), 0.5, head_.seed, step).reshape(20, -1)
+        flat = feats.reshape(20, -1)
+        c = Case.__new__(Case)
+        c.n, c.d, c.v, c.dtype, c.ignore_index = 20, 2048, 30, "bf16" if dtype == "bf16" else "fp32", -1
+        c.t = target.cpu().numpy()
+        c.x = flat * torch.from_numpy(keep).cuda() * 2
+        c.w, c.bias = head_.weight, head_.bias
+        counts = c.t != -1
+        ref = c.oracle("mean", smoothing=0.1)
+        dh = dx.reshape(20, -1).double() / 2                     # exact: dropout's factor at p = 1/2
+        back = torch.from_numpy(keep).cuda()
+        assert (dh[~back] == 0).all()
+        ref_dx = ref["dx"]
+        ref["dx"] = np.where(keep, ref_dx, 0.0)
+        c.check((loss, dh, dw, db), ref, "mean", counts / counts.sum(), smoothing=0.1)
+    assert head_.steps == 2 and torch.isfinite(plain)
+    assert head_.loss_and_grad(feats, target)[1] is None
+    with pytest.raises(ValueError):
+        head_.loss(feats[:, :1], target)
+
+
+def test_net_test_reports_the_cross_entropy():
+    """netTest tail=1: the batch's cross entropy from the library agrees with the harness's restatement in double."""
+    import json
+    import os
+    import subprocess
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cudnntest_b200", "harness", "bin", "netTest")
+    out = subprocess.run([exe, "set", "batch=3", "mode=1", "dtype=bf16", "rounds=1", "tail=1"], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "classifier tail error" not in out.stdout, out.stdout + out.stderr
+    s = json.loads([l for l in out.stdout.splitlines() if l.startswith("{")][-1])
+    assert s["tail_loss"] > 0 and s["tail_loss_max_err"] <= 1e-4
