@@ -178,7 +178,8 @@ int run_dropout(const char* what, int dtype, long long rows, long long cols, lon
     a.threshold_hi = t << 16;
     a.scale = t < 65536u ? (float)(65536.0 / (65536.0 - t)) : 0.f;
     if (t >= 65536u) {              // nothing is kept, and T << 16 has no room for it
-        WINO_CUDA_CHECK(cudaMemset2DAsync(y, (size_t)ldy * es, 0, (size_t)cols * es, (size_t)rows, st));
+        if (rows == 1 || ldy == cols) WINO_CUDA_CHECK(cudaMemsetAsync(y, 0, (size_t)rows * cols * es, st));
+        else WINO_CUDA_CHECK(cudaMemset2DAsync(y, (size_t)ldy * es, 0, (size_t)cols * es, (size_t)rows, st));
         return WINO_OK;
     }
     const bool dense = ldx == cols && ldy == cols;

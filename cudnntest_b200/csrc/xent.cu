@@ -1080,7 +1080,7 @@ struct Cut {
     double us;
 };
 Cut cut_product(long long rows, long long cols, long long chunks, int products, bool join) {
-    const long long pairs = sm_count() / 2;
+    const long long pairs = sm_count() < 4 ? 1 : sm_count() / 2;
     const double part_us = (double)rows * (double)cols * 8.0 / 5e6;
     Cut best = {1, XE_BN, 1e30};
     if (rows == 0) return best;
@@ -1156,7 +1156,8 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.piece = d->v;
     p.pieces = 1;
     if (grad && !p.kept && !p.exps) {
-        long long most = limit / (n > 0 ? n * 2 * p.planes : 1) / XE_BN * XE_BN;
+        // dz, and partial column sums of 32 rows each
+        long long most = limit / (n > 0 ? n * 2 * p.planes + (d->has_bias ? n / 8 : 0) : 1) / XE_BN * XE_BN;
         if (most < XE_BN) most = XE_BN;
         if (most < v) {
             p.pieces = (int)((v + most - 1) / most);
@@ -1351,6 +1352,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     if (db && !d.has_bias) return fail(WINO_E_BADARG, "xent: gradient of a bias the descriptor does not have");
     if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)bias | (uintptr_t)dx | (uintptr_t)dw | (uintptr_t)workspace) & 15)
         return fail(WINO_E_BADARG, "xent: matrices, bias and workspace must be 16-byte aligned");
+    if ((dx && (dx == x || dx == w)) || (dw && (dw == x || dw == w || dw == dx))) return fail(WINO_E_BADARG, "xent: a result in the place of another matrix");
     if (((uintptr_t)target & 7) || (((uintptr_t)loss | (uintptr_t)lse | (uintptr_t)dloss | (uintptr_t)db) & 3)) return fail(WINO_E_BADARG, "xent: misaligned pointer");
     if (!workspace || workspace_bytes < p.total) return fail(WINO_E_WORKSPACE, "xent: workspace of %zu bytes, %zu needed", workspace_bytes, p.total);
     if ((rc = check_device())) return rc;
@@ -1512,6 +1514,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             q.bn = bn;
             q.out.scale = scale;
             q.out.add = add;
+            q.out.exact = direct;
             q.out.ptr = direct ? out : buf;
             q.out.pitch = direct ? ld : p.dpitch;
             const long long chunks = (k + XE_BK - 1) / XE_BK;          // a short last piece adds to fewer of the parts

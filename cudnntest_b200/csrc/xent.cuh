@@ -86,6 +86,7 @@ struct XeOutput {
     long long pitch = 0;
     int splits = 1;                 // parts of the contraction, one buffer each (XE_F32)
     bool add = false;               // XE_F32: add instead of store
+    bool exact = false;             // nothing behind a row's last column may be written
     XeScale scale;                  // XE_F32, XE_BF16: what the product is multiplied by
     // XE_STATS*, XE_DZ
     const float* bias = nullptr;    // of column 0 of this product

@@ -124,6 +124,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// ties registers that tcgen05.ld fills to the wait before this: no use of them can be moved ahead of it
+__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                      "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+
 __device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -364,12 +370,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
 #pragma unroll
                     for (int j = 0; j < WCOLS / 32; ++j) tmem_ld_32x32(tsrc + j * 32, *reinterpret_cast<uint32_t(*)[32]>(&z[32 * j]));
                     tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < WCOLS / 16; ++j) after_wait(*reinterpret_cast<uint32_t(*)[16]>(&z[16 * j]));
                 } else {
 #pragma unroll
                     for (int j = 0; j < WCOLS / 16; ++j) {
                         uint32_t r[16];
                         tmem_ld_32x16(tsrc + j * 16, r);
                         tmem_ld_wait();
+                        after_wait(r);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) z[16 * j + i] += __uint_as_float(r[i]);
                     }
@@ -629,7 +638,7 @@ int run(const XeParams& p, cudaStream_t st) {
     });
     WINO_CUDA_CHECK(attr_err);
     const long long total = (long long)p.prob[0].units + p.prob[1].units;
-    const long long pairs = total < sm_count() / 2 ? total : sm_count() / 2;
+    const long long most = sm_count() < 4 ? 1 : sm_count() / 2, pairs = total < most ? total : most;
     count_launch();
     WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES, BN>, dim3((unsigned)(2 * pairs)), dim3(XE_THREADS), L::TOTAL, st, true, p));
     return WINO_OK;
@@ -651,7 +660,8 @@ int make_problem(const XeProduct& x, XeProblem* out) {
     if ((rc = operand_map(&p.tm_a, x.a, 128)) || (rc = operand_map(&p.tm_b, x.b, (unsigned)x.bn / 2))) return rc;
     const bool f32 = x.epi == XE_F32 || x.epi == XE_STATS_Z;
     const int es = f32 ? 4 : 2;
-    p.plain = x.epi != XE_STATS && (o.pitch * es) % 16 != 0;
+    // a TMA store fills a row's last 16-byte unit with zeros behind the last column (measured), and wants such units as pitch
+    p.plain = x.epi != XE_STATS && ((o.pitch * es) % 16 != 0 || (o.exact && (x.n * es) % 16 != 0));
     if (p.plain && (o.splits > 1 || x.epi > XE_BF16)) return fail(WINO_E_BADARG, "xent: buffer rows must be multiples of 16 bytes");
     if (x.epi == XE_STATS || p.plain) {
         p.tm_out = p.tm_a;
@@ -715,7 +725,7 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
         // ring slots of a unit, and about six more for its epilogue; the product with the longer units goes first
         auto cost = [](const XeProblem& q) { return (double)q.kchunks / q.splits * q.pairs + 6.0; };
         if (cost(p.prob[0]) < cost(p.prob[1])) { const XeProblem t = p.prob[0]; p.prob[0] = p.prob[1]; p.prob[1] = t; }
-        const long long pairs = sm_count() / 2, over = (long long)p.prob[0].units % pairs;
+        const long long pairs = sm_count() < 4 ? 1 : sm_count() / 2, over = (long long)p.prob[0].units % pairs;
         if (over) {
             const long long lead = (long long)(cost(p.prob[0]) / cost(p.prob[1]) + 0.5), most = p.prob[1].units / (pairs - over);
             p.lead = (int)(lead < most ? lead : most);

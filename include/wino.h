@@ -169,7 +169,9 @@ int wino_dropout_backward(int dtype, long long rows, long long cols, long long l
  *   lse_i = log sum_j exp z_ij,   loss_i = lse_i - (1 - s) z_i,t(i) - s/v sum_j z_ij        (s = label_smoothing)
  *   dz_ij = g_i (exp(z_ij - lse_i) - (1 - s) [j = t(i)] - s/v),  dx = dz W,  dW = dz^T x,  dbias = sum_i dz_i
  * x (n, d), W (v, d), dx, dW: row-major with pitches ldx, ldw, lddx, lddw; bias, dbias: v floats; target: n 64-bit
- * integers.  WINO_MEAN divides by the number of rows that count (0 rows: loss and gradients are 0). */
+ * integers.  WINO_MEAN divides by the number of rows that count (0 rows: loss and gradients are 0).  The tensors live on the
+ * current device; results overlap neither inputs nor each other.  Calls with the same workspace are kept on one stream or
+ * otherwise serialised; the first call on a device comes before any stream capture. */
 enum { WINO_MEAN = 0, WINO_SUM = 1, WINO_NONE = 2 };
 typedef struct wino_xent_desc {
     int n, d, v;               /* rows (0 allowed), features, classes                                               */
@@ -184,9 +186,9 @@ typedef struct wino_xent_desc {
     long long ignore_index;    /* any value; may also be a class                                                    */
     float label_smoothing;     /* 0 ... 1                                                                           */
     long long ldx, ldw, lddx, lddw;   /* pitches in elements, 0 = d.  Base addresses: 16-byte aligned               */
-    long long scratch_limit;   /* bytes of scratch that may grow with n * v; 0 = 1 GiB.  Beyond it the gradient is
-                                  computed in pieces of the vocabulary (at least 256 classes each) whose logits are
-                                  computed again                                                                    */
+    long long scratch_limit;   /* bytes of scratch that may grow with n * v, beside the statistics of the logits (n v / 16
+                                  bytes, n v 3 / 32 with label_smoothing); 0 = 1 GiB.  Beyond it the gradient is computed in
+                                  pieces of the vocabulary (at least 256 classes each) whose logits are computed again      */
 } wino_xent_desc;
 
 /* Scratch of wino_xent_forward (grad = 0) or wino_xent_grad (grad = 1); 0 for a bad descriptor. */

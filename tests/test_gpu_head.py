@@ -302,8 +302,8 @@ def test_no_rows():
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-@pytest.mark.parametrize("n,d,v", [(300, 200, 700), (2305, 40, 2100), (14, 201, 7000), (100, 60, 100), (300, 201, 10)])
-@pytest.mark.parametrize("pad", [0, 1, 8])
+@pytest.mark.parametrize("n,d,v", [(300, 200, 700), (2305, 40, 2100), (14, 201, 7000), (100, 60, 100), (300, 201, 10), (300, 206, 700)])
+@pytest.mark.parametrize("pad", [0, 1, 2, 8])
 def test_outputs_stay_inside_their_rows(dtype, n, d, v, pad):
     """dx and dw inside wider buffers with guard rows: nothing but the results is written; left-out products cost nothing."""
     torch = _torch()

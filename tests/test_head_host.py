@@ -113,6 +113,7 @@ def _grad_args(L, s, **kw):
     (dict(x=None), cb._lib.E_BADARG), (dict(w=None), cb._lib.E_BADARG), (dict(target=None), cb._lib.E_BADARG), (dict(loss=None), cb._lib.E_BADARG),
     (dict(x=(1 << 20) + 2), cb._lib.E_BADARG), (dict(dx=(1 << 24) + 8), cb._lib.E_BADARG), (dict(dw=(1 << 24) + 8), cb._lib.E_BADARG),
     (dict(target=(1 << 22) + 4), cb._lib.E_BADARG), (dict(loss=(1 << 23) + 2), cb._lib.E_BADARG), (dict(db=1 << 27), cb._lib.E_BADARG),
+    (dict(dx=1 << 20), cb._lib.E_BADARG), (dict(dw=1 << 21), cb._lib.E_BADARG), (dict(dw=1 << 24), cb._lib.E_BADARG),
     (dict(ws=None), cb._lib.E_WORKSPACE), (dict(bytes=1000), cb._lib.E_WORKSPACE), (dict(ws=(1 << 26) + 4), cb._lib.E_BADARG),
 ])
 def test_xent_call_refusals(kw, code):
