@@ -611,38 +611,44 @@ __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __re
         const long long r = b / spans;
         const int o0 = (int)(b - r * spans) * 1024 + threadIdx.x;
         uint4* at = reinterpret_cast<uint4*>(dz + r * pitch);
-        const float g = rowg[r], l = lse[r];
-        const long long t = target[r];
-        uint4 q[4];
+        uint4 q[4];                                       // everything that is read is asked for at once
         float f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int o = o0 + i * 256;
-            if (o < octs && g != 0.f) {
+            if (o < octs) {
                 q[i] = at[o];
-                f[i] = stats[(long long)(o / (XE_STAT_COLS / 8)) * n + r].x;
+                f[i] = __ldg(&stats[(long long)(o / (XE_STAT_COLS / 8)) * n + r].x);
             }
         }
-        const float pt = g != 0.f ? g * (xe_ex2((zt[r] - l) * XE_LOG2E) * rule.pf - rule.smooth_all - rule.smooth_t) : 0.f;
+        const float g = __ldg(rowg + r), l = __ldg(lse + r), z_t = __ldg(zt + r);
+        const int t = (int)__ldg(target + r), to = t >> 3;
+        if (g == 0.f) {                                   // a row that does not count
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (o0 + i * 256 < octs) at[o0 + i * 256] = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        const float gp = g * rule.pf, ga = g * rule.smooth_all;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int o = o0 + i * 256;
-            if (o >= octs) continue;
-            if (g == 0.f) { at[o] = make_uint4(0, 0, 0, 0); continue; }
-            const float h = xe_ex2((f[i] - l) * XE_LOG2E) * rule.pf;
+            if (o >= octs) break;
+            const float h = xe_ex2((f[i] - l) * XE_LOG2E) * gp;
             uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const __nv_bfloat162 v = __floats2bfloat162_rn((__uint_as_float(w[e] << 16) * h - rule.smooth_all) * g,
-                                                               (__uint_as_float(w[e] & 0xffff0000u) * h - rule.smooth_all) * g);
+                const float2 z = __ffma2_rn(make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), make_float2(h, h),
+                                            make_float2(-ga, -ga));
+                const __nv_bfloat162 v = __floats2bfloat162_rn(z.x, z.y);
                 w[e] = *reinterpret_cast<const uint32_t*>(&v);
             }
-            if (t >> 3 == o) {                            // the target's own value
+            if (o == to) {                                // the target's own value
+                const float pt = xe_ex2((z_t - l) * XE_LOG2E) * gp - ga - g * rule.smooth_t;
                 const uint32_t b16 = __bfloat16_as_ushort(__float2bfloat16_rn(pt));
-                const int e = (int)(t & 7);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (e >> 1 == k) w[k] = e & 1 ? (w[k] & 0xffffu) | b16 << 16 : (w[k] & 0xffff0000u) | b16;
+                    if ((t & 7) >> 1 == k) w[k] = t & 1 ? (w[k] & 0xffffu) | b16 << 16 : (w[k] & 0xffff0000u) | b16;
             }
             at[o] = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -1490,7 +1496,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             if (p.planes == 1) rc = xe_launch(xe_wide_dz_kernel<1>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
             else rc = xe_launch(xe_wide_dz_kernel<3>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
         } else if (p.exps) {
-            rc = xe_launch(xe_dz_from_exp_kernel, loop_blocks(n * ((p.dzpitch / 8 + 1023) / 1024) * 256), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt, ra.lse, ra.rowg, target, dzr);
+            const long long spans = n * ((p.dzpitch / 8 + 1023) / 1024);
+            rc = xe_launch(xe_dz_from_exp_kernel, (unsigned)(spans < 0x7fffffffll ? spans : 0x7fffffffll), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt, ra.lse, ra.rowg, target, dzr);
         } else if (!p.kept) {
             XeProduct pd = {XE_DZ, ox, wp, n, vc, d.d, XeOutput()};
             pd.out.ptr = dz; pd.out.pitch = p.dzpitch;
