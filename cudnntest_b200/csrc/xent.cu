@@ -707,27 +707,23 @@ __global__ void __launch_bounds__(256) xe_finish_kernel(const float* __restrict_
 // 18.5 / 24.7, with 1000 of them 65 against 29.
 // logits: a warp multiplies one class with eight rows, lanes along the features; blockIdx.z: part of the features
 constexpr int XE_SMALL_ROWS = 8, XE_SMALL_SLICE = 2048;
+constexpr int XE_SMALL_MAX = 128;                  // most rows and classes of the plain gradient
+// acc[r] = sum over features k0 ... k1 - 1 of class j's weights with row r0 + r, lanes along the features; every lane gets the sums
 template <typename T>
-__global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int n, int d, int v,
-                                                              int zpitch, float* __restrict__ z, int* zero) {
-    pdl_wait();
-    const int lane = threadIdx.x % 32, j = blockIdx.x * 8 + threadIdx.x / 32, r0 = blockIdx.y * XE_SMALL_ROWS;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
-    if (j >= v) return;
-    const int k0 = blockIdx.z * XE_SMALL_SLICE, k1 = k0 + XE_SMALL_SLICE < d ? k0 + XE_SMALL_SLICE : d;
-    const bool aligned = ldx % 4 == 0 && ldw % 4 == 0;         // the bases are
+__device__ __forceinline__ void small_dots(float (&acc)[XE_SMALL_ROWS], const T* __restrict__ x, long long ldx, const T* __restrict__ wj, bool aligned,
+                                           int r0, int n, int k0, int k1, int lane) {
     const T* row[XE_SMALL_ROWS];                               // rows past the last read it again
 #pragma unroll
-    for (int r = 0; r < XE_SMALL_ROWS; ++r) row[r] = x + (long long)(r0 + r < n ? r0 + r : n - 1) * ldx;
-    float acc[XE_SMALL_ROWS];
-#pragma unroll
-    for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] = 0.f;
+    for (int r = 0; r < XE_SMALL_ROWS; ++r) {
+        row[r] = x + (long long)(r0 + r < n ? r0 + r : n - 1) * ldx;
+        acc[r] = 0.f;
+    }
     if (aligned && (k1 - k0) % 4 == 0) {
         // whole vectors: nine loads in flight per step, two steps
 #pragma unroll 2
         for (int k = k0 + lane * 4; k < k1; k += 128) {
             float a[4], b[XE_SMALL_ROWS][4];
-            load4_aligned(a, w + j * ldw + k);
+            load4_aligned(a, wj + k);
 #pragma unroll
             for (int r = 0; r < XE_SMALL_ROWS; ++r) load4_aligned(b[r], row[r] + k);
 #pragma unroll
@@ -736,23 +732,98 @@ __global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restric
     } else {
 #pragma unroll 4
         for (int k = k0 + lane; k < k1; k += 32) {
-            const float a = to_float<T>(w[j * ldw + k]);
+            const float a = to_float<T>(wj[k]);
 #pragma unroll
             for (int r = 0; r < XE_SMALL_ROWS; ++r) acc[r] += a * to_float<T>(row[r][k]);
         }
     }
 #pragma unroll
-    for (int r = 0; r < XE_SMALL_ROWS; ++r) {
+    for (int r = 0; r < XE_SMALL_ROWS; ++r)
 #pragma unroll
         for (int s = 16; s >= 1; s >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) xe_small_logits_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int n, int d, int v,
+                                                              int zpitch, float* __restrict__ z, int* zero) {
+    pdl_wait();
+    const int lane = threadIdx.x % 32, j = blockIdx.x * 8 + threadIdx.x / 32, r0 = blockIdx.y * XE_SMALL_ROWS;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x < 2) zero[threadIdx.x] = 0;
+    if (j >= v) return;
+    const int k0 = blockIdx.z * XE_SMALL_SLICE, k1 = k0 + XE_SMALL_SLICE < d ? k0 + XE_SMALL_SLICE : d;
+    float acc[XE_SMALL_ROWS];
+    small_dots(acc, x, ldx, w + j * ldw, ldx % 4 == 0 && ldw % 4 == 0, r0, n, k0, k1, lane);     // the bases are aligned
+#pragma unroll
+    for (int r = 0; r < XE_SMALL_ROWS; ++r)
         if (lane == r && r0 + r < n) z[((long long)blockIdx.z * n + r0 + r) * zpitch + j] = acc[r];
+}
+
+// Up to 128 classes that a block's 16 warps multiply in a few steps: logits, statistics and dz of eight rows in one kernel.  One
+// launch fewer is 3.5 us of host time of a call that takes about 17.  A block that is the only one (n <= 8) sums the losses too.
+constexpr int XE_TINY_WARPS = 16, XE_TINY_STEPS = 24;
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(32 * XE_TINY_WARPS) xe_tiny_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ w, long long ldw, int d, int v,
+                                                                     int zpitch, const float* __restrict__ bias, const RowArgs a, const XeDzRule rule,
+                                                                     float* __restrict__ dz) {
+    pdl_wait();
+    __shared__ float z[XE_SMALL_ROWS][XE_SMALL_MAX + 1];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r0 = blockIdx.x * XE_SMALL_ROWS, n = (int)a.n;
+    const bool aligned = ldx % 4 == 0 && ldw % 4 == 0;
+    for (int j = warp; j < v; j += XE_TINY_WARPS) {
+        float acc[XE_SMALL_ROWS];
+        small_dots(acc, x, ldx, w + j * ldw, aligned, r0, n, 0, d, lane);
+        const float b = bias ? bias[j] : 0.f;
+#pragma unroll
+        for (int r = 0; r < XE_SMALL_ROWS; ++r)
+            if (lane == r) z[r][j] = acc[r] + b;
+    }
+    __syncthreads();
+    const long long row = r0 + warp;
+    const bool mine = warp < XE_SMALL_ROWS && row < n, counts = mine && row_counts(a.rule, a.target[row]);
+    if (mine) {
+        const int t = counts ? (int)a.target[row] : -1;
+        float e[4], m = -INFINITY, s = 0.f, zsum = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = q * 32 + lane;
+            e[q] = c < v ? z[warp][c] : -INFINITY;
+            if (c < v) zsum += e[q];
+            m = fmaxf(m, e[q]);
+        }
+#pragma unroll
+        for (int h = 16; h >= 1; h >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, h));
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s += xe_ex2((e[q] - ref) * XE_LOG2E);
+#pragma unroll
+        for (int h = 16; h >= 1; h >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, h);
+            zsum += __shfl_xor_sync(0xffffffffu, zsum, h);
+        }
+        const float lse = m + logf(s);
+        if (lane == 0) finish_row(a, row, lse, zsum, counts ? z[warp][t] : 0.f);
+        if constexpr (GRAD) {
+            const float g = counts ? (a.dloss ? a.dloss[row] : 1.f) : 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = q * 32 + lane;
+                float v1 = xe_ex2((e[q] - lse) * XE_LOG2E) * rule.pf - rule.smooth_all;
+                if (c == t) v1 -= rule.smooth_t;
+                if (c < v) dz[row * zpitch + c] = g == 0.f ? 0.f : v1 * g;       // a row that does not count: exactly 0, whatever its logits
+            }
+        }
+    }
+    if (a.loss.loss) {
+        const int live = __syncthreads_count(counts && lane == 0);
+        if (threadIdx.x == 0) a.count[0] = live;
+        __syncthreads();
+        xe_sum_losses<32 * XE_TINY_WARPS>(a.loss);
     }
 }
 
 // out[o][k] = scale sum_c coef(o, c) M[c][k]: dx (o rows, c classes, M = W) and dW (o classes, c rows, M = x; and dbias),
 // from dz in floats.  A block makes eight o by 128 k; its eight warps share the sum over c, whose coefficients sit in
 // shared memory.  A row that does not count has nothing but zeros there and is not read.
-constexpr int XE_SMALL_MAX = 128;                  // most rows, most classes
 constexpr int XE_SMALL_GRAD_SMEM = 8 * 8 * 128 * 4;
 template <typename T>
 struct SmallGrad {
@@ -764,12 +835,18 @@ struct SmallGrad {
     int n, d, v, dzpitch, kblocks, dx_blocks;
     XeScale scale;
     XeLoss loss;                      // summed by the last block
+    RowRule rule;                     // n <= 256: every block counts the rows itself
+    const long long* target;
+    int* count;
 };
 template <typename T>
 __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a) {
     pdl_wait();
     extern __shared__ __align__(16) float coef[];            // [c][8], then [warp][8][128] sums
+    const int live = __syncthreads_count((int)threadIdx.x < a.n && row_counts(a.rule, a.target[threadIdx.x]));
     if (a.loss.loss && blockIdx.x == gridDim.x - 1) {
+        if (threadIdx.x == 0) *a.count = live;
+        __syncthreads();
         xe_sum_losses<256>(a.loss);
         return;
     }
@@ -783,7 +860,7 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
         coef[c * 8 + o] = in ? a.dz[(long long)(is_dw ? c : o0 + o) * a.dzpitch + (is_dw ? o0 + o : c)] : 0.f;
     }
     __syncthreads();
-    const float scale = xe_scale(a.scale);
+    const float scale = xe_scale(a.scale, live);
     if (is_dw && a.db && k < 128 && threadIdx.x < 8 && o0 + threadIdx.x < outs) {
         float s = 0.f;
         for (int c = 0; c < len; ++c) s += coef[c * 8 + threadIdx.x];
@@ -1044,7 +1121,7 @@ struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
-    bool small, few, few_rows;           // FP32 arithmetic instead of tensor cores: xe_small_*, xe_few_* (of rows, else of classes)
+    bool tiny, small, few, few_rows;           // FP32 arithmetic instead of tensor cores: xe_tiny_kernel, xe_small_*, xe_few_* (of rows, else of classes)
     int splits_few;                      // of the gradient of the matrix of few rows
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
@@ -1145,6 +1222,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const int few_splits = few_split_count(long_tiles, col_tiles);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
     p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && z_bytes * few_splits <= limit;
+    p.tiny = p.small && v <= XE_SMALL_MAX && (v + XE_TINY_WARPS - 1) / XE_TINY_WARPS * ((d->d + 127) / 128) <= XE_TINY_STEPS;
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
@@ -1262,7 +1340,7 @@ int launch_small_logits(const void* x, long long ldx, const void* w, long long l
 
 template <typename T>
 int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* db, const wino_xent_desc& d, const Plan& p, const float* dz, const XeScale& scale,
-                      const XeLoss& loss, cudaStream_t st) {
+                      const XeLoss& loss, const RowArgs& ra, cudaStream_t st) {
     SmallGrad<T> a;
     a.x = (const T*)x; a.w = (const T*)w; a.dx = (T*)dx; a.dw = (T*)dw; a.db = db;
     a.ldx = p.ldx; a.ldw = p.ldw; a.lddx = p.lddx; a.lddw = p.lddw;
@@ -1271,6 +1349,7 @@ int launch_small_grad(const void* x, const void* w, void* dx, void* dw, float* d
     a.dx_blocks = dx ? (d.n + 7) / 8 * a.kblocks : 0;
     a.scale = scale;
     a.loss = loss;
+    a.rule = ra.rule; a.target = ra.target; a.count = ra.count;
     const int dw_blocks = dw || db ? (d.v + 7) / 8 * a.kblocks : 0;
     return xe_launch(xe_small_grad_kernel<T>, (unsigned)(a.dx_blocks + dw_blocks + (loss.loss ? 1 : 0)), 256, XE_SMALL_GRAD_SMEM, st, a);
 }
@@ -1415,7 +1494,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     sum.rowloss = ra.rowloss; sum.n = n; sum.count = ra.count;
     sum.mean = d.reduction == WINO_MEAN;
     const bool later = products && (dx || dw) && n <= 1024 && !p.few;
-    if (!later) ra.loss = sum;
+    const bool tiny = p.tiny && (products ? d.n <= XE_SMALL_MAX : d.reduction == WINO_NONE || d.n <= XE_SMALL_ROWS);
+    if (!later && !(tiny && products)) ra.loss = sum;
     if ((rc = status_word(&ra.status))) return rc;
     const float* b = d.has_bias ? bias : nullptr;
     const bool wide = d.v > XE_ROWS_MAX_V;
@@ -1427,6 +1507,19 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     scale.factor = dz_factor;
     scale.mean = sum.mean;
 
+    if (tiny) {
+        float* z = f(p.off_z);
+        const unsigned blocks = (unsigned)((n + XE_SMALL_ROWS - 1) / XE_SMALL_ROWS);
+        auto go = [&](auto t) {
+            using T = decltype(t);
+            auto kernel = products ? xe_tiny_kernel<T, true> : xe_tiny_kernel<T, false>;
+            return xe_launch(kernel, blocks, 32 * XE_TINY_WARPS, 0, st, (const T*)x, p.ldx, (const T*)w, p.ldw, d.d, d.v, p.zpitch, b, ra, dzr, z);
+        };
+        if ((rc = p.es == 2 ? go(__nv_bfloat16()) : go(float()))) return rc;
+        if (!products) return WINO_OK;
+        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, z, scale, sum, ra, st)
+                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, z, scale, sum, ra, st);
+    }
     const bool kept_stats = p.kept && wide && p.splits_z == 1 && !p.few;
     XeProduct pz = {kept_stats ? XE_STATS_Z : p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
     pz.bn = p.bn_z;
@@ -1475,8 +1568,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
 
     if (!products) return WINO_OK;
     if (p.small)
-        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st)
-                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), st);
+        return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), ra, st)
+                         : launch_small_grad<float>(x, w, dx, dw, db, d, p, f(p.off_z), scale, later ? sum : XeLoss(), ra, st);
     if (p.few) {
         float* z = f(p.off_z);
         if (wide) {

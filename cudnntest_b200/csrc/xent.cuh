@@ -45,11 +45,10 @@ struct XeScale {
     float factor = 1.f;
     int mean = 0;
 };
-__device__ __forceinline__ float xe_scale(const XeScale& s) {
-    if (!s.count) return 1.f;
-    const int n = *s.count;
+__device__ __forceinline__ float xe_scale(const XeScale& s, int n) {
     return s.factor * (s.dloss ? *s.dloss : 1.f) * (s.mean ? 1.f / (float)(n > 0 ? n : 1) : 1.f);
 }
+__device__ __forceinline__ float xe_scale(const XeScale& s) { return s.count ? xe_scale(s, *s.count) : 1.f; }
 
 // the mean or sum of the rows' losses
 struct XeLoss {

@@ -111,7 +111,9 @@ class LinearXent:
         self._desc_ref, self._ws_size = ctypes.byref(s), self.workspace.numel() * self.workspace.element_size()
         self._index = self.workspace.get_device()
         self._forms = [(torch.Size((rows, d)), (ld or d, 1)) for rows, ld in ((n, ldx), (v, ldw), (n, lddx), (v, lddw))]
-        self._like = torch.empty(0, dtype=torch.float32, device=self.workspace.device)
+        # what results are allocated like
+        self._lse_like = torch.empty(n, dtype=torch.float32, device=self.workspace.device)
+        self._loss_like = self._lse_like if s.reduction == _lib.NONE else torch.empty((), dtype=torch.float32, device=self.workspace.device)
 
     def _matrix(self, t, what, form):
         """Device address of a matrix of the plan's rows and pitch; form: (shape, strides)."""
@@ -141,14 +143,10 @@ class LinearXent:
         return (self._matrix(x, "x", self._forms[0]), self._matrix(w, "w", self._forms[1]),
                 None if bias is None else self._vector(bias, "bias", s.v, torch.float32), self._vector(target, "target", s.n, torch.int64))
 
-    def _losses(self):
-        s = self.desc
-        return self._like.new_empty((s.n,) if s.reduction == _lib.NONE else ())
-
     def forward(self, x, w, target, bias=None):
         """(loss, lse): loss is a scalar (or n values), lse_i = log sum_j exp z_ij (0 for an ignored row)."""
         args = self._inputs(x, w, target, bias)
-        loss, lse = self._losses(), self._like.new_empty((self.desc.n,))
+        loss, lse = torch.empty_like(self._loss_like), torch.empty_like(self._lse_like)
         _call(lib().wino_xent_forward, self._index, self._desc_ref, *args, loss.data_ptr(), lse.data_ptr(), self.workspace.data_ptr(),
               self._ws_size)
         return loss, lse
@@ -179,7 +177,7 @@ class LinearXent:
         dx, dx_ptr = result(dx, need_dx, "dx", x, self._forms[2])
         dw, dw_ptr = result(dw, need_dw, "dw", w, self._forms[3])
         db = torch.empty_like(bias) if s.has_bias else None
-        loss = self._losses()
+        loss = torch.empty_like(self._loss_like)
         _call(lib().wino_xent_grad, self._index, self._desc_ref, *args, dloss, loss.data_ptr(), None, dx_ptr, dw_ptr,
               None if db is None else db.data_ptr(), self.workspace.data_ptr(), self._ws_size)
         return loss, dx, dw, db

@@ -138,6 +138,10 @@ CASES = [
     (8, 1002, 3000, "bf16", {}),
     (3, 260, 70001, "fp32", dict(ldx=264, ldw=261)),
     (13, 6001, 130, "fp32", {}),
+    (100, 515, 31, "bf16", {}),                                   # logits, softmax and dz in one kernel; ragged widths
+    (128, 128, 128, "fp32", {}),
+    (9, 2050, 7, "fp32", dict(bias=False, ldx=2053, ldw=2052)),
+    (7, 40, 128, "bf16", {}),
     (3000, 3001, 3, "fp32", {}),                                  # few classes, the same kernels with the matrices exchanged
     (777, 1000, 16, "fp32", dict(ldx=1003, ldw=1001)),
     (300, 260, 1, "fp32", {}),
@@ -172,7 +176,7 @@ def test_gradient_against_definition(n, d, v, dtype, kw, reduction):
 
 
 @pytest.mark.parametrize("n,d,v,dtype", [(40, 4096, 1000, "bf16"), (300, 96, 700, "fp32"), (2305, 40, 2100, "bf16"), (2305, 40, 2100, "fp32"),
-                                         (15, 2300, 700, "fp32"), (7, 2301, 700, "bf16"), (100, 64, 100, "bf16"), (700, 900, 9, "fp32")])
+                                         (15, 2300, 700, "fp32"), (7, 2301, 700, "bf16"), (100, 64, 100, "bf16"), (700, 900, 9, "fp32"), (60, 3000, 100, "fp32")])
 @pytest.mark.parametrize("ignored", [0.3, 1.0])
 @pytest.mark.parametrize("ignore_index", [-100, 3, 2 ** 62])
 def test_ignored_rows_leave_no_trace(n, d, v, dtype, ignored, ignore_index):
@@ -195,16 +199,20 @@ def test_ignored_rows_leave_no_trace(n, d, v, dtype, ignored, ignore_index):
 
 
 @pytest.mark.parametrize("n,d,v,dtype", [(1, 1, 1, "bf16"), (16, 4096, 1000, "bf16"), (777, 512, 1000, "fp32"), (2305, 40, 2100, "bf16"),
-                                         (2305, 40, 2100, "fp32"), (3, 50, 70000, "bf16")])
+                                         (2305, 40, 2100, "fp32"), (3, 50, 70000, "bf16"),
+                                         (500, 96, 33, "fp32"), (8, 512, 10, "bf16"), (500, 2000, 100, "bf16")])
 @pytest.mark.parametrize("smoothing", [0.0, 0.2, 1.0])
 def test_forward_against_definition(n, d, v, dtype, smoothing):
     c = Case(n, d, v, dtype, seed=11)
+    mean = c.plan(reduction="mean", label_smoothing=smoothing, grad=False).forward(c.x, c.w, c.target, c.bias)
     ref = c.oracle("none", smoothing)
     loss, lse = c.plan(reduction="none", label_smoothing=smoothing, grad=False).forward(c.x, c.w, c.target, c.bias)
     ez, el, _ = c.z_error(ref)
     assert (np.abs(lse.double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
     row = el + ez.max(1) + (8 + smoothing * v / 64) * F32 * (np.abs(ref["z"]).max(1) + np.abs(ref["lse"]))
     assert (np.abs(loss.double().cpu().numpy() - ref["loss"]) <= row).all()
+    assert abs(float(mean[0]) - ref["loss"].mean()) <= row.mean() + 2 * F32 * abs(ref["loss"].mean())
+    assert (np.abs(mean[1].double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
