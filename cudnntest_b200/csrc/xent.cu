@@ -913,7 +913,8 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
 // three times more, and a 256-row tensor-core tile would be mostly empty.  In all three kernels a lane owns four features,
 // 32 apart (single elements then make whole lines at any pitch and alignment), whose values of all rows (x, or the sums of dx) it
 // holds in registers as packed pairs, and a warp walks over classes, one piece of 128 features of W or dW per class.
-// ROWS (4, 8 or 16) rows cost ROWS * 4 multiplications a lane and piece, which the FP32 pipe does faster than HBM delivers it.
+// Bound: HBM up to four rows (loss of 4 x 4096 x 32000 at 4.5 TB/s); beyond, the multiplications and, for the logits, the
+// exchange of the lanes' sums (8 rows 3.0 TB/s, 16 rows 1.9 TB/s).
 constexpr int XF_ROWS = 16, XF_COLS = 128, XF_CLASSES = 128;      // most rows; features and classes of a block
 struct FewArgs {
     const float* x; const float* w;       // the matrix of few rows (n), and the long one (v rows); classes and rows may change
@@ -1221,7 +1222,9 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
     const int few_splits = few_split_count(long_tiles, col_tiles);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
-    p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && z_bytes * few_splits <= limit;
+    // Measured with gradients, against tensor cores: 16 x 1024 x 1000 36.9 / 34.3 us, 16 x 4096 x 256 41.0 / 32.9, 8 x 4096 x 1000
+    // 35.6 / 51.4, 16 x 512 x 50000 193 / 231, 8 x 4096 x 32000 390 / 879.
+    p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
     p.tiny = p.small && v <= XE_SMALL_MAX && (v + XE_TINY_WARPS - 1) / XE_TINY_WARPS * ((d->d + 127) / 128) <= XE_TINY_STEPS;
     if (p.small) {
         p.kept = true;
