@@ -1,12 +1,13 @@
 // Linear softmax cross entropy with its gradient: driver and row kernels (the products are in xent_gemm.cu).
 //
-// The logits z = x W^T exist one tile at a time.  Two ways, by size:
+// The logits z = x W^T are never a tensor of the caller's.  Ways, by size (build_plan):
+//   * few products, few rows, few classes: FP32 kernels on the caller's matrices (xe_tiny_kernel, xe_small_*, xe_few_*);
 //   * kept: where rows or classes are few the logits product is split along the features until the GPU is full; its
 //     float parts in the scratch become lse, loss and dz in row kernels.  Unsplit, floats are kept as well where that is
-//     cheaper than a fourth product (below);
+//     cheaper than a fourth product;
 //   * as exponentials: BF16 without a bias whose dz fits the scratch.  The logits product leaves a maximum and a sum per
 //     row and 128 classes and exp(z - maximum) as BF16 in the place of dz; one pass over it makes dz.  Three products
-//     (2 n v d flops each) either way;
+//     (2 n v d flops each) in all these ways;
 //   * recomputed: the logits product leaves only the statistics; the gradient then walks the vocabulary in pieces, computes
 //     a piece's logits again, turns them into dz in the epilogue, and multiplies dz into dx and dW before the next piece:
 //     four products, scratch bounded by desc.scratch_limit.
@@ -333,12 +334,14 @@ __device__ __forceinline__ void store_dz(float (&d)[4], void* dz, long long n, l
     }
 }
 
-// Kept logits -> lse, loss and dz (PLANES BF16 planes; 0: floats, which may replace the first part of the logits) in one go.  A block takes a run of rows; a thread holds the same 4 * QUADS columns of each
-// in registers, from the sum of the parts to dz, and their column sums over the run.  v <= 4 * THREADS * QUADS.
+// Kept logits -> lse, loss and dz (PLANES BF16 planes; 0: floats, which may replace the first part of the logits) in one go.
+// A block takes a run of rows; a thread holds the same 4 * QUADS columns of each in registers, from the sum of the parts to
+// dz, and their column sums over the run.  v <= 4 * THREADS * QUADS.
 // 1024 threads an SM (64 registers), fewer where the parts of the columns have to be in flight.
 template <int THREADS, int QUADS, int PLANES, bool GRAD, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, (!SPLIT ? 1024 : QUADS > 1 ? 512 : 768) / THREADS) xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a,
-                                                          const XeDzRule rule, void* dz, int dpitch, float* __restrict__ db_part) {
+__global__ void __launch_bounds__(THREADS, (!SPLIT ? 1024 : QUADS > 1 ? 512 : 768) / THREADS)
+xe_rows_kernel(const float* z, int splits, int v, int zpitch, const float* __restrict__ bias, const RowArgs a, const XeDzRule rule, void* dz, int dpitch,
+               float* __restrict__ db_part) {
     pdl_wait();
     constexpr int WARPS = THREADS / 32;
     __shared__ float red[2][3][WARPS];          // two sets, used by turns: a row's second barrier frees the other set
@@ -1122,7 +1125,7 @@ struct Plan {
     int planes, es, dp;
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
-    bool tiny, small, few, few_rows;           // FP32 arithmetic instead of tensor cores: xe_tiny_kernel, xe_small_*, xe_few_* (of rows, else of classes)
+    bool tiny, small, few, few_rows;     // FP32 arithmetic instead of tensor cores; few: of rows, else of classes
     int splits_few;                      // of the gradient of the matrix of few rows
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
@@ -1213,10 +1216,6 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.zpitch = round_up(d->v, 4);
     const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll;
     const bool fits = z_bytes * p.splits_z + (grad ? dz_bytes : 0) <= limit;
-    // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
-    // logit (18 in three parts), exponentials 6, against 2 d flops (12 d) for another product.  Measured, with gradients, kept
-    // against computed again: floats 4096 x d x 20000 BF16 d = 512 363 / 316 us, 1024 498 / 500, 2048 841 / 941; FP32X3
-    // 4096 x d x 12000 d = 128 484 / 465, 256 572 / 571, 512 891 / 995; exponentials d = 256 253 / 242, 512 303 / 304, 1024 440 / 495.
     const bool few_tiles = n * v <= 64ll * XE_BM * XE_BN;
     p.few_rows = n <= XF_ROWS;
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
@@ -1226,6 +1225,10 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // 35.6 / 51.4, 16 x 512 x 50000 193 / 231, 8 x 4096 x 32000 390 / 879.
     p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
     p.tiny = p.small && v <= XE_SMALL_MAX && (v + XE_TINY_WARPS - 1) / XE_TINY_WARPS * ((d->d + 127) / 128) <= XE_TINY_STEPS;
+    // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
+    // logit (18 in three parts), exponentials 6, against 2 d flops (12 d) for another product.  Measured, with gradients, kept
+    // against computed again: floats 4096 x d x 20000 BF16 d = 512 363 / 316 us, 1024 498 / 500, 2048 841 / 941; FP32X3
+    // 4096 x d x 12000 d = 128 484 / 465, 256 572 / 571, 512 891 / 995; exponentials d = 256 253 / 242, 512 303 / 304, 1024 440 / 495.
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
@@ -1239,7 +1242,8 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
     if (!grad && p.splits_z == 1 && !p.small && !p.few) p.kept = false;          // statistics are all that is wanted
     if (!p.kept) p.splits_z = 1;
-    p.bn_z = p.kept && (p.splits_z > 1 || d->v <= XE_ROWS_MAX_V) ? cz.bn : XE_BN;                       // the other epilogues make statistics of 128 columns a warp
+    // epilogues with statistics make them of 128 columns a warp
+    p.bn_z = p.kept && (p.splits_z > 1 || d->v <= XE_ROWS_MAX_V) ? cz.bn : XE_BN;
     p.piece = d->v;
     p.pieces = 1;
     if (grad && !p.kept && !p.exps) {
@@ -1254,11 +1258,11 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     }
     p.dzpitch = round_up(p.piece, 8);
     p.dpitch = round_up(d->d, 4);
-    Cut cx = cut_product(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true), cw = cut_product(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
+    const Cut cx = cut_product(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true), cw = cut_product(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
     p.splits_dx = cx.splits; p.splits_dw = cw.splits;
     p.bn_dx = cx.bn; p.bn_dw = cw.bn;
-    // more than one piece adds up in floats: in dx itself, or in the scratch
     p.splits_few = few_split_count(col_tiles, long_tiles);
+    // more than one piece adds up in floats: in dx itself, or in the scratch
     p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
     p.dw_direct = p.splits_dw == 1;
     p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, d->v) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
@@ -1281,7 +1285,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.off_x = take(p.pack_x ? un * p.dp * 2 * p.planes : 0);
     p.off_w = take(p.pack_w ? (size_t)v * p.dp * 2 * p.planes : 0);
     if (grad) {
-        p.off_dz = take(un * p.dzpitch * 2 * p.planes);
+        p.off_dz = take(p.small || p.few ? 0 : un * p.dzpitch * 2 * p.planes);      // those two: in the place of the logits
         p.off_db = take(d->has_bias ? (size_t)p.parts * p.dzpitch * 4 : 0);
         p.off_dx = take(p.few ? (size_t)(p.few_rows ? n : v) * p.dpitch * 4 * p.splits_few : p.dx_direct ? 0 : un * p.dpitch * 4 * p.splits_dx);
         p.off_dw = take(p.few || p.dw_direct ? 0 : (size_t)p.piece * p.dpitch * 4 * p.splits_dw);
@@ -1470,8 +1474,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         const unsigned blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * (p.dp / 4));
         if (d.dtype == WINO_BF16 && ((p.pack_x && p.ldx % 8) || (p.pack_w && p.ldw % 8))) {
             const bool pairs = !(p.pack_x && p.ldx % 2) && !(p.pack_w && p.ldw % 2);
-            const unsigned row_blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * ((p.dp + 255) / 256) * 32);
-            rc = xe_launch(pairs ? xe_pack_rows_kernel<true> : xe_pack_rows_kernel<false>, row_blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
+            const unsigned warp_blocks = loop_blocks((jobs[0].rows + jobs[1].rows) * ((p.dp + 255) / 256) * 32);
+            rc = xe_launch(pairs ? xe_pack_rows_kernel<true> : xe_pack_rows_kernel<false>, warp_blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
         } else if (d.dtype == WINO_BF16) rc = xe_launch(xe_pack_kernel<__nv_bfloat16, 1>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
         else rc = xe_launch(xe_pack_kernel<float, 3>, blocks, 256, 0, st, jobs[0], jobs[1], d.d, p.dp, rule);
         if (rc) return rc;
@@ -1548,7 +1552,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             auto rows_fn = d.v <= 512 ? launch_warp_rows : d.v <= 1024 ? launch_rows<256, 1> : d.v <= 2048 ? launch_rows<256, 2>
                          : d.v <= 4096 ? launch_rows<256, 4> : launch_rows<512, 4>;
             // floats in the place of the logits; column sums where there are more rows than the products' kernels add up
-            if ((p.small || p.few) && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, p.few && !p.few_rows ? db_part : nullptr);
+            float* few_db = p.few && !p.few_rows ? db_part : nullptr;
+            if ((p.small || p.few) && products) rc = rows_fn(0, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, z, p.zpitch, few_db);
             else rc = rows_fn(products ? p.planes : -1, blocks, st, z, p.splits_z, d.v, p.zpitch, b, ra, dzr, dz, p.dzpitch, db_part);
         }
     } else {
@@ -1593,7 +1598,8 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             else rc = xe_launch(xe_wide_dz_kernel<3>, grid, 128, 0, st, f(p.off_z), vc, p.zpitch, n, ra.lse, ra.rowg, target, dzr, dz, p.dzpitch, db_part);
         } else if (p.exps) {
             const long long spans = n * ((p.dzpitch / 8 + 1023) / 1024);
-            rc = xe_launch(xe_dz_from_exp_kernel, (unsigned)(spans < 0x7fffffffll ? spans : 0x7fffffffll), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt, ra.lse, ra.rowg, target, dzr);
+            rc = xe_launch(xe_dz_from_exp_kernel, (unsigned)(spans < 0x7fffffffll ? spans : 0x7fffffffll), 256, 0, st, dz, p.dzpitch, n, pz.out.stats, pz.out.zt,
+                           ra.lse, ra.rowg, target, dzr);
         } else if (!p.kept) {
             XeProduct pd = {XE_DZ, ox, wp, n, vc, d.d, XeOutput()};
             pd.out.ptr = dz; pd.out.pitch = p.dzpitch;
@@ -1634,8 +1640,9 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             zr.along_rows = xr.along_rows = true;
             product(zr, xr, vc, n, p.dw_direct, p.splits_dw, p.bn_dw, false, dw_at, p.lddw, f(p.off_dw));
         }
-        // Both in one launch where one of them has few tiles: the other fills the SMs that it leaves idle (256 x 25088 x 1000: 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU
-        // runs at its power limit either way (8192 x 4096 x 50021: 8.2 ms apart, 8.4 ms together).
+        // Both in one launch where one of them has few tiles: the other fills the SMs that it leaves idle (256 x 25088 x 1000:
+        // 46 -> 38 us).  With many turns of both there is nothing to fill, and the GPU runs at its power limit either way
+        // (8192 x 4096 x 50021: 8.2 ms apart, 8.4 ms together).
         const long long tiles_x = (n + XE_BM - 1) / XE_BM * ((d.d + p.bn_dx - 1) / p.bn_dx) * p.splits_dx;
         const long long tiles_w = ((long long)vc + XE_BM - 1) / XE_BM * ((d.d + p.bn_dw - 1) / p.bn_dw) * p.splits_dw;
         if (first && later) prod[0].out.loss = sum;
