@@ -515,8 +515,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                     }
                     if (p.zsum) {
                         float t[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (whole) {                  // in pairs: a selection per element took 6152 x 64 x 32149 from 108 to 221 us
 #pragma unroll
-                        for (int i = 0; i < WCOLS; ++i) t[i & 3] += whole || wcol + i < p.n ? z[i] : 0.f;
+                            for (int i = 0; i < WCOLS; i += 2) add2(t[i & 2], t[(i & 2) + 1], z[i], z[i + 1]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < WCOLS; ++i) t[i & 3] += wcol + i < p.n ? z[i] : 0.f;
+                        }
                         if (live) p.zsum[wcol / XE_STAT_COLS * p.m + row] = (t[0] + t[1]) + (t[2] + t[3]);
                     }
                     if (!whole) {
