@@ -1,10 +1,11 @@
-// Linear softmax cross entropy with its gradient: driver and row kernels (the products are in xent_gemm.cu).
+// Linear softmax cross entropy with its gradient: driver and row kernels (the products are in xent_gemm.cu and xent_thin.cu).
 //
 // The logits z = x W^T are never a tensor of the caller's.  Ways, by size (build_plan):
 //   * few products, few rows, few classes: FP32 kernels on the caller's matrices (xe_tiny_kernel, xe_small_*, xe_few_*);
 //   * kept: where rows or classes are few the logits product is split along the features until the GPU is full; its
 //     float parts in the scratch become lse, loss and dz in row kernels.  Unsplit, floats are kept as well where that is
-//     cheaper than a fourth product;
+//     cheaper than a fourth product.  FP32X3 with up to 128 rows or classes: the longer matrix is split into BF16 parts
+//     inside its products (xent_thin.cu), the others beforehand;
 //   * as exponentials: BF16 without a bias whose dz fits the scratch.  The logits product leaves a maximum and a sum per
 //     row and 128 classes and exp(z - maximum) as BF16 in the place of dz; one pass over it makes dz.  Three products
 //     (2 n v d flops each) in all these ways;
@@ -911,14 +912,13 @@ __global__ void __launch_bounds__(256) xe_small_grad_kernel(const SmallGrad<T> a
 }
 
 // ---- few rows: FP32 products on the caller's matrices ----------------------------------------------------------
-// FP32X3 with up to 16 rows, or up to 16 classes (for which read: x as W, and the other way round): the products are a read of
-// W (twice) and a write of dW; splitting W into BF16 parts first would move it
-// three times more, and a 256-row tensor-core tile would be mostly empty.  In all three kernels a lane owns four features,
+// FP32X3 with up to 8 rows, or up to 8 classes (for which read: x as W, and the other way round): the products are a read of
+// W (twice) and a write of dW, and a tensor-core tile would be mostly empty.  In all three kernels a lane owns four features,
 // 32 apart (single elements then make whole lines at any pitch and alignment), whose values of all rows (x, or the sums of dx) it
 // holds in registers as packed pairs, and a warp walks over classes, one piece of 128 features of W or dW per class.
 // Bound: HBM up to four rows (loss of 4 x 4096 x 32000 at 4.5 TB/s); beyond, the multiplications and, for the logits, the
-// exchange of the lanes' sums (8 rows 3.0 TB/s, 16 rows 1.9 TB/s).
-constexpr int XF_ROWS = 16, XF_COLS = 128, XF_CLASSES = 128;      // most rows; features and classes of a block
+// exchange of the lanes' sums (8 rows 3.0 TB/s).
+constexpr int XF_ROWS = 8, XF_COLS = 128, XF_CLASSES = 128;      // most rows; features and classes of a block
 struct FewArgs {
     const float* x; const float* w;       // the matrix of few rows (n), and the long one (v rows); classes and rows may change
                                           // places: then x is W, w is x, and dx and dW change places as well
@@ -1126,6 +1126,8 @@ struct Plan {
     long long ldx, ldw, lddx, lddw;
     bool pack_x, pack_w;
     bool tiny, small, few, few_rows;     // FP32 arithmetic instead of tensor cores; few: of rows, else of classes
+    bool thin, thin_rows;                // W (up to 128 rows) or x (up to 128 classes) is split inside the products (xe_thin)
+    XeThinCut thin_z, thin_grad;
     int splits_few;                      // of the gradient of the matrix of few rows
     bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
@@ -1221,9 +1223,22 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
     const int few_splits = few_split_count(long_tiles, col_tiles);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
-    // Measured with gradients, against tensor cores: 16 x 1024 x 1000 36.9 / 34.3 us, 16 x 4096 x 256 41.0 / 32.9, 8 x 4096 x 1000
-    // 35.6 / 51.4, 16 x 512 x 50000 193 / 231, 8 x 4096 x 32000 390 / 879.
-    p.few = !bf16 && !p.small && n > 0 && (n <= XF_ROWS || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
+    // Measured with gradients, against tensor cores that split W themselves, us: 8 x 2048 x 4000 53.3 / 62.7, 8 x 2048 x 20000
+    // 158 / 193, 8000 x 2048 x 8 102 / 129; the same kernels for 16 rows 16 x 2048 x 20000 256 / 197, 8000 x 2048 x 16 145 / 125.
+    p.few = !bf16 && !p.small && n > 0 && (p.few_rows || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
+    // Measured, the long matrix split inside against beforehand, us: loss of 64 x 512 x 1000 16.4 / 16.4, 64 x 2048 x 1000 18.5 / 22.6, 64 x 2048 x 4000
+    // 25.2 / 46.7, 128 x 2048 x 20000 84 / 208; gradient of 64 x 512 x 1000 34.9 / 30.8, 64 x 4096 x 300 43.0 / 44.0, 64 x 2048 x 1000
+    // 39.8 / 45.1, 64 x 2048 x 20000 207 / 322.  A tile of 128 rows takes the products apart that one launch would share:
+    // gradient of 128 x 512 x 20000 137 / 132, 128 x 2048 x 20000 232 / 382.  With few classes the same: loss of 8000 x 2048 x 64
+    // 45.4 / 81.9; gradient of 4000 x 512 x 16 51.3 / 55.4, 8000 x 512 x 64 67.6 / 67.6, 4000 x 2048 x 128 100 / 94, 8000 x 2048 x 128 146 / 157.
+    p.thin_rows = n <= 128 && (v > 128 || v >= n);
+    const long long thin_n = p.thin_rows ? n : v, thin_m = p.thin_rows ? v : n;
+    p.thin = !bf16 && !p.small && !p.few && n > 0 && thin_n <= 128 && thin_m * d->d >= (grad && thin_n > 64 ? 16ll << 20 : 1ll << 20);
+    if (p.thin) {
+        p.thin_z = xe_thin_cut((thin_m + 127) / 128, kd, (double)n * v * 8.0 / 5e6);
+        p.thin_grad = xe_thin_cut(col_tiles, (thin_m + XE_BK - 1) / XE_BK, (double)thin_n * d->d * 8.0 / 5e6);
+        p.thin = z_bytes * p.thin_z.parts + (grad ? dz_bytes : 0) <= limit;
+    }
     p.tiny = p.small && v <= XE_SMALL_MAX && (v + XE_TINY_WARPS - 1) / XE_TINY_WARPS * ((d->d + 127) / 128) <= XE_TINY_STEPS;
     // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
     // logit (18 in three parts), exponentials 6, against 2 d flops (12 d) for another product.  Measured, with gradients, kept
@@ -1237,10 +1252,14 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
         p.splits_z = few_splits;
+    } else if (p.thin) {
+        p.kept = true;
+        (p.thin_rows ? p.pack_w : p.pack_x) = false;
+        p.splits_z = p.thin_z.parts;
     } else if (few_tiles && fits) p.kept = true;
     else if (grad && bf16 && !d->has_bias && dz_bytes <= limit && d->d >= 512) p.exps = true;
     else p.kept = grad && fits && d->d >= (bf16 ? 1024 : 256);
-    if (!grad && p.splits_z == 1 && !p.small && !p.few) p.kept = false;          // statistics are all that is wanted
+    if (!grad && p.splits_z == 1 && !p.small && !p.few && !p.thin) p.kept = false;          // statistics are all that is wanted
     if (!p.kept) p.splits_z = 1;
     // epilogues with statistics make them of 128 columns a warp
     p.bn_z = p.kept && (p.splits_z > 1 || d->v <= XE_ROWS_MAX_V) ? cz.bn : XE_BN;
@@ -1259,7 +1278,8 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.dzpitch = round_up(p.piece, 8);
     p.dpitch = round_up(d->d, 4);
     const Cut cx = cut_product(n, d->d, (p.piece + XE_BK - 1) / XE_BK, products, true), cw = cut_product(p.piece, d->d, (n + XE_BK - 1) / XE_BK, products, true);
-    p.splits_dx = cx.splits; p.splits_dw = cw.splits;
+    p.splits_dx = p.thin && p.thin_rows ? p.thin_grad.parts : cx.splits;
+    p.splits_dw = p.thin && !p.thin_rows ? p.thin_grad.parts : cw.splits;
     p.bn_dx = cx.bn; p.bn_dw = cw.bn;
     p.splits_few = few_split_count(col_tiles, long_tiles);
     // more than one piece adds up in floats: in dx itself, or in the scratch
@@ -1389,12 +1409,11 @@ FewArgs few_args(const void* x, const void* w, const wino_xent_desc& d, const Pl
     return a;
 }
 
-// the kernel for 4, 8 or 16 rows
+// the kernel for 4 or 8 rows
 template <typename Pick>
 int few_launch(int n, dim3 grid, cudaStream_t st, const FewArgs& a, Pick pick) {
     if (n <= 4) return xe_launch(pick(std::integral_constant<int, 4>()), grid, 128, 0, st, a);
-    if (n <= 8) return xe_launch(pick(std::integral_constant<int, 8>()), grid, 128, 0, st, a);
-    return xe_launch(pick(std::integral_constant<int, 16>()), grid, 128, 0, st, a);
+    return xe_launch(pick(std::integral_constant<int, 8>()), grid, 128, 0, st, a);
 }
 
 int launch_few_logits(const void* x, const void* w, const wino_xent_desc& d, const Plan& p, float* z, int* zero, cudaStream_t st) {
@@ -1500,7 +1519,7 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
     sum.loss = d.reduction == WINO_NONE ? nullptr : loss;
     sum.rowloss = ra.rowloss; sum.n = n; sum.count = ra.count;
     sum.mean = d.reduction == WINO_MEAN;
-    const bool later = products && (dx || dw) && n <= 1024 && !p.few;
+    const bool later = products && (dx || dw) && n <= 1024 && !p.few && (!p.thin || (p.thin_rows ? dw : dx));
     const bool tiny = p.tiny && (products ? d.n <= XE_SMALL_MAX : d.reduction == WINO_NONE || d.n <= XE_SMALL_ROWS);
     if (!later && !(tiny && products)) ra.loss = sum;
     if ((rc = status_word(&ra.status))) return rc;
@@ -1527,7 +1546,9 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         return p.es == 2 ? launch_small_grad<__nv_bfloat16>(x, w, dx, dw, db, d, p, z, scale, sum, ra, st)
                          : launch_small_grad<float>(x, w, dx, dw, db, d, p, z, scale, sum, ra, st);
     }
-    const bool kept_stats = p.kept && wide && p.splits_z == 1 && !p.few;
+    XeThin thin = {};                  // the long matrix
+    thin.l = (const float*)(p.thin_rows ? w : x); thin.rows = p.thin_rows ? v : n; thin.ldl = p.thin_rows ? p.ldw : p.ldx; thin.d = d.d;
+    const bool kept_stats = p.kept && wide && p.splits_z == 1 && !p.few && !p.thin;
     XeProduct pz = {kept_stats ? XE_STATS_Z : p.kept ? XE_F32 : p.exps ? XE_STATS_E : XE_STATS, ox, ow, n, v, d.d, XeOutput()};
     pz.bn = p.bn_z;
     pz.out.zero = ra.count;
@@ -1537,7 +1558,15 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
         pz.out.pitch = p.zpitch;
         pz.out.splits = p.splits_z;
         if (p.few) rc = launch_few_logits(x, w, d, p, z, ra.count, st);
-        else if (!p.small) rc = xe_gemm(&pz, 1, st);
+        else if (p.thin) {
+            XeThin t = thin;
+            t.s = p.thin_rows ? ox : ow;
+            t.out = z; t.plane = n * p.zpitch;
+            t.out_s = p.thin_rows ? p.zpitch : 1; t.out_m = p.thin_rows ? 1 : p.zpitch;
+            t.cut = p.thin_z;
+            t.zero = ra.count;
+            rc = xe_thin(t, st);
+        } else if (!p.small) rc = xe_gemm(&pz, 1, st);
         else if (p.es == 2) rc = launch_small_logits<__nv_bfloat16>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
         else rc = launch_small_logits<float>(x, p.ldx, w, p.ldw, d, p, z, ra.count, st);
         if (rc) return rc;
@@ -1630,12 +1659,27 @@ int xent(const wino_xent_desc* dd, bool grad, const void* x, const void* w, cons
             q.out.splits = direct ? 1 : chunks < splits ? (int)chunks : splits;
         };
         void* dw_at = static_cast<char*>(dw) + (size_t)v0 * p.lddw * p.es;
-        if (dx) {
+        const bool thin_dx = p.thin && p.thin_rows, thin_dw = p.thin && !p.thin_rows;
+        if (thin_dx ? dx != nullptr : thin_dw && dw) {
+            XeThin t = thin;
+            t.along_rows = true;
+            t.rowg = thin_dw ? ra.rowg : nullptr;
+            t.s = odz;
+            t.s.along_rows = thin_dw;
+            const bool direct = thin_dx ? p.dx_direct : p.dw_direct;
+            t.out = thin_dx ? (direct ? (float*)dx : f(p.off_dx)) : (direct ? (float*)dw : f(p.off_dw));
+            t.out_s = !direct ? p.dpitch : thin_dx ? p.lddx : p.lddw; t.out_m = 1;
+            t.plane = (thin_dx ? n : v) * p.dpitch;
+            t.cut = p.thin_grad;
+            t.scale = scale;
+            if ((rc = xe_thin(t, st))) return rc;
+        }
+        if (dx && !thin_dx) {
             XeOperand wr = wp;
             wr.along_rows = true;
             product(odz, wr, n, vc, p.dx_direct, p.splits_dx, p.bn_dx, !first, dx, p.lddx, f(p.off_dx));
         }
-        if (dw) {
+        if (dw && !thin_dw) {
             XeOperand zr = odz, xr = ox;
             zr.along_rows = xr.along_rows = true;
             product(zr, xr, vc, n, p.dw_direct, p.splits_dw, p.bn_dw, false, dw_at, p.lddw, f(p.off_dw));

@@ -17,6 +17,25 @@ struct XeOperand {
     bool along_rows;
 };
 
+// boxes of 64 columns (128 bytes, 128-byte swizzle): `share` rows for a K-major share, 64 rows (one contraction element each)
+// for an MN-major one
+int xe_operand_map(CUtensorMap* map, const XeOperand& o, unsigned share);
+
+// MN-major tile with 128-byte swizzle: rows of 64 elements (128 bytes) along M or N, one row per contraction element,
+// groups of 8 contraction elements 1 KiB apart, blocks of 64 M / N elements 8 KiB apart
+__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(8192 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// what a wait that ran out was for
+enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
+
 // What the epilogue does with a 256 x 256 tile of the product (m rows x n columns)
 enum XeEpilogue {
     XE_F32 = 0,       // scale, store floats or add them to what is there
@@ -114,12 +133,56 @@ struct XeProduct {
 // one or two products in one launch; two must have the same bn and epilogues XE_F32 or XE_BF16
 int xe_gemm(const XeProduct* prod, int count, cudaStream_t st);
 
+// how a product is shared: CTAs, and the buffers that hold pieces of the same tile
+struct XeThinCut {
+    int grid, parts;
+};
+// Product of a matrix L of floats as it lies with up to 128 rows s of BF16 planes (xent_thin.cu): out[s][row of L] = s L^T, or,
+// where `along_rows` is set, out[s][column of L] = s L, the contraction along the rows of L.
+struct XeThin {
+    const float* l;
+    long long rows, ldl;
+    int d;                            // columns of L
+    bool along_rows;
+    const float* rowg = nullptr;      // rows of L with weight 0 are taken as zeros, or NULL
+    XeOperand s;                      // its rows: 1 ... 128 (or its columns, where s.along_rows is set)
+    float* out;                       // [parts][..]
+    long long out_s, out_m, plane;    // elements from one row of s to the next, along the other extent, between buffers
+    XeThinCut cut;
+    XeScale scale;
+    int* zero = nullptr;              // two device words set to 0, or NULL
+};
+int xe_thin(const XeThin& t, cudaStream_t st);
+// for `tiles` tiles of 128 and a contraction of `chunks` times 64, where a buffer costs `part_us`
+XeThinCut xe_thin_cut(long long tiles, long long chunks, double part_us);
+
 __device__ __forceinline__ float xe_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 constexpr float XE_LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// ties registers that tcgen05.ld fills to the wait before this: no use of them can be moved ahead of it
+__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                      "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 o = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&o);
+}
 
 // v = p0 + p1 + p2 with BF16 parts (each remainder is rounded to nearest, so three parts hold 24 bits).  A float that
 // rounds to BF16's infinity keeps its upper half instead; infinities and NaN stay in the first part.
@@ -134,5 +197,16 @@ __device__ __forceinline__ void xe_split3(float v, __nv_bfloat16& p0, __nv_bfloa
     p1 = __float2bfloat16_rn(r1);
     p2 = __float2bfloat16_rn(r1 - __bfloat162float(p1));
 }
+
+// Two floats at once, the first in the lower half of each part; neither may be infinite or round to infinity (NaN may be there).
+__device__ __forceinline__ void xe_split3_pair(float a, float b, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    const float2 less = make_float2(-1.f, -1.f);           // (products with -1 are exact)
+    p0 = pack_bf16(a, b);
+    const float2 r1 = __ffma2_rn(make_float2(__uint_as_float(p0 << 16), __uint_as_float(p0 & 0xffff0000u)), less, make_float2(a, b));
+    p1 = pack_bf16(r1.x, r1.y);
+    const float2 r2 = __ffma2_rn(make_float2(__uint_as_float(p1 << 16), __uint_as_float(p1 & 0xffff0000u)), less, r1);
+    p2 = pack_bf16(r2.x, r2.y);
+}
+constexpr float XE_SPLIT_MAX = 3.3895313892515355e38f;       // the largest BF16 value: floats up to it split like that
 
 }  // namespace wino

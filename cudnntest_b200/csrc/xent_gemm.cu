@@ -27,6 +27,15 @@
 
 namespace wino {
 
+// boxes of 64 columns (128 bytes, 128-byte swizzle): `share` rows for a K-major share, 64 rows (one contraction element each)
+// for an MN-major one
+int xe_operand_map(CUtensorMap* map, const XeOperand& o, unsigned share) {
+    const unsigned long long dims[3] = {(unsigned long long)o.cols, (unsigned long long)o.rows, (unsigned long long)o.planes};
+    const unsigned long long strides[2] = {(unsigned long long)o.pitch * 2, (unsigned long long)o.plane_pitch * 2};
+    const unsigned box[3] = {64u, o.along_rows ? 64u : share, 1u};
+    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1);
+}
+
 namespace {
 
 constexpr int XE_THREADS = 320;
@@ -35,7 +44,6 @@ constexpr int XE_STAGE_TILE = 32 * 128;              // epilogue staging: 32 row
 constexpr int XE_EPI_WARPS = 8;
 constexpr int XE_BAND = 8;
 
-enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
 
 struct alignas(64) XeProblem {
     CUtensorMap tm_a, tm_b, tm_out;
@@ -87,18 +95,6 @@ struct XeSmem {
     static constexpr int TOTAL = SLOT_OFF + 16 + 1024;
 };
 
-// MN-major tile with 128-byte swizzle: rows of 64 elements (128 bytes) along M or N, one row per contraction element,
-// groups of 8 contraction elements 1 KiB apart, blocks of 64 M / N elements 8 KiB apart
-__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
-    d |= (uint64_t)(8192 >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
 __device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
     asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
                  "r"(c0), "r"(c1), "r"(c2)
@@ -118,22 +114,6 @@ __device__ __forceinline__ void fma2(float& a, float& b, float c, float d) {
     const float2 r = __ffma2_rn(make_float2(a, b), make_float2(c, c), make_float2(d, d));
     a = r.x; b = r.y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-// ties registers that tcgen05.ld fills to the wait before this: no use of them can be moved ahead of it
-__device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
-    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                      "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-}
-
-__device__ __forceinline__ void prefetch_tensor_map(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
-
 // v[i] of lane l -> lane i returns the sum over lanes of v[i] (halving exchange, 31 shuffles); v is used up
 __device__ __forceinline__ float column_sums(float* v, int lane) {
 #pragma unroll
@@ -146,11 +126,6 @@ __device__ __forceinline__ float column_sums(float* v, int lane) {
         }
     }
     return v[0];
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 o = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&o);
 }
 
 template <int EPI, int PLANES, int BN>
@@ -649,20 +624,11 @@ int run(const XeParams& p, cudaStream_t st) {
     return WINO_OK;
 }
 
-// boxes of 64 columns (128 bytes, 128-byte swizzle): `share` rows for a K-major share, 64 rows (one contraction element each)
-// for an MN-major one
-int operand_map(CUtensorMap* map, const XeOperand& o, unsigned share) {
-    const unsigned long long dims[3] = {(unsigned long long)o.cols, (unsigned long long)o.rows, (unsigned long long)o.planes};
-    const unsigned long long strides[2] = {(unsigned long long)o.pitch * 2, (unsigned long long)o.plane_pitch * 2};
-    const unsigned box[3] = {64u, o.along_rows ? 64u : share, 1u};
-    return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, o.ptr, dims, strides, box, 1);
-}
-
 int make_problem(const XeProduct& x, XeProblem* out) {
     XeProblem& p = *out;
     const XeOutput& o = x.out;
     int rc;
-    if ((rc = operand_map(&p.tm_a, x.a, 128)) || (rc = operand_map(&p.tm_b, x.b, (unsigned)x.bn / 2))) return rc;
+    if ((rc = xe_operand_map(&p.tm_a, x.a, 128)) || (rc = xe_operand_map(&p.tm_b, x.b, (unsigned)x.bn / 2))) return rc;
     const bool f32 = x.epi == XE_F32 || x.epi == XE_STATS_Z;
     const int es = f32 ? 4 : 2;
     // a TMA store fills a row's last 16-byte unit with zeros behind the last column (measured), and wants such units as pitch

@@ -133,7 +133,7 @@ CASES = [
     (700, 1500, 1900, "bf16", {}),
     (1000, 40, 100, "fp32", {}),                                  # plain FP32 kernels up to their most rows and classes
     (3, 1001, 1024, "bf16", {}),
-    (16, 1001, 3000, "fp32", {}),                                 # few rows: FP32 arithmetic on the caller's matrices
+    (16, 1001, 3000, "fp32", {}),                                 # W split inside the products
     (9, 1001, 3000, "bf16", dict(bias=False)),
     (8, 1002, 3000, "bf16", {}),
     (3, 260, 70001, "fp32", dict(ldx=264, ldw=261)),
@@ -142,12 +142,12 @@ CASES = [
     (128, 128, 128, "fp32", {}),
     (9, 2050, 7, "fp32", dict(bias=False, ldx=2053, ldw=2052)),
     (7, 40, 128, "bf16", {}),
-    (3000, 3001, 3, "fp32", {}),                                  # few classes, the same kernels with the matrices exchanged
+    (3000, 3001, 3, "fp32", {}),                                  # few classes: FP32 arithmetic on the caller's matrices
     (2777, 1000, 16, "fp32", dict(ldx=1003, ldw=1001)),
     (9000, 260, 1, "fp32", {}),
     (300, 202, 1100, "bf16", {}),                                 # repacked by pairs
     (300, 600, 70, "bf16", dict(ldx=603, ldw=604)),
-    (17, 1001, 3000, "fp32", {}),                                 # one row more than that
+    (17, 1001, 3000, "fp32", {}),
     (64, 1001, 3000, "fp32", {}),
     (300, 2200, 700, "bf16", dict(bias=False)),                   # blocks of the contraction: 1024 + 1024 + 152
     (2100, 700, 2400, "fp32", {}),                                # 256 + 256 + 188, logits recomputed below
@@ -213,6 +213,44 @@ def test_forward_against_definition(n, d, v, dtype, smoothing):
     assert (np.abs(loss.double().cpu().numpy() - ref["loss"]) <= row).all()
     assert abs(float(mean[0]) - ref["loss"].mean()) <= row.mean() + 2 * F32 * abs(ref["loss"].mean())
     assert (np.abs(mean[1].double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
+
+
+# The longer float matrix split inside the products: W (one past and up to both widths of a tile of rows), or x with up to 128
+# classes; features, classes and rows that end inside a tile, a step of 64 and a block of 256; rows on any boundary; statistics
+# in one kernel and in two; more parts than one.  (8 rows: FP32 arithmetic instead.)
+LONG_W = [(8, 1001, 3001, {}), (9, 2001, 1000, {}), (17, 4099, 300, {}), (64, 2048, 1000, dict(ldw=2052)), (65, 1023, 2001, dict(ldw=1030, ldx=1027)),
+          (65, 1023, 17001, dict(ldw=1030, ldx=1027)), (128, 515, 8201, {}), (128, 2055, 8201, {}), (100, 64, 17000, dict(bias=False)),
+          (33, 20001, 130, dict(ldw=20004)), (127, 1000, 17841, dict(ldw=1001)), (128, 128, 8192, {}),
+          (3001, 1030, 17, {}), (2777, 1001, 64, dict(ldx=1003)), (1025, 1500, 33, dict(bias=False, ldx=1504)), (17001, 1000, 100, dict(ldw=1001)),
+          (8200, 2052, 128, {}), (131, 9001, 70, {})]
+
+
+@pytest.mark.parametrize("n,d,v,kw", LONG_W)
+@pytest.mark.parametrize("ignored,smoothing", [(0.0, 0.0), (0.3, 0.1)])
+def test_long_float_weight(n, d, v, kw, ignored, smoothing):
+    torch = _torch()
+    c = Case(n, d, v, "fp32", seed=101, ignored=ignored, **kw)
+    off = torch.from_numpy(c.t == -100).cuda()
+    c.x[off] = float("nan")
+    ref = c.oracle("mean", smoothing=smoothing)
+    plan = c.plan(reduction="mean", label_smoothing=smoothing, lddx=d + 1, lddw=d + 3)
+    bx, bw = torch.full((n + 1, d + 1), 5.0, device="cuda"), torch.full((v + 1, d + 3), 5.0, device="cuda")
+    got = plan.loss_and_grad(c.x, c.w, c.target, c.bias, dx=bx[:n, :d], dw=bw[:v, :d])
+    counts = c.t != -100
+    c.check(got, ref, "mean", counts / counts.sum(), smoothing=smoothing)
+    assert (bx[n:] == 5).all() and (bx[:, d:] == 5).all() and (bw[v:] == 5).all() and (bw[:, d:] == 5).all()
+    again = plan.loss_and_grad(c.x, c.w, c.target, c.bias)
+    assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(got, again))
+    only = plan.loss_and_grad(c.x, c.w, c.target, c.bias, need_dw=False)
+    assert only[2] is None and torch.equal(only[0], got[0]) and torch.equal(only[1], got[1])
+    loss, lse = c.plan(reduction="none", label_smoothing=smoothing, grad=False).forward(c.x, c.w, c.target, c.bias)
+    rows = c.oracle("none", smoothing)
+    ez, el, _ = c.z_error(rows)
+    keep = counts & np.isfinite(rows["lse"])
+    row = el + ez.max(1) + (8 + smoothing * v / 64) * F32 * (np.abs(rows["z"]).max(1) + np.abs(rows["lse"]))
+    assert (np.abs(loss.double().cpu().numpy() - rows["loss"])[keep] <= row[keep]).all() and (loss[off] == 0).all() and (lse[off] == 0).all()
+    import cudnntest_b200 as cb
+    cb.device_status()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
