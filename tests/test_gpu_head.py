@@ -253,6 +253,50 @@ def test_long_float_weight(n, d, v, kw, ignored, smoothing):
     cb.device_status()
 
 
+@pytest.mark.parametrize("n,d,v,ldx,ldw", [(20, 200, 6000, 0, 0), (20, 201, 6000, 0, 0), (6000, 200, 20, 0, 0), (6000, 200, 20, 203, 201)])
+def test_long_floats_near_the_largest_float(n, d, v, ldx, ldw):
+    """Floats that would round to BF16's infinity, in the matrix that is split inside the products."""
+    torch = _torch()
+    c = Case(n, d, v, "fp32", seed=111, ldx=ldx, ldw=ldw)
+    long, short = (c.w, c.x) if n < v else (c.x, c.w)
+    far = torch.tensor([3.4e38, -3.4e38, 3.3961775e38, 1.0], device="cuda")
+    long[:, 0] = far[torch.arange(long.shape[0], device="cuda") % 4]
+    short[:, 0] = 2.0 ** -100 * (1 + torch.arange(short.shape[0], device="cuda") / 64)
+    ref = c.oracle("none")
+    assert np.abs(ref["z"]).max() > 2.0 ** 27
+    loss, lse = c.plan(reduction="none", grad=False).forward(c.x, c.w, c.target, c.bias)
+    ez, el, _ = c.z_error(ref)
+    assert (np.abs(lse.double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
+    row = el + ez.max(1) + 8 * F32 * (np.abs(ref["z"]).max(1) + np.abs(ref["lse"]))
+    assert (np.abs(loss.double().cpu().numpy() - ref["loss"]) <= row).all()
+
+
+@pytest.mark.parametrize("n,d,v", [(40, 600, 3000), (3000, 600, 40)])
+def test_long_float_matrix_in_a_graph(n, d, v):
+    """A captured call, replayed on other values and beside an eager call on another stream: the same as eager."""
+    torch = _torch()
+    c = Case(n, d, v, "fp32", seed=121)
+    plan, other = c.plan(reduction="mean"), c.plan(reduction="mean")
+    plan.loss_and_grad(c.x, c.w, c.target, c.bias)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = plan.loss_and_grad(c.x, c.w, c.target, c.bias)
+    for _ in range(2):
+        c.x.mul_(0.75)
+        c.w.mul_(-1.25)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g.replay()
+        with torch.cuda.stream(side):
+            eager = other.loss_and_grad(c.x, c.w, c.target, c.bias)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, eager))
+    import cudnntest_b200 as cb
+    cb.device_status()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("n,d,v,limit", [(700, 130, 3000, 1), (2305, 40, 2100, 2305 * 2 * 600), (600, 1032, 11000, 1 << 20)])
 def test_pieces_of_the_vocabulary(dtype, n, d, v, limit):
