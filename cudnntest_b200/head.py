@@ -87,7 +87,8 @@ class LinearXent:
     bfloat16 parts, FP32-level accuracy); bias: v float32; target: n int64.  reduction "mean" (over the rows that count),
     "sum" or "none"; ignore_index: rows with that target leave no trace, whatever they hold.  The scratch is owned here
     (or handed in as ``workspace``); ``scratch_limit`` bounds the part that grows with n * v.  grad=False plans for
-    ``forward`` alone.  Calls that share a plan share its scratch: keep them on one stream or otherwise serialised.
+    ``forward`` alone, grad=True for both calls.  Calls that share a plan share its scratch: keep them on one stream or
+    otherwise serialised.
     """
 
     def __init__(self, n, d, v, dtype="bf16", bias=False, reduction="mean", ignore_index=None, label_smoothing=0.0,
@@ -100,9 +101,11 @@ class LinearXent:
         s.label_smoothing = label_smoothing
         s.ldx, s.ldw, s.lddx, s.lddw, s.scratch_limit = ldx, ldw, lddx, lddw, scratch_limit
         self.desc, self.grad, self.device = s, bool(grad), torch.device(device)
-        self.ws_bytes = lib().wino_xent_workspace_bytes(ctypes.byref(s), int(self.grad))
-        if self.ws_bytes == 0:
+        # forward plans for itself, and may need more than the gradient (whose dz counts against scratch_limit too)
+        needs = [lib().wino_xent_workspace_bytes(ctypes.byref(s), g) for g in ((0, 1) if self.grad else (0,))]
+        if 0 in needs:
             raise _lib.WinoError(_lib.E_BADARG, lib().wino_last_error_string().decode())
+        self.ws_bytes = max(needs)
         self.io_dtype = _TORCH_DTYPE[s.dtype]
         if workspace is not None and workspace.numel() * workspace.element_size() >= self.ws_bytes:
             self.workspace = workspace

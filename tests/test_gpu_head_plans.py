@@ -1,0 +1,46 @@
+"""Calls of the classifier head that go across plans, sizes and streams, against the definitions in 64 bits.
+
+Cases, bounds and their derivation are those of test_gpu_head.py.
+"""
+import numpy as np
+import pytest
+
+from test_gpu_head import F32, Case, _torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_forward(c, plan, reduction, smoothing=0.0):
+    """forward of a plan with reduction "mean", "sum" or "none" against the definition, element by element."""
+    loss, lse = (a.double().cpu().numpy() for a in plan.forward(c.x, c.w, c.target, c.bias))
+    ref = c.oracle("none", smoothing)
+    ez, el, _ = c.z_error(ref)
+    counts = np.ones(c.n, bool) if c.ignore_index is None else c.t != c.ignore_index
+    assert (np.abs(lse - ref["lse"]) <= (el + 2 * F32 * np.abs(ref["lse"])) * counts).all()
+    row = (el + ez.max(1) + (8 + smoothing * c.v / 64) * F32 * (np.abs(ref["z"]).max(1) + np.abs(ref["lse"]))) * counts
+    if reduction == "none":
+        assert (np.abs(loss - ref["loss"]) <= row).all()
+    else:
+        rows = max(1, counts.sum()) if reduction == "mean" else 1
+        want = ref["loss"].sum() / rows
+        assert abs(loss - want) <= row.sum() / rows + 2 * F32 * abs(want)
+
+
+@pytest.mark.parametrize("n,d,v,dtype,kw", [
+    (677, 1500, 1383, "bf16", dict(label_smoothing=0.1, scratch_limit=4 << 20)),  # forward keeps logits, the gradient does not
+    (1457, 1, 7119, "bf16", {}),                                                  # forward in the plain kernels
+    (58, 5, 4892, "fp32", dict(scratch_limit=1)),
+    (100, 2000, 300, "fp32", {}), (3, 40, 9, "bf16", {}),
+])
+def test_forward_of_a_plan_with_gradients(n, d, v, dtype, kw):
+    """Both calls on one plan, in either order: the loss alone, then with gradients, then alone again."""
+    torch = _torch()
+    c = Case(n, d, v, dtype, seed=131)
+    plan = c.plan(reduction="mean", **kw)
+    smoothing = kw.get("label_smoothing", 0.0)
+    first = plan.forward(c.x, c.w, c.target, c.bias)
+    got = plan.loss_and_grad(c.x, c.w, c.target, c.bias)
+    c.check(got, c.oracle("mean", smoothing), "mean", np.full(n, 1.0 / n), smoothing=smoothing)
+    again = plan.forward(c.x, c.w, c.target, c.bias)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    _check_forward(c, plan, "mean", smoothing)
