@@ -1120,6 +1120,10 @@ unsigned loop_blocks(long long items) {
 
 // ---- plan ----------------------------------------------------------------------------------------------------
 constexpr long long XE_SMALL_PRODUCTS = 16ll << 20;   // n v d up to which xe_small_* run
+// Most logits and rows of the plain loss alone, whose warps make eight logits each whatever d is.  Measured, plain against tensor
+// cores, BF16 / FP32X3, us: 512 x 64 x 100 10.4 / 11.2 against 10.6 / 13.4, 64 x 64 x 1000 10.2 / 11.6 against 10.0 / 13.2, 256 x 64 x 1000
+// 24.3 / 28.5 against 10.0 / 14.0, 2000 x 800 x 10 15.8 (BF16) against 14.3, 500000 x 9 x 3 510 / 581 against 313 / 382.
+constexpr long long XE_SMALL_LOGITS = 64ll << 10, XE_SMALL_ROWS_MAX = 1024;
 
 struct Plan {
     int planes, es, dp;
@@ -1222,7 +1226,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.few_rows = n <= XF_ROWS;
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
     const int few_splits = few_split_count(long_tiles, col_tiles);
-    p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : v <= XE_ROWS_MAX_V);
+    p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : n * v <= XE_SMALL_LOGITS && n <= XE_SMALL_ROWS_MAX && v <= XE_ROWS_MAX_V);
     // Measured with gradients, against tensor cores that split W themselves, us: 8 x 2048 x 4000 53.3 / 62.7, 8 x 2048 x 20000
     // 158 / 193, 8000 x 2048 x 8 102 / 129; the same kernels for 16 rows 16 x 2048 x 20000 256 / 197, 8000 x 2048 x 16 145 / 125.
     p.few = !bf16 && !p.small && n > 0 && (p.few_rows || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;

@@ -44,3 +44,12 @@ def test_forward_of_a_plan_with_gradients(n, d, v, dtype, kw):
     again = plan.forward(c.x, c.w, c.target, c.bias)
     assert all(torch.equal(a, b) for a, b in zip(first, again))
     _check_forward(c, plan, "mean", smoothing)
+
+
+@pytest.mark.parametrize("n,d,v", [(600000, 9, 3), (524281, 2, 1), (1 << 20, 1, 15), (1025, 16, 9), (1024, 16, 64), (40, 16, 1700), (600000, 2, 9)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_of_many_rows_with_few_products(n, d, v, dtype, reduction):
+    """Few products however many rows there are: to both sides of what the plain kernels take."""
+    c = Case(n, d, v, dtype, seed=141)
+    _check_forward(c, c.plan(reduction=reduction, grad=False), reduction)
