@@ -1226,7 +1226,11 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     p.few_rows = n <= XF_ROWS;
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
     const int few_splits = few_split_count(long_tiles, col_tiles);
-    p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : n * v <= XE_SMALL_LOGITS && n <= XE_SMALL_ROWS_MAX && v <= XE_ROWS_MAX_V);
+    const int small_splits = (d->d + XE_SMALL_SLICE - 1) / XE_SMALL_SLICE;
+    const long long piece_bytes = grad ? n * XE_BN * 2ll * p.planes : 0;        // the least that any gradient takes
+    const bool small_fits = z_bytes * small_splits <= (limit > piece_bytes ? limit : piece_bytes);
+    p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && small_fits &&
+              (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : n * v <= XE_SMALL_LOGITS && n <= XE_SMALL_ROWS_MAX && v <= XE_ROWS_MAX_V);
     // Measured with gradients, against tensor cores that split W themselves, us: 8 x 2048 x 4000 53.3 / 62.7, 8 x 2048 x 20000
     // 158 / 193, 8000 x 2048 x 8 102 / 129; the same kernels for 16 rows 16 x 2048 x 20000 256 / 197, 8000 x 2048 x 16 145 / 125.
     p.few = !bf16 && !p.small && n > 0 && (p.few_rows || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
@@ -1251,7 +1255,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     if (p.small) {
         p.kept = true;
         p.pack_x = p.pack_w = false;
-        p.splits_z = (d->d + XE_SMALL_SLICE - 1) / XE_SMALL_SLICE;
+        p.splits_z = small_splits;
     } else if (p.few) {
         p.kept = true;
         p.pack_x = p.pack_w = false;

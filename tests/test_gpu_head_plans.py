@@ -53,3 +53,14 @@ def test_loss_of_many_rows_with_few_products(n, d, v, dtype, reduction):
     """Few products however many rows there are: to both sides of what the plain kernels take."""
     c = Case(n, d, v, dtype, seed=141)
     _check_forward(c, c.plan(reduction=reduction, grad=False), reduction)
+
+
+@pytest.mark.parametrize("n,d,v,limit", [(1, 1, 1, 1), (7, 40, 9, 1), (128, 16, 64, 1), (100, 1001, 128, 1), (64, 16, 1000, 1000), (1, 1 << 14, 15, 100),
+                                         (8, 1000, 3000, 1000), (3000, 1000, 8, 1000), (100, 1030, 2000, 1 << 16)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_few_products_within_a_small_scratch(n, d, v, dtype, limit):
+    """A limit below what the plain kernels, those of few rows or classes, and the split inside take."""
+    c = Case(n, d, v, dtype, seed=151)
+    plan = c.plan(reduction="sum", scratch_limit=limit)
+    c.check(plan.loss_and_grad(c.x, c.w, c.target, c.bias), c.oracle("sum"), "sum", np.ones(n))
+    _check_forward(c, c.plan(reduction="mean", scratch_limit=limit, grad=False), "mean")

@@ -24,3 +24,47 @@ def test_a_plan_with_gradients_has_room_for_forward(n, d, v, kw):
     assert plan.ws_bytes >= need and plan.workspace.numel() >= need
     alone = cb.LinearXent(n, d, v, device="meta", grad=False, **kw)
     assert alone.ws_bytes == _bytes(alone, 0)
+
+
+def _round(a, q):
+    return -(-a // q) * q
+
+
+def _desc(n, d, v, dtype, limit, **kw):
+    s = cb.XentDesc()
+    s.n, s.d, s.v, s.dtype, s.scratch_limit = n, d, v, dtype, limit
+    for k, x in kw.items():
+        setattr(s, k, x)
+    return s
+
+
+@pytest.mark.parametrize("dtype", [cb.BF16, cb.FP32X3])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1])
+@pytest.mark.parametrize("limit", [1, 1000, 1 << 14, 1 << 20, 16 << 20, 1 << 28])
+def test_scratch_of_the_loss_alone_stays_within_the_limit(dtype, smoothing, limit):
+    """Beside scratch_limit: the statistics, five vectors over the rows, x and W repacked, and 256 bytes of rounding for each."""
+    L = cb.lib()
+    planes = 1 if dtype == cb.BF16 else 3
+    for n in (1, 8, 64, 128, 1000, 4096, 16384, 100000):
+        for d in (1, 9, 64, 2050, 1 << 14, 1 << 20):
+            for v in (1, 15, 128, 1000, 8192, 30000):
+                s = _desc(n, d, v, dtype, limit, label_smoothing=smoothing)
+                stats = -(-v // 128) * n * (8 if smoothing == 0 else 12)
+                packed = (n + v) * _round(d, 8) * 2 * planes
+                assert L.wino_xent_workspace_bytes(ctypes.byref(s), 0) <= limit + stats + 20 * n + packed + 12 * 256, (n, d, v)
+
+
+@pytest.mark.parametrize("dtype", [cb.BF16, cb.FP32X3])
+def test_small_gradients_keep_to_the_limit_or_to_a_piece(dtype):
+    """The plain kernels' logits, parts and column sums: within the limit, or what a piece of 256 classes of dz takes."""
+    L = cb.lib()
+    planes = 1 if dtype == cb.BF16 else 3
+    for n, d, v in ((128, 16, 64), (128, 1, 128), (1, 1 << 20, 15), (2, 1 << 18, 31), (7, 1 << 16, 33), (128, 1000, 128), (1, 1, 1)):
+        for limit in (1, 1 << 12, 1 << 15, 1 << 30):
+            for bias in (0,):
+                s = _desc(n, d, v, dtype, limit, has_bias=bias)
+                floor = n * 256 * 2 * planes
+                dx = 64 * (n + 256) * _round(d, 4) * 4             # at most 64 float parts of dx, and of 256 classes of dW
+                packed = (n + v) * _round(d, 8) * 2 * planes
+                got = L.wino_xent_workspace_bytes(ctypes.byref(s), 1)
+                assert got <= max(limit, floor) + -(-v // 128) * n * 8 + 20 * n + 14 * 256 + (0 if limit == 1 << 30 else packed + dx), (n, d, v, limit, bias)
