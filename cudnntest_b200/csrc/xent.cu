@@ -1220,20 +1220,23 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     const Cut cz = cut_product(n, v, kd, products, false);
     p.splits_z = cz.splits;
     p.zpitch = round_up(d->v, 4);
+    // what kept logits take beside them with gradients: dz, and the column sums of runs of rows
+    const int kept_parts = d->v <= XE_ROWS_MAX_V ? row_blocks(n, d->v) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
     const long long dz_bytes = n * round_up(d->v, 8) * 2ll * p.planes, z_bytes = n * p.zpitch * 4ll;
-    const bool fits = z_bytes * p.splits_z + (grad ? dz_bytes : 0) <= limit;
+    const long long db_bytes = grad && d->has_bias ? kept_parts * (round_up(d->v, 8) * 4ll) : 0, beside = (grad ? dz_bytes : 0) + db_bytes;
+    const bool fits = z_bytes * p.splits_z + beside <= limit;
     const bool few_tiles = n * v <= 64ll * XE_BM * XE_BN;
     p.few_rows = n <= XF_ROWS;
     const long long long_tiles = ((p.few_rows ? v : n) + XF_CLASSES - 1) / XF_CLASSES, col_tiles = (d->d + XF_COLS - 1) / XF_COLS;
     const int few_splits = few_split_count(long_tiles, col_tiles);
     const int small_splits = (d->d + XE_SMALL_SLICE - 1) / XE_SMALL_SLICE;
     const long long piece_bytes = grad ? n * XE_BN * 2ll * p.planes : 0;        // the least that any gradient takes
-    const bool small_fits = z_bytes * small_splits <= (limit > piece_bytes ? limit : piece_bytes);
+    const bool small_fits = z_bytes * small_splits + db_bytes <= (limit > piece_bytes ? limit : piece_bytes);
     p.small = n > 0 && n * v <= XE_SMALL_PRODUCTS / d->d && small_fits &&
               (grad ? n <= XE_SMALL_MAX && v <= XE_SMALL_MAX : n * v <= XE_SMALL_LOGITS && n <= XE_SMALL_ROWS_MAX && v <= XE_ROWS_MAX_V);
     // Measured with gradients, against tensor cores that split W themselves, us: 8 x 2048 x 4000 53.3 / 62.7, 8 x 2048 x 20000
     // 158 / 193, 8000 x 2048 x 8 102 / 129; the same kernels for 16 rows 16 x 2048 x 20000 256 / 197, 8000 x 2048 x 16 145 / 125.
-    p.few = !bf16 && !p.small && n > 0 && (p.few_rows || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits <= limit;
+    p.few = !bf16 && !p.small && n > 0 && (p.few_rows || v <= XF_ROWS) && (p.few_rows ? v : n) * d->d >= 2ll << 20 && z_bytes * few_splits + db_bytes <= limit;
     // Measured, the long matrix split inside against beforehand, us: loss of 64 x 512 x 1000 16.4 / 16.4, 64 x 2048 x 1000 18.5 / 22.6, 64 x 2048 x 4000
     // 25.2 / 46.7, 128 x 2048 x 20000 84 / 208; gradient of 64 x 512 x 1000 34.9 / 30.8, 64 x 4096 x 300 43.0 / 44.0, 64 x 2048 x 1000
     // 39.8 / 45.1, 64 x 2048 x 20000 207 / 322.  A tile of 128 rows takes the products apart that one launch would share:
@@ -1245,7 +1248,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     if (p.thin) {
         p.thin_z = xe_thin_cut((thin_m + 127) / 128, kd, (double)n * v * 8.0 / 5e6);
         p.thin_grad = xe_thin_cut(col_tiles, (thin_m + XE_BK - 1) / XE_BK, (double)thin_n * d->d * 8.0 / 5e6);
-        p.thin = z_bytes * p.thin_z.parts + (grad ? dz_bytes : 0) <= limit;
+        p.thin = z_bytes * p.thin_z.parts + beside <= limit;
     }
     p.tiny = p.small && v <= XE_SMALL_MAX && (v + XE_TINY_WARPS - 1) / XE_TINY_WARPS * ((d->d + 127) / 128) <= XE_TINY_STEPS;
     // Logits are kept where the product is split, or has too few tiles for the GPU.  Elsewhere kept floats cost 14 bytes a
@@ -1293,7 +1296,7 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // more than one piece adds up in floats: in dx itself, or in the scratch
     p.dx_direct = p.splits_dx == 1 && (p.pieces == 1 || !bf16);
     p.dw_direct = p.splits_dw == 1;
-    p.parts = p.kept && d->v <= XE_ROWS_MAX_V ? row_blocks(n, d->v) : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
+    p.parts = p.kept ? kept_parts : (int)((n + XE_ROWS_PER_PART - 1) / XE_ROWS_PER_PART);
     size_t off = 0;
     auto take = [&](size_t bytes) {
         const size_t at = off;

@@ -64,3 +64,13 @@ def test_few_products_within_a_small_scratch(n, d, v, dtype, limit):
     plan = c.plan(reduction="sum", scratch_limit=limit)
     c.check(plan.loss_and_grad(c.x, c.w, c.target, c.bias), c.oracle("sum"), "sum", np.ones(n))
     _check_forward(c, c.plan(reduction="mean", scratch_limit=limit, grad=False), "mean")
+
+
+@pytest.mark.parametrize("n,d,v,dtype,limit", [(1000, 1024, 9000, "bf16", 1000 * 9000 * 6), (2304, 300, 2050, "fp32", 2304 * 2052 * 10)])
+def test_kept_logits_at_the_edge_of_the_scratch(n, d, v, dtype, limit):
+    """Room for the logits and dz but not for dbias's column sums, and one with room for all three: the same gradient."""
+    c = Case(n, d, v, dtype, seed=161)
+    ref = c.oracle("mean")
+    for more in (0, 64 << 20):
+        got = c.plan(reduction="mean", scratch_limit=limit + more).loss_and_grad(c.x, c.w, c.target, c.bias)
+        c.check(got, ref, "mean", np.full(n, 1.0 / n))

@@ -54,6 +54,25 @@ def test_scratch_of_the_loss_alone_stays_within_the_limit(dtype, smoothing, limi
                 assert L.wino_xent_workspace_bytes(ctypes.byref(s), 0) <= limit + stats + 20 * n + packed + 12 * 256, (n, d, v)
 
 
+@pytest.mark.parametrize("n,d,v,dtype", [(4096, 1024, 9000, cb.BF16), (8192, 2048, 20000, cb.BF16), (4096, 256, 9000, cb.FP32X3), (2304, 1024, 2050, cb.BF16)])
+def test_column_sums_of_kept_logits_count_against_the_limit(n, d, v, dtype):
+    """Float logits (unsplit here: more tiles than CTA pairs), dz and the column sums for dbias are kept only where all three fit:
+    runs of 32 rows each behind 8192 classes, up to then at least one run per SM."""
+    L = cb.lib()
+    planes = 1 if dtype == cb.BF16 else 3
+    z, dz = n * _round(v, 4) * 4, n * _round(v, 8) * 2 * planes
+    sums = (-(-n // 32) if v > 8192 else 148) * _round(v, 8) * 4
+
+    def at(limit):
+        return L.wino_xent_workspace_bytes(ctypes.byref(_desc(n, d, v, dtype, limit, has_bias=1)), 1)
+    kept = at(1 << 60)
+    assert kept >= z + dz + sums
+    assert at(z + dz + sums - 1) < kept
+    no_bias = _desc(n, d, v, dtype, z + dz, has_bias=0)
+    if dtype == cb.FP32X3:                                        # without a bias there are no such sums
+        assert L.wino_xent_workspace_bytes(ctypes.byref(no_bias), 1) >= z + dz
+
+
 @pytest.mark.parametrize("dtype", [cb.BF16, cb.FP32X3])
 def test_small_gradients_keep_to_the_limit_or_to_a_piece(dtype):
     """The plain kernels' logits, parts and column sums: within the limit, or what a piece of 256 classes of dz takes."""
@@ -61,9 +80,9 @@ def test_small_gradients_keep_to_the_limit_or_to_a_piece(dtype):
     planes = 1 if dtype == cb.BF16 else 3
     for n, d, v in ((128, 16, 64), (128, 1, 128), (1, 1 << 20, 15), (2, 1 << 18, 31), (7, 1 << 16, 33), (128, 1000, 128), (1, 1, 1)):
         for limit in (1, 1 << 12, 1 << 15, 1 << 30):
-            for bias in (0,):
+            for bias in (0, 1):
                 s = _desc(n, d, v, dtype, limit, has_bias=bias)
-                floor = n * 256 * 2 * planes
+                floor = n * 256 * 2 * planes + (-(-n // 32)) * 256 * 4 * bias
                 dx = 64 * (n + 256) * _round(d, 4) * 4             # at most 64 float parts of dx, and of 256 classes of dW
                 packed = (n + v) * _round(d, 8) * 2 * planes
                 got = L.wino_xent_workspace_bytes(ctypes.byref(s), 1)
