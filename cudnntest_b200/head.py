@@ -88,7 +88,7 @@ class LinearXent:
     "sum" or "none"; ignore_index: rows with that target leave no trace, whatever they hold.  The scratch is owned here
     (or handed in as ``workspace``); ``scratch_limit`` bounds the part that grows with n * v.  grad=False plans for
     ``forward`` alone, grad=True for both calls.  Calls that share a plan share its scratch: keep them on one stream or
-    otherwise serialised.
+    otherwise serialised.  A graph that holds a call needs the plan for as long as it is replayed.
     """
 
     def __init__(self, n, d, v, dtype="bf16", bias=False, reduction="mean", ignore_index=None, label_smoothing=0.0,
@@ -113,6 +113,7 @@ class LinearXent:
             self.workspace = torch.empty(self.ws_bytes, dtype=torch.uint8, device=self.device)
         self._desc_ref, self._ws_size = ctypes.byref(s), self.workspace.numel() * self.workspace.element_size()
         self._index = self.workspace.get_device()
+        self._made_on = _raw_stream(self._index) if self._index >= 0 else None
         self._forms = [(torch.Size((rows, d)), (ld or d, 1)) for rows, ld in ((n, ldx), (v, ldw), (n, lddx), (v, lddw))]
         # what results are allocated like
         self._lse_like = torch.empty(n, dtype=torch.float32, device=self.workspace.device)
@@ -137,6 +138,12 @@ class LinearXent:
             raise ValueError("%s must be %d contiguous %s values on the plan's device" % (what, count, dtype))
         return t.data_ptr()
 
+    def _scratch(self):
+        """(address, bytes) of the scratch, which the allocator keeps for the current stream's work even if the plan is dropped."""
+        if _raw_stream(self._index) != self._made_on:
+            self.workspace.record_stream(torch.cuda.current_stream(self._index))
+        return self.workspace.data_ptr(), self._ws_size
+
     def _inputs(self, x, w, target, bias):
         s = self.desc
         if self._index < 0:
@@ -150,8 +157,7 @@ class LinearXent:
         """(loss, lse): loss is a scalar (or n values), lse_i = log sum_j exp z_ij (0 for an ignored row)."""
         args = self._inputs(x, w, target, bias)
         loss, lse = torch.empty_like(self._loss_like), torch.empty_like(self._lse_like)
-        _call(lib().wino_xent_forward, self._index, self._desc_ref, *args, loss.data_ptr(), lse.data_ptr(), self.workspace.data_ptr(),
-              self._ws_size)
+        _call(lib().wino_xent_forward, self._index, self._desc_ref, *args, loss.data_ptr(), lse.data_ptr(), *self._scratch())
         return loss, lse
 
     def loss_and_grad(self, x, w, target, bias=None, dloss=None, dx=None, dw=None, need_dx=True, need_dw=True):
@@ -182,5 +188,5 @@ class LinearXent:
         db = torch.empty_like(bias) if s.has_bias else None
         loss = torch.empty_like(self._loss_like)
         _call(lib().wino_xent_grad, self._index, self._desc_ref, *args, dloss, loss.data_ptr(), None, dx_ptr, dw_ptr,
-              None if db is None else db.data_ptr(), self.workspace.data_ptr(), self._ws_size)
+              None if db is None else db.data_ptr(), *self._scratch())
         return loss, dx, dw, db

@@ -74,3 +74,30 @@ def test_kept_logits_at_the_edge_of_the_scratch(n, d, v, dtype, limit):
     for more in (0, 64 << 20):
         got = c.plan(reduction="mean", scratch_limit=limit + more).loss_and_grad(c.x, c.w, c.target, c.bias)
         c.check(got, ref, "mean", np.full(n, 1.0 / n))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_plan_dropped_while_a_side_stream_uses_it(grad):
+    """The scratch of a plan whose call still waits on a side stream is not handed out again before that call is over."""
+    torch = _torch()
+    c = Case(300, 512, 1000, "bf16", seed=171)
+    plan = c.plan(reduction="mean", grad=grad)
+
+    def call():
+        return plan.loss_and_grad(c.x, c.w, c.target, c.bias) if grad else plan.forward(c.x, c.w, c.target, c.bias)
+    want = call()
+    torch.cuda.synchronize()
+    at, size = plan.workspace.data_ptr(), plan.workspace.numel()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)                            # about a tenth of a second
+        got = call()
+    del plan
+    others = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    early = not side.query()
+    if early:                                                     # else the host was held up, and nothing can be said
+        assert all(o.data_ptr() + size <= at or at + size <= o.data_ptr() for o in others)
+    for o in others:
+        o.fill_(255)
+    side.synchronize()
+    assert early and all(torch.equal(a, b) for a, b in zip(got, want))

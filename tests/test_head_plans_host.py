@@ -87,3 +87,33 @@ def test_small_gradients_keep_to_the_limit_or_to_a_piece(dtype):
                 packed = (n + v) * _round(d, 8) * 2 * planes
                 got = L.wino_xent_workspace_bytes(ctypes.byref(s), 1)
                 assert got <= max(limit, floor) + -(-v // 128) * n * 8 + 20 * n + 14 * 256 + (0 if limit == 1 << 30 else packed + dx), (n, d, v, limit, bias)
+
+
+def test_scratch_is_kept_for_the_stream_that_uses_it(monkeypatch):
+    """A call on another stream than the plan's own tells the allocator, so that a plan dropped while the call runs does not hand
+    its scratch to somebody else."""
+    import torch
+    from cudnntest_b200 import head
+    plan = cb.LinearXent(8, 16, 10, device="meta")
+    told, now = [], [5]
+
+    class Scratch:
+        def data_ptr(self):
+            return 1 << 20
+
+        def record_stream(self, stream):
+            told.append(stream)
+    monkeypatch.setattr(head, "_raw_stream", lambda index: now[0])
+    monkeypatch.setattr(head, "_call", lambda *args: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: now[0])
+    monkeypatch.setattr(plan, "_inputs", lambda *args: (0, 0, None, 0))
+    plan.workspace, plan._index, plan._made_on = Scratch(), 0, 5
+    x, w = torch.empty(8, 16, dtype=torch.bfloat16, device="meta"), torch.empty(10, 16, dtype=torch.bfloat16, device="meta")
+    for call in (lambda: plan.forward(x, w, None), lambda: plan.loss_and_grad(x, w, None, need_dx=False, need_dw=False)):
+        told.clear()
+        now[0] = 5
+        call()
+        assert told == []
+        now[0] = 6
+        call()
+        assert told == [6]
