@@ -94,12 +94,14 @@ class LinearXent:
     def __init__(self, n, d, v, dtype="bf16", bias=False, reduction="mean", ignore_index=None, label_smoothing=0.0,
                  grad=True, ldx=0, ldw=0, lddx=0, lddw=0, scratch_limit=0, device="cuda", workspace=None):
         s = XentDesc()
-        s.n, s.d, s.v = n, d, v
-        s.dtype, s.reduction = _code(DTYPE_CODES, dtype), _code(REDUCTION_CODES, reduction)
-        s.has_bias, s.has_ignore = int(bias), int(ignore_index is not None)
-        s.ignore_index = 0 if ignore_index is None else ignore_index
+        fields = dict(n=n, d=d, v=v, dtype=_code(DTYPE_CODES, dtype), reduction=_code(REDUCTION_CODES, reduction), has_bias=int(bias),
+                      has_ignore=int(ignore_index is not None), ignore_index=0 if ignore_index is None else ignore_index,
+                      ldx=ldx, ldw=ldw, lddx=lddx, lddw=lddw, scratch_limit=scratch_limit)
+        for name, value in fields.items():
+            setattr(s, name, value)
+            if getattr(s, name) != value:       # ctypes keeps the lower bits without a word
+                raise ValueError("%s = %d does not fit wino_xent_desc" % (name, value))
         s.label_smoothing = label_smoothing
-        s.ldx, s.ldw, s.lddx, s.lddw, s.scratch_limit = ldx, ldw, lddx, lddw, scratch_limit
         self.desc, self.grad, self.device = s, bool(grad), torch.device(device)
         # forward plans for itself, and may need more than the gradient (whose dz counts against scratch_limit too)
         needs = [lib().wino_xent_workspace_bytes(ctypes.byref(s), g) for g in ((0, 1) if self.grad else (0,))]

@@ -117,3 +117,13 @@ def test_scratch_is_kept_for_the_stream_that_uses_it(monkeypatch):
         now[0] = 6
         call()
         assert told == [6]
+
+
+@pytest.mark.parametrize("kw", [dict(n=2 ** 32 + 8), dict(n=2 ** 31), dict(d=2 ** 32 + 16), dict(v=2 ** 32 + 10), dict(v=-2 ** 32 + 10), dict(reduction=2 ** 32),
+                                dict(ignore_index=2 ** 64 + 3), dict(ignore_index=2 ** 63), dict(ldx=2 ** 64 + 16), dict(scratch_limit=2 ** 64)])
+def test_numbers_that_the_descriptor_cannot_hold(kw):
+    """They are refused: taken modulo 2^32 or 2^64 they would be another plan for tensors of these sizes."""
+    with pytest.raises(ValueError):
+        cb.LinearXent(**{**dict(n=8, d=16, v=10, device="meta"), **kw})
+    plan = cb.LinearXent(8, 16, 10, device="meta", ignore_index=-2 ** 63)
+    assert plan.desc.ignore_index == -2 ** 63
