@@ -109,6 +109,8 @@ class LinearXent:
             raise _lib.WinoError(_lib.E_BADARG, lib().wino_last_error_string().decode())
         self.ws_bytes = max(needs)
         self.io_dtype = _TORCH_DTYPE[s.dtype]
+        if workspace is not None and not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         if workspace is not None and workspace.numel() * workspace.element_size() >= self.ws_bytes:
             self.workspace = workspace
         else:

@@ -127,3 +127,16 @@ def test_numbers_that_the_descriptor_cannot_hold(kw):
         cb.LinearXent(**{**dict(n=8, d=16, v=10, device="meta"), **kw})
     plan = cb.LinearXent(8, 16, 10, device="meta", ignore_index=-2 ** 63)
     assert plan.desc.ignore_index == -2 ** 63
+
+
+def test_handed_in_scratch_is_contiguous():
+    """A tensor whose elements share memory has less of it than it has elements."""
+    import torch
+    plan = cb.LinearXent(8, 16, 10, device="meta")
+    for strided in (torch.empty(1, dtype=torch.uint8, device="meta").expand(plan.ws_bytes), torch.empty(2 * plan.ws_bytes, dtype=torch.uint8, device="meta")[::2]):
+        with pytest.raises(ValueError):
+            cb.LinearXent(8, 16, 10, device="meta", workspace=strided)
+    own = torch.empty(plan.ws_bytes // 4 + 1, dtype=torch.float32, device="meta")
+    assert cb.LinearXent(8, 16, 10, device="meta", workspace=own).workspace is own
+    small = torch.empty(8, dtype=torch.uint8, device="meta")
+    assert cb.LinearXent(8, 16, 10, device="meta", workspace=small).workspace is not small
