@@ -157,7 +157,7 @@ class ClassifierHead:
     What a program fits on frozen convolutions, and the last layer of the reference's network (fc16 + softmax,
     netTest/cudnn_test_0124/VGG_Batched/Network.h:668-704) with the dropout that its training puts before it.  Takes the
     output of ``VGG16ConvStack`` as it comes, flattened per image in the stack's NHWC or NCHW order (CHWN has the images
-    innermost: relay it out first).  Weights are seeded; ``weight`` (classes, features) and ``bias`` may be overwritten."""
+    innermost: relay it out first; it is refused where its first axis shows that).  Weights are seeded; ``weight`` (classes, features) and ``bias`` may be overwritten."""
 
     def __init__(self, batch, features, classes, dtype="bf16", p=0.5, ignore_index=None, label_smoothing=0.0, seed=0xC0DE0041,
                  device="cuda"):
@@ -170,10 +170,10 @@ class ClassifierHead:
         self.bias = torch.zeros(classes, dtype=torch.float32, device=device)
 
     def _flat(self, features):
-        x = features.reshape(self.batch, -1)
-        if x.shape[1] != self.features:
-            raise ValueError("%d features per image, the head was made for %d" % (x.shape[1], self.features))
-        return x
+        shape = tuple(features.shape)
+        if shape[:1] != (self.batch,) or math.prod(shape[1:]) != self.features:
+            raise ValueError("features %s: the head was made for %d images, one after the other, of %d features" % (shape, self.batch, self.features))
+        return features.reshape(self.batch, self.features)
 
     def loss(self, features, target):
         """Mean cross entropy, without dropout."""

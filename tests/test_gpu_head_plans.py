@@ -101,3 +101,14 @@ def test_plan_dropped_while_a_side_stream_uses_it(grad):
         o.fill_(255)
     side.synchronize()
     assert early and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_classifier_head_of_no_images():
+    torch = _torch()
+    from cudnntest_b200 import vgg
+    head_ = vgg.ClassifierHead(0, 16, 10)
+    feats = torch.empty((0, 2, 2, 4), dtype=torch.bfloat16, device="cuda")
+    target = torch.empty(0, dtype=torch.int64, device="cuda")
+    assert float(head_.loss(feats, target)) == 0
+    loss, dx, dw, db = head_.loss_and_grad(feats, target, need_dx=True)
+    assert float(loss) == 0 and dx.shape == feats.shape and (dw == 0).all() and (db == 0).all()

@@ -140,3 +140,24 @@ def test_handed_in_scratch_is_contiguous():
     assert cb.LinearXent(8, 16, 10, device="meta", workspace=own).workspace is own
     small = torch.empty(8, dtype=torch.uint8, device="meta")
     assert cb.LinearXent(8, 16, 10, device="meta", workspace=small).workspace is not small
+
+
+def test_classifier_head_takes_images_first():
+    """Features whose first axis is not the batch (a CHWN stack's output) would be flattened across images."""
+    import torch
+    from cudnntest_b200 import vgg
+    head_ = vgg.ClassifierHead(6, 4 * 2 * 2, 10, device="meta")
+    for shape in ((6, 16), (6, 2, 2, 4), (6, 4, 2, 2)):
+        assert head_._flat(torch.empty(shape, dtype=torch.bfloat16, device="meta")).shape == (6, 16)
+    for shape in ((4, 2, 2, 6), (16, 6), (96,), (6, 15), (7, 16), (6, 2, 2, 5), (2, 3, 16), ()):
+        with pytest.raises(ValueError):
+            head_._flat(torch.empty(shape, dtype=torch.bfloat16, device="meta"))
+
+
+def test_classifier_head_of_no_images():
+    import torch
+    from cudnntest_b200 import vgg
+    head_ = vgg.ClassifierHead(0, 16, 10, device="meta")
+    assert head_._flat(torch.empty((0, 2, 2, 4), dtype=torch.bfloat16, device="meta")).shape == (0, 16)
+    with pytest.raises(ValueError):
+        head_._flat(torch.empty((0, 2, 2, 5), dtype=torch.bfloat16, device="meta"))
