@@ -142,10 +142,15 @@ class LinearXent:
             raise ValueError("%s must be %d contiguous %s values on the plan's device" % (what, count, dtype))
         return t.data_ptr()
 
+    def _keep(self, *tensors):
+        """The allocator keeps them for the current stream's work, even if their owner is dropped."""
+        if self._index >= 0 and _raw_stream(self._index) != self._made_on:
+            stream = torch.cuda.current_stream(self._index)
+            for t in tensors:
+                t.record_stream(stream)
+
     def _scratch(self):
-        """(address, bytes) of the scratch, which the allocator keeps for the current stream's work even if the plan is dropped."""
-        if _raw_stream(self._index) != self._made_on:
-            self.workspace.record_stream(torch.cuda.current_stream(self._index))
+        self._keep(self.workspace)
         return self.workspace.data_ptr(), self._ws_size
 
     def _inputs(self, x, w, target, bias):

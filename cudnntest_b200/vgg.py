@@ -157,17 +157,29 @@ class ClassifierHead:
     What a program fits on frozen convolutions, and the last layer of the reference's network (fc16 + softmax,
     netTest/cudnn_test_0124/VGG_Batched/Network.h:668-704) with the dropout that its training puts before it.  Takes the
     output of ``VGG16ConvStack`` as it comes, flattened per image in the stack's NHWC or NCHW order (CHWN has the images
-    innermost: relay it out first; it is refused where its first axis shows that).  Weights are seeded; ``weight`` (classes, features) and ``bias`` may be overwritten."""
+    innermost: relay it out first; it is refused where its first axis shows that).  Weights are seeded; ``weight`` (classes, features) and
+    ``bias`` may be overwritten.  ``loss`` and ``loss_and_grad`` share their scratch and the number of the mask: keep them on one
+    stream or otherwise serialised."""
 
     def __init__(self, batch, features, classes, dtype="bf16", p=0.5, ignore_index=None, label_smoothing=0.0, seed=0xC0DE0041,
                  device="cuda"):
-        self.batch, self.features, self.classes, self.p, self.seed, self.steps = batch, features, classes, p, seed, 0
+        self.batch, self.features, self.classes, self.p, self.seed = batch, features, classes, p, seed
+        self._step = torch.zeros(1, dtype=torch.int64, device=device)     # on the device: a replayed graph advances it too
         common = dict(dtype=dtype, bias=True, reduction="mean", ignore_index=ignore_index, label_smoothing=label_smoothing, device=device)
         self.plan = LinearXent(batch, features, classes, **common)
         self.eval_plan = LinearXent(batch, features, classes, grad=False, workspace=self.plan.workspace, **common)
         gen = torch.Generator(device="cpu").manual_seed(seed)
         self.weight = (torch.randn((classes, features), generator=gen) * math.sqrt(1.0 / features)).to(self.plan.io_dtype).to(device)
         self.bias = torch.zeros(classes, dtype=torch.float32, device=device)
+
+    @property
+    def steps(self):
+        """Number of the next call's dropout mask (its offset); reading it synchronises."""
+        return int(self._step.item())
+
+    @steps.setter
+    def steps(self, number):
+        self._step.fill_(number)
 
     def _flat(self, features):
         shape = tuple(features.shape)
@@ -177,13 +189,17 @@ class ClassifierHead:
 
     def loss(self, features, target):
         """Mean cross entropy, without dropout."""
-        return self.eval_plan.forward(self._flat(features), self.weight, target, self.bias)[0]
+        x = self._flat(features)
+        self.plan._keep(self.weight, self.bias)
+        return self.eval_plan.forward(x, self.weight, target, self.bias)[0]
 
     def loss_and_grad(self, features, target, need_dx=False):
-        """(loss, gradient of the features or None, of the weight, of the bias); every call draws its own dropout mask."""
-        x, step = self._flat(features), self.steps
-        self.steps += 1
-        h = dropout(x, self.p, self.seed, step)
+        """(loss, gradient of the features or None, of the weight, of the bias); every call, and every replay of a captured
+        one, draws its own dropout mask."""
+        x = self._flat(features)
+        self.plan._keep(self._step, self.weight, self.bias)
+        h = dropout(x, self.p, self.seed, offset_dev=self._step)
         loss, dh, dw, db = self.plan.loss_and_grad(h, self.weight, target, self.bias, need_dx=need_dx)
-        dx = dropout_backward(dh, self.p, self.seed, step, out=dh).view(features.shape) if need_dx else None
+        dx = dropout_backward(dh, self.p, self.seed, offset_dev=self._step, out=dh).view(features.shape) if need_dx else None
+        self._step.add_(1)
         return loss, dx, dw, db

@@ -112,3 +112,30 @@ def test_classifier_head_of_no_images():
     assert float(head_.loss(feats, target)) == 0
     loss, dx, dw, db = head_.loss_and_grad(feats, target, need_dx=True)
     assert float(loss) == 0 and dx.shape == feats.shape and (dw == 0).all() and (db == 0).all()
+
+
+def test_captured_classifier_step_draws_a_mask_per_replay():
+    """Every replay has the mask of its number, as eager calls before and after it do."""
+    torch = _torch()
+    from cudnntest_b200 import vgg
+    from oracle import head
+    head_ = vgg.ClassifierHead(20, 512, 30, dtype="fp32x3")
+    feats = torch.rand((20, 512), device="cuda") + 0.5
+    target = torch.arange(20, device="cuda")
+
+    def mask(step):
+        return torch.from_numpy(head.dropout_keep(0, feats.numel(), 0.5, head_.seed, step).reshape(20, 512)).cuda()
+
+    assert torch.equal(head_.loss_and_grad(feats, target, need_dx=True)[1] != 0, mask(0))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = head_.loss_and_grad(feats, target, need_dx=True)
+    for step in (1, 2, 3):
+        g.replay()
+        assert torch.equal(got[1] != 0, mask(step))
+        plain = vgg.ClassifierHead(20, 512, 30, dtype="fp32x3")
+        plain.steps = step
+        assert all(torch.equal(a, b) for a, b in zip(got, plain.loss_and_grad(feats, target, need_dx=True)))
+    assert head_.steps == 4
+    assert torch.equal(head_.loss_and_grad(feats, target, need_dx=True)[1] != 0, mask(4))

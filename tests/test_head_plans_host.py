@@ -161,3 +161,24 @@ def test_classifier_head_of_no_images():
     assert head_._flat(torch.empty((0, 2, 2, 4), dtype=torch.bfloat16, device="meta")).shape == (0, 16)
     with pytest.raises(ValueError):
         head_._flat(torch.empty((0, 2, 2, 5), dtype=torch.bfloat16, device="meta"))
+
+
+def test_classifier_head_keeps_what_it_owns_for_the_stream(monkeypatch):
+    import torch
+    from cudnntest_b200 import head, vgg
+    head_ = vgg.ClassifierHead(6, 16, 10, device="meta")
+    x, t = torch.empty((6, 16), dtype=torch.bfloat16, device="meta"), torch.empty(6, dtype=torch.int64, device="meta")
+    for call in (head_.loss, head_.loss_and_grad):                # no GPU: refused
+        with pytest.raises(ValueError):
+            call(x, t)
+    head_.plan._index = 0
+    told = []
+    monkeypatch.setattr(head, "_raw_stream", lambda index: 6)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: 6)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, stream: told.append(id(self)))
+    owned = {id(head_.weight), id(head_.bias)}
+    for call, want in ((head_.loss, owned), (head_.loss_and_grad, owned | {id(head_._step)})):
+        told.clear()
+        with pytest.raises(ValueError):
+            call(x, t)
+        assert want <= set(told)
