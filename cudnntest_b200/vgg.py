@@ -185,7 +185,7 @@ class ClassifierHead:
         shape = tuple(features.shape)
         if shape[:1] != (self.batch,) or math.prod(shape[1:]) != self.features:
             raise ValueError("features %s: the head was made for %d images, one after the other, of %d features" % (shape, self.batch, self.features))
-        return features.reshape(self.batch, self.features)
+        return features.reshape(self.batch, self.features).contiguous()
 
     def loss(self, features, target):
         """Mean cross entropy, without dropout."""

@@ -139,3 +139,15 @@ def test_captured_classifier_step_draws_a_mask_per_replay():
         assert all(torch.equal(a, b) for a, b in zip(got, plain.loss_and_grad(feats, target, need_dx=True)))
     assert head_.steps == 4
     assert torch.equal(head_.loss_and_grad(feats, target, need_dx=True)[1] != 0, mask(4))
+
+
+def test_classifier_head_on_features_inside_wider_rows():
+    torch = _torch()
+    from cudnntest_b200 import vgg
+    wide = torch.randn((20, 40), device="cuda", dtype=torch.bfloat16)
+    target = torch.arange(20, device="cuda")
+    a, b = (vgg.ClassifierHead(20, 32, 30) for _ in range(2))
+    x = wide[:, :32]
+    assert torch.equal(a.loss(x, target), b.loss(x.clone(), target))
+    for got, want in zip(a.loss_and_grad(x, target, need_dx=True), b.loss_and_grad(x.clone(), target, need_dx=True)):
+        assert torch.equal(got, want)

@@ -182,3 +182,13 @@ def test_classifier_head_keeps_what_it_owns_for_the_stream(monkeypatch):
         with pytest.raises(ValueError):
             call(x, t)
         assert want <= set(told)
+
+
+def test_classifier_head_takes_features_inside_wider_rows():
+    """loss took only contiguous ones, loss_and_grad any pitch."""
+    import torch
+    from cudnntest_b200 import vgg
+    head_ = vgg.ClassifierHead(6, 16, 10, device="meta")
+    for x in (torch.empty((6, 24), dtype=torch.bfloat16, device="meta")[:, :16], torch.empty((16, 6), dtype=torch.bfloat16, device="meta").t(),
+              torch.empty((6, 2, 2, 8), dtype=torch.bfloat16, device="meta")[..., :4]):
+        assert head_._flat(x).is_contiguous() and head_._flat(x).shape == (6, 16)
