@@ -192,3 +192,24 @@ def test_classifier_head_takes_features_inside_wider_rows():
     for x in (torch.empty((6, 24), dtype=torch.bfloat16, device="meta")[:, :16], torch.empty((16, 6), dtype=torch.bfloat16, device="meta").t(),
               torch.empty((6, 2, 2, 8), dtype=torch.bfloat16, device="meta")[..., :4]):
         assert head_._flat(x).is_contiguous() and head_._flat(x).shape == (6, 16)
+
+
+def test_the_documented_c_example_compiles(tmp_path):
+    """INTEGRATION.md's calls, with every tensor declared as what the text says it is (device memory: pointers)."""
+    import os
+    import re
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    cc = shutil.which("gcc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    text = open(os.path.join(root, "INTEGRATION.md")).read()
+    code = re.search(r"## 5\..*?```c\n(.*?)```", text, re.S).group(1)
+    (tmp_path / "example.c").write_text('#include <stddef.h>\n#include "wino.h"\n'
+                                        "void example(int images, int classes, unsigned long long seed, unsigned long long step, void* features, void* h,\n"
+                                        "             void* dh, void* dfeatures, void* weight, void* dweight, float* bias, float* dbias, float* loss,\n"
+                                        "             long long* labels, void* workspace, wino_stream_t stream) {\n" + code + "(void)bytes;\n}\n")
+    r = subprocess.run([cc, "-std=c11", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(root, "include"), "example.c"], cwd=tmp_path,
+                       capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
