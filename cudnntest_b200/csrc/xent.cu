@@ -7,7 +7,7 @@
 //     cheaper than a fourth product.  FP32X3 with up to 128 rows or classes: the longer matrix is split into BF16 parts
 //     inside its products (xent_thin.cu), the others beforehand;
 //   * as exponentials: BF16 without a bias whose dz fits the scratch.  The logits product leaves a maximum and a sum per
-//     row and 128 classes and exp(z - maximum) as BF16 in the place of dz; one pass over it makes dz.  Three products
+//     row and 128 classes and exp(z - maximum) in 16 bits in the place of dz; one pass over it makes dz.  Three products
 //     (2 n v d flops each) in all these ways;
 //   * recomputed: the logits product leaves only the statistics; the gradient then walks the vocabulary in pieces, computes
 //     a piece's logits again, turns them into dz in the epilogue, and multiplies dz into dx and dW before the next piece:
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(128) xe_wide_dz_kernel(const float* z, int v, 
 }
 
 // exponentials (kept in the place of dz) -> dz, eight classes per thread.  The target's probability comes from its logit in
-// FP32, the others' from the rounded exponential: off by one more BF16 rounding.
+// FP32, the others' from the exponential in 16 bits (xe_pack_exp): off by 2^-10 before dz itself is rounded.
 __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __restrict__ dz, int pitch, long long n, const float2* __restrict__ stats,
                                                              const float* __restrict__ zt, const float* __restrict__ lse, const float* __restrict__ rowg,
                                                              const long long* __restrict__ target, const XeDzRule rule) {
@@ -642,8 +642,7 @@ __global__ void __launch_bounds__(256) xe_dz_from_exp_kernel(__nv_bfloat16* __re
             uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 z = __ffma2_rn(make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)), make_float2(h, h),
-                                            make_float2(-ga, -ga));
+                const float2 z = __ffma2_rn(xe_unpack_exp(w[e]), make_float2(h, h), make_float2(-ga, -ga));
                 const __nv_bfloat162 v = __floats2bfloat162_rn(z.x, z.y);
                 w[e] = *reinterpret_cast<const uint32_t*>(&v);
             }
@@ -1133,7 +1132,7 @@ struct Plan {
     bool thin, thin_rows;                // W (up to 128 rows) or x (up to 128 classes) is split inside the products (xe_thin)
     XeThinCut thin_z, thin_grad;
     int splits_few;                      // of the gradient of the matrix of few rows
-    bool kept, exps;                     // floats of all logits, BF16 exponentials of all logits (else recomputed by piece)
+    bool kept, exps;                     // floats of all logits, exponentials of all logits in 16 bits (else recomputed by piece)
     int splits_z, splits_dx, splits_dw, bn_z, bn_dx, bn_dw;
     int zpitch, piece, pieces, dzpitch, parts;
     bool dx_direct, dw_direct;           // the product's epilogue stores the caller's matrix

@@ -41,7 +41,7 @@ enum XeEpilogue {
     XE_F32 = 0,       // scale, store floats or add them to what is there
     XE_BF16 = 1,      // scale, round and store
     XE_STATS = 2,     // per row and 128 columns: maximum, sum of exponentials (and of logits); the target's logit
-    XE_STATS_E = 3,   // the same, and the exponentials exp(z - maximum) themselves, rounded to BF16
+    XE_STATS_E = 3,   // the same, and the exponentials exp(z - maximum) themselves, in 16 bits (xe_pack_exp)
     XE_STATS_Z = 4,   // the same as XE_STATS, and the logits themselves (with the bias) as floats
     XE_DZ = 5,        // the gradient of the logits, rounded to BF16 (or split into three BF16 planes), and its column sums
 };
@@ -182,6 +182,16 @@ __device__ __forceinline__ void after_wait(uint32_t (&r)[16]) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 o = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&o);
+}
+
+// Two exponentials of at most 1 in a word, the first in the lower half: a float's sign and upper exponent bit are 0 there, so
+// 16 bits hold its other 7 exponent bits and 9 of the fraction, two more than BF16 (rounded to nearest: off by 2^-10 of itself,
+// where BF16 is off by 2^-8; dz, which is made of them, is rounded to BF16 afterwards).  NaN becomes some number.
+__device__ __forceinline__ uint32_t xe_pack_exp(float lo, float hi) {
+    return __byte_perm((__float_as_uint(lo) << 2) + 0x8000u, (__float_as_uint(hi) << 2) + 0x8000u, 0x7632);
+}
+__device__ __forceinline__ float2 xe_unpack_exp(uint32_t w) {
+    return make_float2(__uint_as_float((w << 14) & 0x3fffc000u), __uint_as_float((w >> 2) & 0x3fffc000u));
 }
 
 // v = p0 + p1 + p2 with BF16 parts (each remainder is rounded to nearest, so three parts hold 24 bits).  A float that

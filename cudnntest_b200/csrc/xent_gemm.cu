@@ -525,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
                                 const uint32_t buf = next_buffer();
                                 uint32_t pk[32];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) pk[i] = pack_bf16(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
+                                for (int i = 0; i < 32; ++i) pk[i] = xe_pack_exp(z[64 * h + 2 * i], z[64 * h + 2 * i + 1]);
                                 stage64(pk, buf);
                                 store64(buf, wcol + h * 64, 0);
                             }

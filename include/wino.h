@@ -176,7 +176,8 @@ enum { WINO_MEAN = 0, WINO_SUM = 1, WINO_NONE = 2 };
 typedef struct wino_xent_desc {
     int n, d, v;               /* rows (0 allowed), features, classes                                               */
     int dtype;                 /* WINO_BF16: bfloat16 x, W, dx, dW; products exact, sums in FP32, dz rounded to bfloat16
-                                  for the two gradient products.  WINO_FP32X3: float tensors, every operand split into
+                                  for the two gradient products (without a bias, from 512 features on, the softmax that dz
+                                  is made of may have waited in 16 bits, off by 2^-10 of itself).  WINO_FP32X3: float tensors, every operand split into
                                   three bfloat16 parts, six partial products: FP32-level accuracy on tensor cores
                                   (values below 2^-110 lose the parts that BF16 cannot hold, under 2^-133)             */
     int has_bias;

@@ -151,3 +151,29 @@ def test_classifier_head_on_features_inside_wider_rows():
     assert torch.equal(a.loss(x, target), b.loss(x.clone(), target))
     for got, want in zip(a.loss_and_grad(x, target, need_dx=True), b.loss_and_grad(x.clone(), target, need_dx=True)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n,v,limit", [(512, 9000, 0), (500, 1003, 1 << 20), (512, 9001, 0)])
+@pytest.mark.parametrize("spread", [2.0, 16.0])
+def test_probabilities_kept_in_16_bits(n, v, limit, spread):
+    """BF16 without a bias: exp(z - maximum) waits in 16 bits for the rows' sums.  With x the identity dW is dz itself, one element each,
+    rounded once to BF16 (2^-8); what was kept before is off by at most 2^-10, the exponentials and the sum by 2^-14 together
+    (ex2 2^-22 each, |z - max| below 256 rounded to 2^-24 of itself, a sum of v terms in float pairs)."""
+    torch = _torch()
+    import cudnntest_b200 as cb
+    d = 512
+    x = torch.eye(n, d, dtype=torch.bfloat16, device="cuda")
+    w = (torch.randn((v, d), generator=torch.Generator().manual_seed(5)) * spread).to(torch.bfloat16).cuda()
+    target = torch.arange(n, device="cuda") * 7 % v
+    loss, dx, dw, _ = cb.LinearXent(n, d, v, reduction="sum", scratch_limit=limit).loss_and_grad(x, w, target)
+    p = torch.softmax(w[:, :n].double().t(), 1)
+    want = p.clone()
+    want[torch.arange(n, device="cuda"), target] -= 1
+    got = dw.double()[:, :n].t()
+    off = torch.ones_like(p, dtype=torch.bool)
+    off[torch.arange(n, device="cuda"), target] = False
+    err, tol = (got - want).abs(), p * (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -14) + 2.0 ** -124
+    assert (err <= tol)[off].all(), float((err / tol)[off].max())
+    # the target's own value comes from its logit in FP32
+    assert (err <= want.abs() * 2.0 ** -8 + p * 2.0 ** -14 + 2.0 ** -22)[~off].all()
+    assert (dw[:, n:] == 0).all()
