@@ -24,6 +24,7 @@
 
 #include "tcgen05.cuh"
 #include "xent.cuh"
+#include "xent_turns.cuh"
 
 namespace wino {
 
@@ -171,17 +172,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
 
     const unsigned pair = blockIdx.x / 2, npairs = gridDim.x / 2;
 
-    // The i-th unit of this pair, -1 after the last.  Units of the first product go round the pairs; the pairs that its last
-    // turn leaves out take `lead` units of the second product each in that time, the rest of which goes round all pairs.
-    const unsigned units0 = pp.prob[0].units, units1 = pp.prob[1].units, over = units0 % npairs;
-    const unsigned mine0 = units0 / npairs + (pair < over ? 1 : 0), ahead = over && pair >= over ? pp.lead : 0;
-    const unsigned base1 = over ? (npairs - over) * pp.lead : 0;
-    auto unit_at = [&](unsigned i) -> long long {
-        if (i < mine0) return pair + i * npairs;
-        i -= mine0;
-        const unsigned long long u = i < ahead ? pair - over + i * (npairs - over) : (unsigned long long)base1 + pair + (unsigned long long)(i - ahead) * npairs;
-        return u < units1 ? (long long)(units0 + u) : -1;
-    };
+    const unsigned units0 = pp.prob[0].units;
+    const XeTurns turns(units0, pp.prob[1].units, npairs, pp.lead, pair);
+    auto unit_at = [&](unsigned i) { return turns.at(i); };
 
     // work unit -> problem, part of the contraction (ring slots c0 ... c1), tile
     struct Unit { int sp, mp, nb, c0, c1; };
@@ -605,6 +598,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
     }
 }
 
+// CTA pairs of a launch
+unsigned launch_pairs(const XeParams& p) {
+    const long long total = (long long)p.prob[0].units + p.prob[1].units, most = sm_count() < 4 ? 1 : sm_count() / 2;
+    return (unsigned)(total < most ? total : most);
+}
+
 template <int EPI, int PLANES, int BN = XE_BN>
 int run(const XeParams& p, cudaStream_t st) {
     using L = XeSmem<EPI, PLANES, BN>;
@@ -617,10 +616,9 @@ int run(const XeParams& p, cudaStream_t st) {
         attr_err = cudaFuncSetAttribute(xe_gemm_kernel<EPI, PLANES, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL);
     });
     WINO_CUDA_CHECK(attr_err);
-    const long long total = (long long)p.prob[0].units + p.prob[1].units;
-    const long long most = sm_count() < 4 ? 1 : sm_count() / 2, pairs = total < most ? total : most;
+    const unsigned pairs = launch_pairs(p);
     count_launch();
-    WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES, BN>, dim3((unsigned)(2 * pairs)), dim3(XE_THREADS), L::TOTAL, st, true, p));
+    WINO_CUDA_CHECK(launch_kernel(xe_gemm_kernel<EPI, PLANES, BN>, dim3(2 * pairs), dim3(XE_THREADS), L::TOTAL, st, true, p));
     return WINO_OK;
 }
 
@@ -696,11 +694,7 @@ int xe_gemm(const XeProduct* prod, int count, cudaStream_t st) {
         // ring slots of a unit, and about six more for its epilogue; the product with the longer units goes first
         auto cost = [](const XeProblem& q) { return (double)q.kchunks / q.splits * q.pairs + 6.0; };
         if (cost(p.prob[0]) < cost(p.prob[1])) { const XeProblem t = p.prob[0]; p.prob[0] = p.prob[1]; p.prob[1] = t; }
-        const long long pairs = sm_count() < 4 ? 1 : sm_count() / 2, over = (long long)p.prob[0].units % pairs;
-        if (over) {
-            const long long lead = (long long)(cost(p.prob[0]) / cost(p.prob[1]) + 0.5), most = p.prob[1].units / (pairs - over);
-            p.lead = (int)(lead < most ? lead : most);
-        }
+        p.lead = (int)xe_turns_lead(p.prob[0].units, p.prob[1].units, launch_pairs(p), cost(p.prob[0]) / cost(p.prob[1]));
     }
     if ((rc = status_word(&p.status))) return rc;
     switch (prod[0].epi) {

@@ -213,3 +213,54 @@ def test_the_documented_c_example_compiles(tmp_path):
     r = subprocess.run([cc, "-std=c11", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(root, "include"), "example.c"], cwd=tmp_path,
                        capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stderr
+
+
+_TURNS = r"""
+#include <cstdio>
+#include <vector>
+#include "xent_turns.cuh"
+using namespace wino;
+int main() {
+    for (unsigned most : {1u, 2u, 7u, 74u})
+        for (unsigned u0 = 1; u0 <= 3 * most + 2; ++u0)
+            for (unsigned u1 = 0; u1 <= 3 * most + 2; ++u1)
+                for (double ratio : {1.0, 1.4, 2.0, 5.0}) {
+                    const unsigned total = u0 + u1, pairs = total < most ? total : most, lead = xe_turns_lead(u0, u1, pairs, ratio);
+                    std::vector<int> seen(total, 0);
+                    unsigned fewest = ~0u, longest = 0;
+                    for (unsigned p = 0; p < pairs; ++p) {
+                        const XeTurns t(u0, u1, pairs, lead, p);
+                        unsigned i = 0;
+                        long long last = -1;
+                        for (long long u; (u = t.at(i)) >= 0; ++i, last = u)
+                            if (u >= total || u <= last || seen[u]++) return printf("unit %lld of %u + %u on %u pairs\n", u, u0, u1, pairs), 1;
+                        if (t.at(i + 1) >= 0 || t.at(i + 1000) >= 0) return printf("a unit behind the last\n"), 1;
+                        if (i < fewest) fewest = i;
+                        if (i > longest) longest = i;
+                    }
+                    for (int s : seen)
+                        if (!s) return printf("a unit of %u + %u is missing\n", u0, u1), 1;
+                    /* nobody waits while another has two units to do */
+                    if (fewest == 0 || (total <= most && longest > 1)) return printf("%u + %u units on %u pairs: %u ... %u\n", u0, u1, pairs, fewest, longest), 1;
+                    /* without units taken ahead the shares differ by one at most */
+                    if (!lead && longest > fewest + 1) return printf("%u + %u units on %u pairs: %u ... %u\n", u0, u1, pairs, fewest, longest), 1;
+                }
+    return 0;
+}
+"""
+
+
+def test_two_products_share_the_pairs(tmp_path):
+    """Every unit of both products exactly once, in order, and no pair idle while another has two."""
+    import os
+    import shutil
+    import subprocess
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    csrc = os.path.join(os.path.dirname(cb.__file__), "csrc")
+    (tmp_path / "turns.cpp").write_text(_TURNS)
+    r = subprocess.run([cxx, "-std=c++17", "-O2", "-Wall", "-Werror", "-I", csrc, "turns.cpp", "-o", "turns"], cwd=tmp_path, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run(["./turns"], cwd=tmp_path, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout
