@@ -177,3 +177,22 @@ def test_probabilities_kept_in_16_bits(n, v, limit, spread):
     # the target's own value comes from its logit in FP32
     assert (err <= want.abs() * 2.0 ** -8 + p * 2.0 ** -14 + 2.0 ** -22)[~off].all()
     assert (dw[:, n:] == 0).all()
+
+
+@pytest.mark.parametrize("n,d,v,ldx,ldw", [(300, 200, 1100, 0, 0), (300, 201, 1100, 203, 202), (20, 200, 6000, 0, 0), (6000, 201, 20, 0, 0), (5, 513, 5000, 0, 0)])
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_floats_near_the_largest_float_on_tensor_cores(n, d, v, ldx, ldw, which):
+    """Floats that would round to BF16's infinity, in either matrix: split beforehand, or inside the products."""
+    torch = _torch()
+    c = Case(n, d, v, "fp32", seed=181, ldx=ldx, ldw=ldw)
+    large, other = (c.x, c.w) if which == "x" else (c.w, c.x)
+    far = torch.tensor([3.4e38, -3.4e38, 3.3961775e38, 1.0], device="cuda")
+    large[:, 0] = far[torch.arange(large.shape[0], device="cuda") % 4]
+    other[:, 0] = 2.0 ** -100 * (1 + (torch.arange(other.shape[0], device="cuda") % 64) / 64)
+    ref = c.oracle("none")
+    assert np.abs(ref["z"]).max() > 2.0 ** 27
+    loss, lse = c.plan(reduction="none", grad=False).forward(c.x, c.w, c.target, c.bias)
+    ez, el, _ = c.z_error(ref)
+    assert (np.abs(lse.double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
+    row = el + ez.max(1) + 8 * F32 * (np.abs(ref["z"]).max(1) + np.abs(ref["lse"]))
+    assert (np.abs(loss.double().cpu().numpy() - ref["loss"]) <= row).all()
