@@ -1240,10 +1240,12 @@ int build_plan(const wino_xent_desc* d, bool grad, Plan* out) {
     // 25.2 / 46.7, 128 x 2048 x 20000 84 / 208; gradient of 64 x 512 x 1000 34.9 / 30.8, 64 x 4096 x 300 43.0 / 44.0, 64 x 2048 x 1000
     // 39.8 / 45.1, 64 x 2048 x 20000 207 / 322.  A tile of 128 rows takes the products apart that one launch would share:
     // gradient of 128 x 512 x 20000 137 / 132, 128 x 2048 x 20000 232 / 382.  With few classes the same: loss of 8000 x 2048 x 64
-    // 45.4 / 81.9; gradient of 4000 x 512 x 16 51.3 / 55.4, 8000 x 512 x 64 67.6 / 67.6, 4000 x 2048 x 128 100 / 94, 8000 x 2048 x 128 146 / 157.
+    // 45.4 / 81.9; gradient of 4000 x 512 x 16 51.3 / 55.4, 8000 x 512 x 64 67.6 / 67.6, 4000 x 2048 x 128 100 / 94, 8000 x 2048 x 128 144 / 155.
+    // Between them, near the threshold of 12M elements: 128 x 512 x 25000 143 / 153, 128 x 2048 x 6400 109 / 129, 6200 x 2048 x 128 127 / 128,
+    // 25000 x 512 x 128 164 / 157.
     p.thin_rows = n <= 128 && (v > 128 || v >= n);
     const long long thin_n = p.thin_rows ? n : v, thin_m = p.thin_rows ? v : n;
-    p.thin = !bf16 && !p.small && !p.few && n > 0 && thin_n <= 128 && thin_m * d->d >= (grad && thin_n > 64 ? 16ll << 20 : 1ll << 20);
+    p.thin = !bf16 && !p.small && !p.few && n > 0 && thin_n <= 128 && thin_m * d->d >= (grad && thin_n > 64 ? 12ll << 20 : 1ll << 20);
     if (p.thin) {
         p.thin_z = xe_thin_cut((thin_m + 127) / 128, kd, (double)n * v * 8.0 / 5e6);
         p.thin_grad = xe_thin_cut(col_tiles, (thin_m + XE_BK - 1) / XE_BK, (double)thin_n * d->d * 8.0 / 5e6);

@@ -264,3 +264,11 @@ def test_two_products_share_the_pairs(tmp_path):
     assert r.returncode == 0, r.stderr
     r = subprocess.run(["./turns"], cwd=tmp_path, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout
+
+
+def test_measured_sizes_split_inside_the_products():
+    """Gradients of more than 64 rows or classes, on the side that was measured faster: split beforehand, the longer matrix alone takes
+    six bytes an element of scratch."""
+    for n, d, v, inside in ((8000, 2048, 128, True), (128, 2048, 20000, True), (4000, 2048, 128, False), (128, 512, 20000, False)):
+        got = cb.LinearXent(n, d, v, dtype="fp32x3", bias=True, device="meta")
+        assert (_bytes(got, 1) < max(n, v) * d * 6) == inside, (n, d, v)
