@@ -253,7 +253,7 @@ int wino_device_status(void) {
     int s = 0;
     if ((rc = read_and_clear_status(&s))) return rc;
     if (s == 100) return fail(WINO_E_BADARG, "xent: a target was neither a class nor the ignored index");
-    if (s != 0) return fail(WINO_E_TIMEOUT, "a CTA gave up a bounded wait (code %d: tile GEMM 1 ring slot free, 2 ring slot filled, 3 accumulator drained, 4 accumulator ready; 5, 6 input-transform patch load; 1x row-fused GEMM, 2x CTA-pair GEMM, 4x direct convolution, 5x cross entropy, 90 self-test)", s);
+    if (s != 0) return fail(WINO_E_TIMEOUT, "a CTA gave up a bounded wait (code %d: tile GEMM 1 ring slot free, 2 ring slot filled, 3 accumulator drained, 4 accumulator ready; 5, 6 input-transform patch load; 1x row-fused GEMM, 2x CTA-pair GEMM, 4x direct convolution, 5x cross entropy, 6x its products that split a float matrix, 90 self-test)", s);
     return WINO_OK;
 }
 

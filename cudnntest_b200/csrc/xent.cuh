@@ -34,7 +34,10 @@ __device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t saddr) {
 }
 
 // what a wait that ran out was for
-enum XeWaitCode { XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54 };
+enum XeWaitCode {
+    XE_WAIT_EMPTY = 51, XE_WAIT_FULL = 52, XE_WAIT_TMEM_EMPTY = 53, XE_WAIT_TMEM_FULL = 54,        // xent_gemm.cu
+    XT_WAIT_EMPTY = 61, XT_WAIT_FULL = 62, XT_WAIT_TMEM_EMPTY = 63, XT_WAIT_TMEM_FULL = 64,        // xent_thin.cu
+};
 
 // What the epilogue does with a 256 x 256 tile of the product (m rows x n columns)
 enum XeEpilogue {

@@ -199,7 +199,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
         uint32_t phase = 0;
         bool ok = true;
         long long u;
-            for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
+        for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
             Unit w;
             const XeProblem& p = decode(u, w);
             if (i == 0) pdl_wait();        // all of the above ran under the predecessor; now its results are read
@@ -301,7 +301,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1) xe_ge
             return buf;
         };
         long long u;
-            for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
+        for (unsigned i = 0; ok && (u = unit_at(i)) >= 0; ++i) {
             Unit w;
             const XeProblem& p = decode(u, w);
             const long long row0 = (long long)(w.mp * 2 + (int)rank) * 128 + quarter * 32;

@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) xe_thin_kernel(const __grid_con
                 const Piece w = piece_at(g);
                 g = w.next;
                 for (int c = w.c0; c < w.c1; ++c) {
-                    if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XE_WAIT_EMPTY)) { ok = false; break; }
+                    if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XT_WAIT_EMPTY)) { ok = false; break; }
                     if (issuer) {
                         const uint32_t bar = bar_full + 8 * stage, dst = base + stage * L::STAGE + 3 * XT_TILE;
                         mbar_arrive_expect_tx(bar, 3 * L::S_BYTES);
@@ -168,11 +168,11 @@ __global__ void __launch_bounds__(XT_THREADS, 1) xe_thin_kernel(const __grid_con
                 g = w.next;
                 for (int cb = w.c0; ok && cb < w.c1; cb += XT_BLOCK) {
                     const int steps = w.c1 - cb < XT_BLOCK ? w.c1 - cb : XT_BLOCK;
-                    if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XE_WAIT_TMEM_EMPTY)) { ok = false; break; }
+                    if (!mbar_wait_warp(bar_tempty + 8 * as, aphase ^ 1, abort_flag, p.status, XT_WAIT_TMEM_EMPTY)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t large = tmem_base + (uint32_t)(as * 2 * NP), small = large + NP;
                     for (int c = 0; c < steps; ++c) {
-                        if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XE_WAIT_FULL)) { ok = false; break; }
+                        if (!mbar_wait_warp(bar_full + 8 * stage, phase, abort_flag, p.status, XT_WAIT_FULL)) { ok = false; break; }
                         tc_fence_after();
                         const uint64_t ld = l0 + (uint64_t)(stage * (L::STAGE >> 4)), sd = s0 + (uint64_t)(stage * (L::STAGE >> 4));
                         constexpr int pl[6] = {2, 1, 0, 1, 0, 0}, ps[6] = {0, 1, 2, 0, 1, 0};
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) xe_thin_kernel(const __grid_con
             }
         };
         auto put = [&](const float (&v)[32]) {
-            if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XE_WAIT_EMPTY)) return false;
+            if (!mbar_wait_warp(bar_empty + 8 * stage, phase ^ 1, abort_flag, p.status, XT_WAIT_EMPTY)) return false;
             store(v);
             fence_async_shared();
             __syncwarp();
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) xe_thin_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < COLS; ++i) z[i] = 0.f;
             for (int cb = w.c0; cb < w.c1; cb += XT_BLOCK) {
-                if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XE_WAIT_TMEM_FULL)) { ok = false; break; }
+                if (!mbar_wait_warp(bar_tfull + 8 * as, aphase, abort_flag, p.status, XT_WAIT_TMEM_FULL)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t src = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(as * 2 * NP + half * COLS);
 #pragma unroll

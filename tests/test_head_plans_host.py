@@ -272,3 +272,19 @@ def test_measured_sizes_split_inside_the_products():
     for n, d, v, inside in ((8000, 2048, 128, True), (128, 2048, 20000, True), (4000, 2048, 128, False), (128, 512, 20000, False)):
         got = cb.LinearXent(n, d, v, dtype="fp32x3", bias=True, device="meta")
         assert (_bytes(got, 1) < max(n, v) * d * 6) == inside, (n, d, v)
+
+
+def test_wait_codes_name_their_kernel():
+    """A wait that ran out reports a code that one kernel alone uses."""
+    import glob
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(cb.__file__), "csrc")
+    values = {}
+    for path in glob.glob(os.path.join(csrc, "xent*.cu*")):
+        values.update((name, int(code)) for name, code in re.findall(r"(X[ET]_WAIT_\w+) = (\d+)", open(path).read()))
+    used = {}
+    for name in ("xent_gemm.cu", "xent_thin.cu"):
+        used[name] = {values[code] for code in re.findall(r"X[ET]_WAIT_\w+", open(os.path.join(csrc, name)).read())}
+        assert len(used[name]) == 4
+    assert not used["xent_gemm.cu"] & used["xent_thin.cu"]
