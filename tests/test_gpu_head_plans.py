@@ -196,3 +196,39 @@ def test_floats_near_the_largest_float_on_tensor_cores(n, d, v, ldx, ldw, which)
     assert (np.abs(lse.double().cpu().numpy() - ref["lse"]) <= el + 2 * F32 * np.abs(ref["lse"])).all()
     row = el + ez.max(1) + 8 * F32 * (np.abs(ref["z"]).max(1) + np.abs(ref["lse"]))
     assert (np.abs(loss.double().cpu().numpy() - ref["loss"]) <= row).all()
+
+
+@pytest.mark.parametrize("bias,limit", [(False, 8 << 30), (True, 20 << 30), (True, 0)])
+def test_more_than_2_31_logits(bias, limit):
+    """Offsets past 32 bits in kept exponentials, kept floats and pieces: some rows of dx, some classes of dW, against 64 bits.
+
+    dz is off by its own rounding (2^-8), by that of a kept exponential (2^-10) and by less than 2^-12 in the exponentials, the sums and
+    the products; the result by one rounding more."""
+    torch = _torch()
+    import cudnntest_b200 as cb
+    n, d, v = 40000, 1024, 60001
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((n, d), generator=gen, device="cuda").relu_().to(torch.bfloat16)
+    w = (torch.randn((v, d), generator=gen, device="cuda") * 2 / (0.5 * d) ** 0.5).to(torch.bfloat16)
+    b = torch.randn(v, generator=gen, device="cuda") if bias else None
+    target = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    target[-1] = v - 1
+    plan = cb.LinearXent(n, d, v, bias=bias, reduction="sum", scratch_limit=limit)
+    loss, dx, dw, db = plan.loss_and_grad(x, w, target, b)
+    lse = plan.forward(x, w, target, b)[1].double()
+    dz_eps = 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -12
+
+    def check(got, want, mag):
+        assert ((got.double() - want).abs() <= mag * dz_eps + want.abs() * 2.0 ** -8).all(), ((got.double() - want).abs() / mag).max()
+    rows = torch.tensor([0, 1, 17777, 35791, 35792, n - 2, n - 1], device="cuda")
+    z = x[rows].double() @ w.double().t() + (b.double() if bias else 0)
+    assert ((lse[rows] - torch.logsumexp(z, 1)).abs() <= 2.0 ** -14).all()
+    dz = torch.softmax(z, 1)
+    dz[torch.arange(len(rows), device="cuda"), target[rows]] -= 1
+    check(dx[rows], dz @ w.double(), dz.abs() @ w.double().abs())
+    classes = torch.cat([torch.tensor([0, 1, 30000, 53687, v - 2, v - 1], device="cuda"), target[[0, n // 2, n - 1]]])
+    zt = x.double() @ w[classes].double().t() + (b[classes].double() if bias else 0)
+    dz = torch.exp(zt - lse[:, None]) - (target[:, None] == classes).double()
+    check(dw[classes], dz.t() @ x.double(), dz.abs().t() @ x.double().abs())
+    if bias:
+        assert ((db[classes].double() - dz.sum(0)).abs() <= dz.abs().sum(0) * 2.0 ** -12).all()
