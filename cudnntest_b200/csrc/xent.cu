@@ -1,6 +1,6 @@
 // Linear softmax cross entropy with its gradient: driver and row kernels (the products are in xent_gemm.cu and xent_thin.cu).
 //
-// The logits z = x W^T are never a tensor of the caller's.  Ways, by size (build_plan):
+// The logits z = x W^T exist in the workspace at most, as far as desc.scratch_limit allows.  Ways, by size (build_plan):
 //   * few products, few rows, few classes: FP32 kernels on the caller's matrices (xe_tiny_kernel, xe_small_*, xe_few_*);
 //   * kept: where rows or classes are few the logits product is split along the features until the GPU is full; its
 //     float parts in the scratch become lse, loss and dz in row kernels.  Unsplit, floats are kept as well where that is

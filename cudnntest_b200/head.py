@@ -80,8 +80,8 @@ def dropout_backward(dy, p, seed, offset=0, offset_dev=None, out=None):
 
 
 class LinearXent:
-    """loss = cross entropy of softmax(x W^T + bias) against class numbers, and its gradient, without an (n, v) tensor of
-    logits in the caller's memory.
+    """loss = cross entropy of softmax(x W^T + bias) against class numbers, and its gradient, in one call; an (n, v) matrix
+    exists at most in the scratch, as far as ``scratch_limit`` (0: 1 GiB) allows.
 
     x: (n, d), w: (v, d), both bfloat16 (dtype "bf16") or both float32 (dtype "fp32x3": operands split into three
     bfloat16 parts, FP32-level accuracy); bias: v float32; target: n int64.  reduction "mean" (over the rows that count),

@@ -165,21 +165,24 @@ int wino_dropout_backward(int dtype, long long rows, long long cols, long long l
                           unsigned long long seed, unsigned long long offset, const unsigned long long* offset_dev,
                           const void* dy, void* dx, wino_stream_t stream);
 
-/* Softmax cross entropy of a linear layer, z = x W^T + bias, without an (n, v) tensor of logits in the caller's memory:
+/* Softmax cross entropy of a linear layer, z = x W^T + bias, in one call: an (n, v) matrix (of logits, exponentials or
+ * dz) exists in the workspace at most, and there only as far as scratch_limit allows:
  *   lse_i = log sum_j exp z_ij,   loss_i = lse_i - (1 - s) z_i,t(i) - s/v sum_j z_ij        (s = label_smoothing)
  *   dz_ij = g_i (exp(z_ij - lse_i) - (1 - s) [j = t(i)] - s/v),  dx = dz W,  dW = dz^T x,  dbias = sum_i dz_i
  * x (n, d), W (v, d), dx, dW: row-major with pitches ldx, ldw, lddx, lddw; bias, dbias: v floats; target: n 64-bit
- * integers.  WINO_MEAN divides by the number of rows that count (0 rows: loss and gradients are 0).  The tensors live on the
- * current device; results overlap neither inputs nor each other.  Calls with the same workspace are kept on one stream or
- * otherwise serialised; the first call on a device comes before any stream capture. */
+ * integers.  WINO_MEAN divides by the number of rows that count (0 rows: loss and gradients are 0).  All tensors, loss among
+ * them, live in the memory of the current device; results overlap neither inputs nor each other.  Calls with the same
+ * workspace are kept on one stream or otherwise serialised; the first call on a device comes before any stream capture. */
 enum { WINO_MEAN = 0, WINO_SUM = 1, WINO_NONE = 2 };
 typedef struct wino_xent_desc {
     int n, d, v;               /* rows (0 allowed), features, classes                                               */
     int dtype;                 /* WINO_BF16: bfloat16 x, W, dx, dW; products exact, sums in FP32, dz rounded to bfloat16
                                   for the two gradient products (without a bias, from 512 features on, the softmax that dz
-                                  is made of may have waited in 16 bits, off by 2^-10 of itself).  WINO_FP32X3: float tensors, every operand split into
-                                  three bfloat16 parts, six partial products: FP32-level accuracy on tensor cores
-                                  (values below 2^-110 lose the parts that BF16 cannot hold, under 2^-133)             */
+                                  is made of may have waited in 16 bits, off by 2^-10 of itself).  WINO_FP32X3: float
+                                  tensors, every operand split into three bfloat16 parts, six partial products: FP32-level
+                                  accuracy on tensor cores
+                                  (values below 2^-110 lose the parts that BF16 cannot hold, under 2^-133; an infinity in x
+                                  or W may make its rows NaN: mask classes by the bias)                                */
     int has_bias;
     int reduction;             /* WINO_MEAN, WINO_SUM: one float of loss; WINO_NONE: n floats                       */
     int has_ignore;            /* rows with target == ignore_index leave no trace: loss_i = lse_i = 0, dx_i = 0, and
@@ -188,8 +191,10 @@ typedef struct wino_xent_desc {
     float label_smoothing;     /* 0 ... 1                                                                           */
     long long ldx, ldw, lddx, lddw;   /* pitches in elements, 0 = d.  Base addresses: 16-byte aligned               */
     long long scratch_limit;   /* bytes of scratch that may grow with n * v, beside the statistics of the logits (n v / 16
-                                  bytes, n v 3 / 32 with label_smoothing); 0 = 1 GiB.  Beyond it the gradient is computed in
-                                  pieces of the vocabulary (at least 256 classes each) whose logits are computed again      */
+                                  bytes, n v 3 / 32 with label_smoothing); 0 = 1 GiB.  More of it saves time: within it
+                                  the logits (or their exponentials) and dz of all classes are kept.  Beyond it the
+                                  gradient is computed in pieces of the vocabulary (at least 256 classes each) whose logits
+                                  are computed again.  Another limit may give other last bits                           */
 } wino_xent_desc;
 
 /* Scratch of wino_xent_forward (grad = 0) or wino_xent_grad (grad = 1); 0 for a bad descriptor. */
@@ -199,8 +204,8 @@ int wino_xent_forward(const wino_xent_desc* d, const void* x, const void* w, con
                       float* loss, float* lse, void* workspace, size_t workspace_bytes, wino_stream_t stream);
 /* loss (and lse unless NULL) and the gradients in one call.  dloss: upstream gradient, one float (WINO_MEAN, WINO_SUM) or
  * n floats (WINO_NONE) on the device, NULL = 1.  dx, dw, dbias: NULL where not wanted.  A target outside 0 ... v-1 that is
- * not ignored makes its row's loss NaN, keeps the row out of the gradients, and the next wino_device_status() returns
- * WINO_E_BADARG (wino_xent_forward likewise).  Results are deterministic (no atomics on results). */
+ * not ignored makes its row's loss NaN, keeps the row (if x_i is finite) out of the gradients, and the next
+ * wino_device_status() returns WINO_E_BADARG (wino_xent_forward likewise).  Results are deterministic (no atomics on results). */
 int wino_xent_grad(const wino_xent_desc* d, const void* x, const void* w, const float* bias, const long long* target,
                    const float* dloss, float* loss, float* lse, void* dx, void* dw, float* dbias, void* workspace,
                    size_t workspace_bytes, wino_stream_t stream);
