@@ -90,17 +90,19 @@ def test_plan_dropped_while_a_side_stream_uses_it(grad):
     at, size = plan.workspace.data_ptr(), plan.workspace.numel()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(200_000_000)                            # about a tenth of a second
+        torch.cuda._sleep(800_000_000)                            # less than half a second
         got = call()
     del plan
     others = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
     early = not side.query()
-    if early:                                                     # else the host was held up, and nothing can be said
+    if early:
         assert all(o.data_ptr() + size <= at or at + size <= o.data_ptr() for o in others)
     for o in others:
         o.fill_(255)
     side.synchronize()
-    assert early and all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if not early:
+        pytest.skip("the host was held up until the call was over: nothing to see")
 
 
 def test_classifier_head_of_no_images():
